@@ -19,9 +19,11 @@
 
 #include "fa_attn.h"
 #include "fa_fmha_launch.h"
+#include "fa_host.h"
 #include "fa_launch.cuh"
 #include "fa_decode_tc.h"
 #include "fa_relpos.h"
+#include "fa_paged.h"
 #include "fa_peer.h"
 
 namespace {
@@ -252,6 +254,39 @@ int check_ptr(const void* ptr, int device, const char* what) {
   if (attr.type == cudaMemoryTypeHost && attr.devicePointer != nullptr) return FA_OK;
   return fail(FA_ERR_ARG, "%s is pageable host memory; device memory is needed here", what);
 }
+
+}  // namespace
+
+// The parts of the above that the ABI's other translation units use (fa_host.h).
+namespace fa {
+namespace host {
+
+int fail(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  g_last_error = buf;
+  return code;
+}
+
+int cuda_fail(cudaError_t e, const char* what) { return ::cuda_fail(e, what); }
+
+int device_info(int device, int* sms, unsigned** err) {
+  Device* dev = nullptr;
+  if (int rc = device_state(device, &dev)) return rc;
+  *sms = dev->sms;
+  *err = dev->err;
+  return FA_OK;
+}
+
+int pointer_on(const void* ptr, int device, const char* what) { return check_ptr(ptr, device, what); }
+
+}  // namespace host
+}  // namespace fa
+
+namespace {
 
 #define FA_PTR(ptr, device) \
   do {                      \
@@ -861,7 +896,7 @@ const char* fa_last_error(void) { return g_last_error.c_str(); }
 int fa_capabilities(int32_t* flags, int32_t* head_dims, int32_t max_head_dims,
                     int32_t* n_head_dims) {
   static const int32_t dims[] = {16, 32, 64, 128, 256};
-  if (flags) *flags = 1 | 2 | (fa::fmha_supported(1, 128) ? 4 : 0) | 8;
+  if (flags) *flags = 1 | 2 | (fa::fmha_supported(1, 128) ? 4 : 0) | 8 | 16;
   const int n = int(sizeof dims / sizeof dims[0]);
   if (head_dims)
     for (int i = 0; i < n && i < max_head_dims; ++i) head_dims[i] = dims[i];
@@ -2368,8 +2403,13 @@ int fa_device_status(void* stream) {
   FA_CUDA(cudaMemcpy(&word, dev->err, sizeof word, cudaMemcpyDeviceToHost), "read error word");
   if (word != 0) {
     FA_CUDA(cudaMemset(dev->err, 0, sizeof word), "clear error word");
-    dev->epoch.fetch_add(1);
-    return fail(FA_ERR_TIMEOUT, "a device-side wait gave up (error word 0x%x)", word);
+    if (word & fa::kErrTimeout) {
+      dev->epoch.fetch_add(1);
+      return fail(FA_ERR_TIMEOUT, "a device-side wait gave up (error word 0x%x)", word);
+    }
+    if (word & fa::kErrPagedSpan)
+      return fail(FA_ERR_CAPACITY, "a paged call's row_starts, firsts or positions were out of range");
+    return fail(FA_ERR_ARG, "a paged call's tables named a page out of range");
   }
   return FA_OK;
 }

@@ -1,0 +1,350 @@
+// Rows into pages and back: head norm, RoPE and the 8-bit quantisation of a call's keys and
+// values as they are written (PagedWriteArgs), and the rows read back out (PagedReadArgs).
+//
+// 8-bit pages: with a = max|x_e| over a head's elements, scale = a / 127 and q_e = round(x_e *
+// (127 / a)) to the nearest even, in f32: |x_e - q_e scale| <= scale / 2. A head below 2^-100
+// everywhere is kept as zeros (127 / a must not overflow), and one with an infinity or a NaN as
+// a NaN scale (it reads back as NaN throughout, and attends as NaN where it is seen).
+#include <cuda_bf16.h>
+
+#include "fa_paged.h"
+#include "fa_ptx.cuh"
+
+namespace fa {
+
+namespace {
+
+constexpr int kRowWarps = 8;
+
+// The sequence that holds row r: the number of sequences that end at or before it (one warp;
+// row_starts rises, or the span check refuses what is found). Up to 32 sequences take one load,
+// up to 1024 two.
+__device__ __forceinline__ int sequence_of(const PagedSpans& b, int r, int lane) {
+  int base = 0;
+  if (b.sequences > 32) {
+    const int at = (lane + 1) * 32;  // the end of block `lane` of 32 sequences
+    const bool past = at <= b.sequences && b.row_starts[at] <= r;
+    base = 32 * __popc(__ballot_sync(0xffffffffu, past));
+  }
+  const int at = base + lane + 1;
+  const bool past = at <= b.sequences && b.row_starts[at] <= r;
+  return base + __popc(__ballot_sync(0xffffffffu, past));
+}
+
+// Row r's place: its page and slot and its sequence's span, or false (with the error word set)
+// if the batch's numbers are out of range. Rows past the last sequence's are left alone.
+__device__ __forceinline__ bool place_of(const PagedSpans& b, const PagedPool& pool, int r,
+                                         int lane, int* page, int* slot, unsigned* err) {
+  const int s = sequence_of(b, r, lane);
+  if (s >= b.sequences) return false;
+  PagedSpan span;
+  const bool ok = paged_span(b, pool.page_shift, s, &span);
+  if (!ok || r < span.row0 || r >= span.row0 + span.n) {
+    if (lane == 0) atomicOr(err, kErrPagedSpan);
+    return false;
+  }
+  const int pos = span.first + (r - span.row0);
+  *page = b.tables[int64_t(s) * b.table_stride + (pos >> pool.page_shift)];
+  *slot = pos & ((1 << pool.page_shift) - 1);
+  if (!paged_page_ok(*page, pool.pages)) {
+    if (lane == 0) atomicOr(err, kErrPagedPage);
+    return false;
+  }
+  return true;
+}
+
+// E consecutive elements as f32: one vector load where the row is aligned for it.
+template <typename T, int E>
+__device__ __forceinline__ void load_elems(const T* p, bool vec, float (&x)[E]) {
+  if (vec) {
+    constexpr int B = E * int(sizeof(T));
+    alignas(16) T raw[E];
+    if constexpr (B == 4) *reinterpret_cast<uint32_t*>(raw) = __ldcs(reinterpret_cast<const unsigned int*>(p));
+    else if constexpr (B == 8) *reinterpret_cast<uint2*>(raw) = __ldcs(reinterpret_cast<const uint2*>(p));
+    else {
+#pragma unroll
+      for (int i = 0; i < B / 16; ++i)
+        reinterpret_cast<uint4*>(raw)[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = float(raw[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = float(p[e]);
+  }
+}
+
+template <int E>
+__device__ __forceinline__ void store_elems(void* base, int64_t at, bool bf16, bool vec,
+                                            const float (&x)[E]) {
+  if (bf16) {
+    __nv_bfloat16* p = static_cast<__nv_bfloat16*>(base) + at;
+    if (vec) {
+      alignas(16) __nv_bfloat162 raw[E / 2];
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) raw[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+      if constexpr (E == 2) *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<uint32_t*>(raw);
+      else if constexpr (E == 4) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(raw);
+      else *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(raw);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) p[e] = __float2bfloat16_rn(x[e]);
+    }
+  } else {
+    float* p = static_cast<float*>(base) + at;
+    if (vec) {
+      if constexpr (E == 2) *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
+      else {
+#pragma unroll
+        for (int e = 0; e < E / 4; ++e)
+          reinterpret_cast<float4*>(p)[e] =
+              make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) p[e] = x[e];
+    }
+  }
+}
+
+// A head's row kept in its page: E elements a lane, quantised over the warp for 8-bit pages.
+template <int E>
+__device__ __forceinline__ void keep_head(const PagedPool& pool, bool is_key, int page, int kv,
+                                          int slot, int lane, const float (&x)[E]) {
+  const int64_t row = ((int64_t(page) * pool.kv_heads + kv) << pool.page_shift) + slot;
+  unsigned char* base = is_key ? pool.keys : pool.values;
+  if (!pool.q8) {
+    store_elems<E>(base, row * (32 * E) + lane * E, true, true, x);
+    return;
+  }
+  float top = 0.0f;
+  bool finite = true;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    top = fmaxf(top, fabsf(x[e]));
+    finite = finite && fabsf(x[e]) <= 3.402823466e38f;
+  }
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  finite = __all_sync(0xffffffffu, finite);
+  const bool live = finite && top >= 7.888609052e-31f;  // 2^-100
+  const float inverse = live ? __fdiv_rn(127.0f, top) : 0.0f;
+  const float scale = !finite ? __int_as_float(0x7fffffff) : live ? __fdiv_rn(top, 127.0f) : 0.0f;
+  alignas(8) signed char q[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float y = finite ? __fmul_rn(x[e], inverse) : 0.0f;
+    q[e] = static_cast<signed char>(max(-127, min(127, __float2int_rn(y))));
+  }
+  unsigned char* p = base + row * (32 * E) + lane * E;
+  if constexpr (E == 2) *reinterpret_cast<uint16_t*>(p) = *reinterpret_cast<uint16_t*>(q);
+  else if constexpr (E == 4) *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<uint32_t*>(q);
+  else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(q);
+  if (lane == 0) (is_key ? pool.key_scales : pool.value_scales)[row] = scale;
+}
+
+// One CTA per row; a warp takes every kRowWarps-th head unit (query heads, key heads, value
+// heads), two at a time so that their loads are in flight together. Lane l holds elements lE ..
+// lE + E - 1 of a head: RoPE by halves finds the partner of e in lane l ^ 16, interleaved RoPE
+// within the lane, and the row's cosines and sines are loaded once for all of the warp's heads.
+// Arithmetic of the rotation: each product rounded, then the difference or sum (ops.rs:77-95).
+template <typename T, int D>
+__global__ void __launch_bounds__(kRowWarps * 32)
+    paged_write_kernel(const __grid_constant__ PagedWriteArgs a) {
+  constexpr int E = D / 32;
+  constexpr int U = 2;
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r = blockIdx.x;
+  const int kvh = a.pool.kv_heads;
+  const int units = a.heads + 2 * kvh;
+  int page, slot;
+  if (!place_of(a.spans, a.pool, r, lane, &page, &slot, a.err)) return;  // the warp's, as one
+  float c[E], s[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) c[e] = s[e] = 0.0f;
+  if (a.rope == 1) {
+    const float* cs = a.angles + int64_t(r) * D + (lane & 15) * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) { c[e] = cs[e]; s[e] = cs[D / 2 + e]; }
+  } else if (a.rope == 2) {
+    const float* cs = a.angles + int64_t(r) * D + lane * (E / 2);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) { c[e] = cs[e]; s[e] = cs[D / 2 + e]; }
+  }
+  for (int u0 = warp; u0 < units; u0 += U * kRowWarps) {
+    float xs[U][E];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = u0 + i * kRowWarps;
+      if (u >= units || (u < a.heads && a.q_out == nullptr)) continue;
+      const T* p;
+      if (u < a.heads)
+        p = static_cast<const T*>(a.q) + int64_t(r) * a.q_stride + int64_t(u) * D;
+      else if (u < a.heads + kvh)
+        p = static_cast<const T*>(a.k) + int64_t(r) * a.k_stride + int64_t(u - a.heads) * a.k_head_stride;
+      else
+        p = static_cast<const T*>(a.v) + int64_t(r) * a.v_stride +
+            int64_t(u - a.heads - kvh) * a.v_head_stride;
+      load_elems<T, E>(p + lane * E, a.vec != 0, xs[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = u0 + i * kRowWarps;
+      if (u >= units || (u < a.heads && a.q_out == nullptr)) continue;
+      float(&x)[E] = xs[i];
+      const bool is_query = u < a.heads, is_key = !is_query && u < a.heads + kvh;
+      if (is_query || is_key) {
+        const float* weight = is_query ? a.q_norm : a.k_norm;
+        if (weight != nullptr) {
+          float ss = 0.0f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) ss = fmaf(x[e], x[e], ss);
+#pragma unroll
+          for (int off = 16; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+          const float inverse = 1.0f / sqrtf(ss / float(D) + a.eps);
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            x[e] = __fmul_rn(__fmul_rn(x[e], inverse), weight[lane * E + e]);
+        }
+        if (a.rope == 1) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const float o = __shfl_xor_sync(0xffffffffu, x[e], 16);
+            const float xc = __fmul_rn(x[e], c[e]), os = __fmul_rn(o, s[e]);
+            x[e] = lane < 16 ? __fsub_rn(xc, os) : __fadd_rn(xc, os);
+          }
+        } else if (a.rope == 2) {
+#pragma unroll
+          for (int e = 0; e < E / 2; ++e) {
+            const float y0 = x[2 * e], y1 = x[2 * e + 1];
+            x[2 * e] = __fsub_rn(__fmul_rn(y0, c[e]), __fmul_rn(y1, s[e]));
+            x[2 * e + 1] = __fadd_rn(__fmul_rn(y1, c[e]), __fmul_rn(y0, s[e]));
+          }
+        }
+      }
+      if (is_query)
+        store_elems<E>(a.q_out, int64_t(r) * a.q_out_stride + int64_t(u) * D + lane * E,
+                       a.q_out_bf16 != 0, a.q_out_vec != 0, x);
+      else
+        keep_head<E>(a.pool, is_key, page, is_key ? u - a.heads : u - a.heads - kvh, slot, lane, x);
+    }
+  }
+}
+
+// 16 rows a CTA: their places once, then every thread 16 bytes of a page's row at a time (keys
+// and values), four such loads in flight.
+constexpr int kReadRows = 16;
+
+__global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__ PagedReadArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ int64_t place[kReadRows];  // (page, slot)'s row of KV head 0, or -1
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r0 = blockIdx.x * kReadRows;
+  for (int i = warp; i < kReadRows; i += 8) {
+    int page = 0, slot = 0;
+    const bool ok = r0 + i < a.spans.rows &&
+                    place_of(a.spans, a.pool, r0 + i, lane, &page, &slot, a.err);
+    if (lane == 0)
+      place[i] = ok ? ((int64_t(page) * a.pool.kv_heads) << a.pool.page_shift) + slot : -1;
+  }
+  __syncthreads();
+  const int d = a.pool.head_dim;
+  const int elems = a.pool.q8 ? 16 : 8;  // of a 16-byte vector
+  const int per_head = d / elems, per_row = per_head * a.pool.kv_heads;
+  const int items = kReadRows * per_row * 2;
+  constexpr int U = 4;
+  for (int i0 = threadIdx.x; i0 < items; i0 += 256 * U) {
+    uint4 raw[U];
+    float scale[U];
+    int64_t to[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * 256;
+      to[u] = -1;
+      if (i >= items) continue;
+      const int c = i % per_head, rest = i / per_head;
+      const int h = rest % a.pool.kv_heads, row = (rest / a.pool.kv_heads) % kReadRows;
+      const bool is_key = rest / a.pool.kv_heads < kReadRows;
+      if (place[row] < 0) continue;
+      const int64_t at = place[row] + (int64_t(h) << a.pool.page_shift);
+      const unsigned char* base = is_key ? a.pool.keys : a.pool.values;
+      raw[u] = __ldcs(reinterpret_cast<const uint4*>(base) + at * per_head + c);
+      scale[u] = a.pool.q8 ? (is_key ? a.pool.key_scales : a.pool.value_scales)[at] : 1.0f;
+      to[u] = int64_t(r0 + row) * (is_key ? a.k_stride : a.v_stride) +
+              int64_t(h) * (is_key ? a.k_head_stride : a.v_head_stride) + c * elems;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (to[u] < 0) continue;
+      const int i = i0 + u * 256;
+      const bool is_key = i / per_head / a.pool.kv_heads < kReadRows;
+      void* out = is_key ? a.k : a.v;
+      if (a.pool.q8) {
+        const signed char* q = reinterpret_cast<const signed char*>(&raw[u]);
+        float x[8], y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = float(q[e]) * scale[u];
+          y[e] = float(q[8 + e]) * scale[u];
+        }
+        store_elems<8>(out, to[u], a.out_bf16 != 0, a.vec != 0, x);
+        store_elems<8>(out, to[u] + 8, a.out_bf16 != 0, a.vec != 0, y);
+      } else {
+        const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[2 * e] = bf16_lo(w[e]);
+          x[2 * e + 1] = bf16_hi(w[e]);
+        }
+        store_elems<8>(out, to[u], a.out_bf16 != 0, a.vec != 0, x);
+      }
+    }
+  }
+}
+
+// A plain stream-ordered launch that the kernel before it may overlap (it waits for it).
+template <typename Args>
+cudaError_t launch(void (*kernel)(Args), int grid, int block, const Args& args,
+                   cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(grid));
+  cfg.blockDim = dim3(unsigned(block));
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args);
+}
+
+}  // namespace
+
+cudaError_t launch_paged_write(const PagedWriteArgs& a, cudaStream_t stream) {
+  if (a.spans.rows == 0) return cudaSuccess;
+  const int d = a.pool.head_dim;
+  auto go = [&](void (*k)(PagedWriteArgs)) {
+    return launch(k, a.spans.rows, kRowWarps * 32, a, stream);
+  };
+  if (a.in_bf16) {
+    if (d == 64) return go(paged_write_kernel<__nv_bfloat16, 64>);
+    if (d == 128) return go(paged_write_kernel<__nv_bfloat16, 128>);
+    if (d == 256) return go(paged_write_kernel<__nv_bfloat16, 256>);
+  } else {
+    if (d == 64) return go(paged_write_kernel<float, 64>);
+    if (d == 128) return go(paged_write_kernel<float, 128>);
+    if (d == 256) return go(paged_write_kernel<float, 256>);
+  }
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_paged_read(const PagedReadArgs& a, cudaStream_t stream) {
+  if (a.spans.rows == 0) return cudaSuccess;
+  return launch(paged_read_kernel, (a.spans.rows + kReadRows - 1) / kReadRows, 256, a, stream);
+}
+
+}  // namespace fa

@@ -1,0 +1,690 @@
+// Attention of a few packed rows over a paged cache: single tokens, and spans whose rows x query
+// heads of a KV head fit in 16 columns (bound by the bytes of the pages: each is read once).
+//
+// The products run transposed on mma.sync m16n8k16, so that the keys fill the 16 rows and a KV
+// head's packed rows (column c = row offset x group + query head) the 8 or 16 columns:
+//   S^T (16 keys x columns) = K Q^T, then O^T (head_dim x columns) += V^T P^T.
+// Each product's A operand comes straight from a page's rows: the order of the elements within
+// the sums is free (Q is laid out to match, O is written back by the same order), so a thread's
+// fragments are 16-byte vectors of its keys' rows, and an 8-bit page's bytes become f16 (keys) or
+// bf16 (values) integers in registers, at one and a half to two instructions an element. tcgen05
+// would want the converted tile written to shared memory and read again; at 16 columns the tensor
+// pipe is idle either way.
+//   keys: integers are exact in f16; the queries are scaled by a power of two to f16's range, the
+//     key's scale multiplies the score;
+//   values: the probability times the value's scale is rounded to bf16 (a f16 would lose weights
+//     below 2^-24 of the largest); integers up to 127 are exact in bf16.
+// Scores, maxima, sums and outputs are f32. The maximum is lazy: moved when a score exceeds it by
+// 2^8.
+//
+// A CTA has 4 warps, each with its own ring of 16-key stages filled by cp.async (16 consecutive
+// keys lie in one page, so a stage is one contiguous block of keys, one of values, and 16 scales
+// of each): no barrier among the warps until a unit ends, and a warp loads ahead across units.
+// Rows of a stage are swizzled by 16-byte chunks so that both products' reads are free of bank
+// conflicts. Work is shared out as fa_paged_work.cuh says.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "fa_paged_work.cuh"
+
+namespace fa {
+
+constexpr int kTokWarps = 4;
+constexpr int kTokThreads = kTokWarps * 32;
+constexpr int kTokTile = 16 * kTokWarps;  // keys of a CTA's tile
+
+template <int D, bool Q8, int NT>
+struct TokShape {
+  static constexpr int kCols = 8 * NT;
+  static constexpr int kElem = Q8 ? 1 : 2;
+  static constexpr int kRowBytes = D * kElem;
+  static constexpr int kChunks = kRowBytes / 16;        // 16-byte chunks of a row
+  static constexpr int kPer = 16 / kElem;               // elements of a chunk
+  static constexpr int kBlock = 16 * kRowBytes;         // keys (or values) of a stage
+  static constexpr int kStageBytes = 2 * kBlock + (Q8 ? 128 : 0);
+  static constexpr int kStages = kRowBytes >= 512 ? 2 : 3;  // what shared memory holds
+  static constexpr int kSteps = D / 16;                 // k steps of S, and m tiles of O
+  static constexpr int kRing = kTokWarps * kStages * kStageBytes;
+  static constexpr int kMergeRow = D + 4;               // floats: O, then max and sum (16-byte rows)
+  static constexpr int kMerge = kTokWarps * kCols * kMergeRow * 4;
+  static constexpr int kSmem = kRing + kMerge;
+  // resident CTAs per SM: what 227 KB hold (1 KB each is the system's), at most three
+  static constexpr int kFit = (227 * 1024) / (kSmem + 10240);
+  static constexpr int kCtas = kFit > 3 ? 3 : (kFit < 1 ? 1 : kFit);
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+template <bool F16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  if constexpr (F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The 8 x 8 matrix of 16-bit elements transposed over the warp.
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// Two signed bytes, at bits 0-7 and 16-23 of w, as f16: the byte plus 128 becomes the low bits of
+// 1024 + (byte + 128), less 1152 (all exact). Bits 8-15 and 24-31 are ignored.
+__device__ __forceinline__ uint32_t bytes_to_f16(uint32_t w) {
+  const uint32_t x = (w & 0x00FF00FFu) ^ 0x64806480u;
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// The same as bf16: 128 + (the low 7 bits), less 128 or, for a negative byte, 256 (all exact).
+__device__ __forceinline__ uint32_t bytes_to_bf16(uint32_t w) {
+  const uint32_t x = (w & 0x007F007Fu) | 0x43004300u;
+  const uint32_t y = (w & 0x00800080u) | 0x43004300u;
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x),
+                                   *reinterpret_cast<const __nv_bfloat162*>(&y));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 r = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  const __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// A walk over the CTA's share of the units' tiles: unit (s, h), its tiles [tile, tile_end) within
+// this share, and the unit's own numbers. All of it is uniform over the CTA.
+struct TokWalk {
+  int64_t t, t_end;    // the global tile of `tile`, and the share's end
+  int s, h;
+  int tile, tile_end;  // of the unit's tiles
+  int tiles;           // the unit's tiles
+  int lo, hi;          // key positions that any of its rows sees
+  int row0, n, first;
+};
+
+struct TokPlan {
+  const int64_t* before;  // [sequences + 1]: tiles of the sequences before, of one KV head each
+  int kvh;
+};
+
+// A sequence's part in the token kernel: its span, the keys that its rows see and their tiles
+// (0 if it is empty, out of range or the chunk kernel's).
+__device__ __forceinline__ int token_tiles(const PagedAttendArgs& a, int s, TokWalk* w) {
+  PagedSpan sp;
+  if (!paged_span(a.spans, a.pool.page_shift, s, &sp)) return -1;
+  if (sp.n == 0 || int64_t(sp.n) * a.group > a.token_cols) return 0;
+  int lo, hi, unused;
+  paged_keys(a.kind, a.window, sp.first, sp.first + sp.n, &lo, &unused);
+  hi = sp.first + sp.n;
+  if (w != nullptr) {
+    w->row0 = sp.row0;
+    w->n = sp.n;
+    w->first = sp.first;
+    w->lo = lo;
+    w->hi = hi;
+  }
+  return (hi + kTokTile - 1) / kTokTile - lo / kTokTile;
+}
+
+// Moves the walk to the unit that holds global tile w->t (w->s at or before it); false at the
+// share's end.
+__device__ __forceinline__ bool token_seek(const PagedAttendArgs& a, const TokPlan& plan, TokWalk* w) {
+  if (w->t >= w->t_end) return false;
+  while (plan.before[w->s + 1] * plan.kvh <= w->t) ++w->s;
+  w->tiles = token_tiles(a, w->s, w);
+  const int64_t rest = w->t - plan.before[w->s] * plan.kvh;
+  w->h = int(rest / w->tiles);
+  w->tile = int(rest - int64_t(w->h) * w->tiles);
+  w->tile_end = int(min(int64_t(w->tiles), int64_t(w->tile) + (w->t_end - w->t)));
+  return true;
+}
+
+template <int D, bool Q8, int NT>
+__global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
+    paged_tokens_kernel(const __grid_constant__ PagedAttendArgs a) {
+  using S = TokShape<D, Q8, NT>;
+  constexpr int kRB = S::kRowBytes, kC = S::kChunks, kPer = S::kPer;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int64_t before[kMaxPagedSequences + 1];
+  __shared__ int64_t scratch[kTokWarps];
+  __shared__ int arrived;
+  float* merge = reinterpret_cast<float*>(smem + S::kRing);
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t4 = lane & 3;
+  unsigned char* ring = smem + warp * (S::kStages * S::kStageBytes);
+
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- the plan: tiles before every sequence --------------------------------------------------
+  const int nseq = a.spans.sequences, kvh = a.pool.kv_heads;
+  {
+    const int each = (nseq + kTokThreads - 1) / kTokThreads;
+    const int s0 = min(nseq, int(threadIdx.x) * each), s1 = min(nseq, s0 + each);
+    int64_t sum = 0;
+    for (int s = s0; s < s1; ++s) {
+      const int n = token_tiles(a, s, nullptr);
+      if (n < 0) atomicOr(a.err, kErrPagedSpan);
+      sum += max(n, 0);
+      before[s] = sum;  // inclusive within the thread's sequences, for now
+    }
+    int64_t total;
+    const int64_t base = block_prefix<kTokThreads>(sum, scratch, &total);
+    int64_t prev = base;
+    for (int s = s0; s < s1; ++s) {
+      const int64_t inc = base + before[s];
+      before[s] = prev;
+      prev = inc;
+    }
+    if (threadIdx.x == 0) before[nseq] = total;
+    __syncthreads();
+  }
+  const TokPlan plan{before, kvh};
+  const int64_t work = before[nseq] * kvh;
+  if (work == 0) return;
+  // at least two tiles a CTA: a piece costs about as much as streaming one
+  const int ctas = int(min(int64_t(gridDim.x), (work + 1) / 2));
+  const int cta = blockIdx.x;
+  if (cta >= ctas) return;
+
+  TokWalk lw, cw;  // the loads' walk and the products' walk
+  lw.t = cw.t = share_begin(work, cta, ctas);
+  lw.t_end = cw.t_end = share_begin(work, cta + 1, ctas);
+  {
+    int s0 = 0, s1 = nseq;  // the last s with before[s] * kvh <= t
+    while (s1 - s0 > 1) {
+      const int mid = (s0 + s1) / 2;
+      if (before[mid] * kvh <= cw.t) s0 = mid; else s1 = mid;
+    }
+    lw.s = cw.s = s0;
+  }
+
+  // ---- loads: one 16-key stage at a time ------------------------------------------------------
+  const int shift = a.pool.page_shift;
+  bool more = token_seek(a, plan, &lw);
+  int next_page = -1;  // the page of the next stage's keys (-1: none of them is seen)
+  auto fetch_page = [&]() {
+    next_page = -1;
+    if (!more) return;
+    const int pos = (lw.lo / kTokTile + lw.tile) * kTokTile + warp * 16;
+    if (pos < lw.hi && pos + 16 > lw.lo)
+      next_page = __ldg(a.spans.tables + int64_t(lw.s) * a.spans.table_stride + (pos >> shift));
+  };
+  fetch_page();
+  uint32_t ring_live = 0;  // a bit per stage: its keys are there (a page in range, some key seen)
+  auto issue = [&](int stage) {
+    if (!more) return;
+    bool live = next_page >= 0;
+    const int pos = (lw.lo / kTokTile + lw.tile) * kTokTile + warp * 16;
+    if (!paged_page_ok(next_page, a.pool.pages)) {
+      if (pos < lw.hi && pos + 16 > lw.lo && lane == 0) atomicOr(a.err, kErrPagedPage);
+      live = false;
+    }
+    ring_live = (ring_live & ~(1u << stage)) | (uint32_t(live) << stage);
+    if (live) {
+      const int64_t row = ((int64_t(next_page) * kvh + lw.h) << shift) + (pos & ((1 << shift) - 1));
+      const unsigned char* ks = a.pool.keys + row * kRB;
+      const unsigned char* vs = a.pool.values + row * kRB;
+      const uint32_t kd = smem_u32(ring + stage * S::kStageBytes), vd = kd + S::kBlock;
+#pragma unroll
+      for (int i = 0; i < kC / 2; ++i) {
+        const int q = lane + 32 * i;  // the block's 16-byte chunk
+        const int key = q / kC, c = q % kC;
+        // rows outside the keys seen (a page's stale end, or before the window) come as zeros
+        const uint32_t bytes = pos + key >= lw.lo && pos + key < lw.hi ? 16u : 0u;
+        const int ck = kC >= 8 ? c ^ ((key & 1) << 2) : c;
+        const int cv = kC >= 8 ? c ^ (((key >> 1) & 3) << 1) : c;
+        cp_async16(kd + key * kRB + ck * 16, ks + q * 16, bytes);
+        cp_async16(vd + key * kRB + cv * 16, vs + q * 16, bytes);
+      }
+      if constexpr (Q8) {
+        const int key = lane & 15;
+        const uint32_t bytes = pos + key >= lw.lo && pos + key < lw.hi ? 4u : 0u;
+        const float* sc = lane < 16 ? a.pool.key_scales : a.pool.value_scales;
+        cp_async4(vd + S::kBlock + lane * 4, sc + row + key, bytes);
+      }
+    }
+    ++lw.t;
+    if (++lw.tile == lw.tile_end) more = token_seek(a, plan, &lw);
+    fetch_page();
+  };
+#pragma unroll
+  for (int i = 0; i < S::kStages - 1; ++i) {
+    issue(i);
+    cp_async_commit();
+  }
+
+  // ---- the products ---------------------------------------------------------------------------
+  int stage = 0;
+  while (token_seek(a, plan, &cw)) {
+    // this lane's query column g (+ 8): its fragments, scaled to f16's range for 8-bit pages
+    uint32_t qf[NT][S::kSteps][2];
+    float qscale[NT][2];  // of this lane's score columns 2 t4, 2 t4 + 1
+    int col_lo[NT][2], col_hi[NT][2];
+    int lo_max = 0, hi_min = 0x7fffffff;  // keys that every column sees
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int col = nt * 8 + g;
+      const int r = col / a.group;
+      const bool valid = r < cw.n;
+      float top = 0.0f;
+      float x[S::kSteps][4];
+      const int64_t at = int64_t(cw.row0 + r) * a.q_stride +
+                         int64_t(cw.h * a.group + col % a.group) * D;
+#pragma unroll
+      for (int i = 0; i < kC / 4 + (kC < 4); ++i) {
+        const int64_t e0 = at + (t4 + 4 * i) * kPer;
+#pragma unroll
+        for (int j = 0; j < kPer / 4; ++j) {
+          float(&y)[4] = x[i * (kPer / 4) + j];
+          y[0] = y[1] = y[2] = y[3] = 0.0f;
+          if (!valid) continue;
+          if (a.q_bf16) {
+            const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q) + e0 + 4 * j;
+            if (a.q_vec) {
+              const uint2 w = *reinterpret_cast<const uint2*>(p);
+              y[0] = bf16_lo(w.x); y[1] = bf16_hi(w.x); y[2] = bf16_lo(w.y); y[3] = bf16_hi(w.y);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[e] = __bfloat162float(p[e]);
+            }
+          } else {
+            const float* p = static_cast<const float*>(a.q) + e0 + 4 * j;
+            if (a.q_vec) {
+              const float4 w = *reinterpret_cast<const float4*>(p);
+              y[0] = w.x; y[1] = w.y; y[2] = w.z; y[3] = w.w;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[e] = p[e];
+            }
+          }
+        }
+      }
+      float up = 1.0f, down = 1.0f;
+      if constexpr (Q8) {
+#pragma unroll
+        for (int k = 0; k < S::kSteps; ++k)
+          top = fmaxf(top, fmaxf(fmaxf(fabsf(x[k][0]), fabsf(x[k][1])), fmaxf(fabsf(x[k][2]), fabsf(x[k][3]))));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // the power of two that takes the largest element to [1, 2): exponents within 2^+-126
+        const int e = min(max(int(__float_as_uint(top) >> 23), 1), 253);
+        up = __uint_as_float(uint32_t(254 - e) << 23);
+        down = __uint_as_float(uint32_t(e) << 23);
+      }
+#pragma unroll
+      for (int k = 0; k < S::kSteps; ++k) {
+        if constexpr (Q8) {
+          // 8-bit keys come as bytes 0, 2 then 1, 3 of a word
+          qf[nt][k][0] = pack_f16(x[k][0] * up, x[k][2] * up);
+          qf[nt][k][1] = pack_f16(x[k][1] * up, x[k][3] * up);
+        } else {
+          qf[nt][k][0] = pack_bf16x2(x[k][0], x[k][1]);
+          qf[nt][k][1] = pack_bf16x2(x[k][2], x[k][3]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int cc = nt * 8 + 2 * t4 + j, rr = cc / a.group;
+        qscale[nt][j] = a.scale_log2 * __shfl_sync(0xffffffffu, down, (2 * t4 + j) * 4);
+        col_lo[nt][j] = 0;
+        col_hi[nt][j] = 0;  // a column without a row sees nothing
+        if (rr < cw.n)
+          paged_keys(a.kind, a.window, cw.first + rr, cw.hi, &col_lo[nt][j], &col_hi[nt][j]);
+      }
+    }
+    {
+      int l0, h0;
+      paged_keys(a.kind, a.window, cw.first, cw.hi, &l0, &hi_min);
+      paged_keys(a.kind, a.window, cw.first + cw.n - 1, cw.hi, &lo_max, &h0);
+    }
+
+    float o[S::kSteps][NT][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < S::kSteps; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[k][nt][e] = 0.0f;
+    }
+    bool poisoned[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) poisoned[nt][0] = poisoned[nt][1] = false;
+
+    for (; cw.tile < cw.tile_end; ++cw.tile, ++cw.t) {
+      cp_async_wait<S::kStages - 2>();
+      __syncwarp();
+      const int fill = stage == 0 ? S::kStages - 1 : stage - 1;  // the stage read last time
+      issue(fill);
+      cp_async_commit();
+      const unsigned char* kb = ring + stage * S::kStageBytes;
+      const unsigned char* vb = kb + S::kBlock;
+      const float* scales = reinterpret_cast<const float*>(vb + S::kBlock);
+      const bool live = (ring_live >> stage) & 1u;
+      stage = stage + 1 == S::kStages ? 0 : stage + 1;
+      if (!live) continue;  // uniform over the warp
+      const int pos = (cw.lo / kTokTile + cw.tile) * kTokTile + warp * 16;
+
+      // S^T: keys g and g + 8 of the stage
+      float sc[NT][2][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[nt][0][e] = sc[nt][1][e] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kC / 4; ++i) {
+        const int c = t4 + 4 * i;
+        const int cs = kC >= 8 ? c ^ ((g & 1) << 2) : c;
+        const uint4 ra = *reinterpret_cast<const uint4*>(kb + g * kRB + cs * 16);
+        const uint4 rb = *reinterpret_cast<const uint4*>(kb + (g + 8) * kRB + cs * 16);
+        const uint32_t wa[4] = {ra.x, ra.y, ra.z, ra.w}, wb[4] = {rb.x, rb.y, rb.z, rb.w};
+        if constexpr (Q8) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t fr[4] = {bytes_to_f16(wa[j]), bytes_to_f16(wb[j]),
+                                    bytes_to_f16(wa[j] >> 8), bytes_to_f16(wb[j] >> 8)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816<true>(sc[nt][j & 1], fr, qf[nt][4 * i + j][0], qf[nt][4 * i + j][1]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t fr[4] = {wa[2 * j], wb[2 * j], wa[2 * j + 1], wb[2 * j + 1]};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816<false>(sc[nt][j & 1], fr, qf[nt][2 * i + j][0], qf[nt][2 * i + j][1]);
+          }
+        }
+      }
+      float ks[2] = {1.0f, 1.0f}, vs[2] = {1.0f, 1.0f};
+      if constexpr (Q8) {
+        ks[0] = scales[g];
+        ks[1] = scales[g + 8];
+        vs[0] = scales[16 + g];
+        vs[1] = scales[16 + g + 8];
+      }
+      const bool whole = pos >= lo_max && pos + 16 <= hi_min;
+      float s[NT][4];  // e: key g + 8 (e / 2), column 2 t4 + e % 2
+      bool grow = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = (sc[nt][0][e] + sc[nt][1][e]) * (qscale[nt][e & 1] * ks[e >> 1]);
+          const int p = pos + g + 8 * (e >> 1);
+          s[nt][e] = whole || (p >= col_lo[nt][e & 1] && p < col_hi[nt][e & 1]) ? x : -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float top = fmaxf(s[nt][j], s[nt][2 + j]);
+          grow = grow || top > m[nt][j] + 8.0f || (m[nt][j] == -INFINITY && top > -INFINITY);
+        }
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float alpha[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float top = fmaxf(s[nt][j], s[nt][2 + j]);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            alpha[j] = 1.0f;
+            if (top > m[nt][j]) {
+              if (m[nt][j] > -INFINITY) alpha[j] = exp2_approx(m[nt][j] - top);
+              m[nt][j] = top;
+            }
+            l[nt][j] *= alpha[j];
+          }
+#pragma unroll
+          for (int k = 0; k < S::kSteps; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[k][nt][e] *= alpha[e & 1];
+        }
+      }
+      uint32_t pf[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float ms = m[nt][e & 1] == -INFINITY ? 0.0f : m[nt][e & 1];
+          const float p = exp2_approx(s[nt][e] - ms);
+          l[nt][e & 1] += p;
+          // a key that the column does not see keeps its scale out (it may be infinite or NaN)
+          w[e] = Q8 ? (s[nt][e] > -INFINITY ? p * vs[e >> 1] : 0.0f) : p;
+        }
+        pf[nt][0] = movmatrix(pack_bf16x2(w[0], w[1]));
+        pf[nt][1] = movmatrix(pack_bf16x2(w[2], w[3]));
+      }
+
+      // O^T: values of keys 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9
+      constexpr int kPiece = kC >= 8 ? 16 : 8;             // bytes a lane takes of a row at a time
+      constexpr int kPieces = kRB / (8 * kPiece);
+      constexpr int kWords = kPiece / 4;
+      uint32_t bad = 0;  // bf16: which of the lane's four keys has a value that is not finite
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        uint32_t wv[4][kWords];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int key = 2 * t4 + (q & 1) + 8 * (q >> 1);
+          if constexpr (kPiece == 16) {
+            const int c = (g + 8 * i) ^ (((key >> 1) & 3) << 1);
+            const uint4 r = *reinterpret_cast<const uint4*>(vb + key * kRB + c * 16);
+            wv[q][0] = r.x; wv[q][1] = r.y; wv[q][2] = r.z; wv[q][3] = r.w;
+          } else {
+            const uint2 r = *reinterpret_cast<const uint2*>(vb + key * kRB + g * 8);
+            wv[q][0] = r.x; wv[q][1] = r.y;
+          }
+        }
+        if constexpr (!Q8) {
+          if (!whole) {
+            // a value that is not finite would reach columns that do not see its key (0 x inf):
+            // it is taken out here and every column that sees it marked below
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int x = 0; x < kWords; ++x) {
+                if ((wv[q][x] & 0x7F80u) == 0x7F80u) { wv[q][x] &= 0xFFFF0000u; bad |= 1u << q; }
+                if ((wv[q][x] & 0x7F800000u) == 0x7F800000u) { wv[q][x] &= 0xFFFFu; bad |= 1u << q; }
+              }
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < kWords; ++x) {
+          if constexpr (Q8) {
+            // bytes 0..3 of word x: elements 4x .. 4x + 3 of the piece, two m tiles
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              const uint32_t sel0 = b == 0 ? 0x0400u : 0x0602u;  // bytes 2b of both keys
+              const uint32_t sel1 = b == 0 ? 0x0501u : 0x0703u;  // bytes 2b + 1
+              const uint32_t fr[4] = {bytes_to_bf16(__byte_perm(wv[0][x], wv[1][x], sel0)),
+                                      bytes_to_bf16(__byte_perm(wv[0][x], wv[1][x], sel1)),
+                                      bytes_to_bf16(__byte_perm(wv[2][x], wv[3][x], sel0)),
+                                      bytes_to_bf16(__byte_perm(wv[2][x], wv[3][x], sel1))};
+              const int mt = i * (kPiece / 2) + 2 * x + b;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma16816<false>(o[mt][nt], fr, pf[nt][0], pf[nt][1]);
+            }
+          } else {
+            const uint32_t fr[4] = {__byte_perm(wv[0][x], wv[1][x], 0x5410),
+                                    __byte_perm(wv[0][x], wv[1][x], 0x7632),
+                                    __byte_perm(wv[2][x], wv[3][x], 0x5410),
+                                    __byte_perm(wv[2][x], wv[3][x], 0x7632)};
+            const int mt = i * (kPiece / 4) + x;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816<false>(o[mt][nt], fr, pf[nt][0], pf[nt][1]);
+          }
+        }
+      }
+      if constexpr (!Q8) {
+        if (!whole) {
+          // the keys with such a value, over the warp: bit k for key k of the stage
+          uint32_t keys = 0;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if ((bad >> q) & 1u) keys |= 1u << (2 * t4 + (q & 1) + 8 * (q >> 1));
+          keys = __reduce_or_sync(0xffffffffu, keys);
+          for (uint32_t rest = keys; rest != 0; rest &= rest - 1) {
+            const int p = pos + __ffs(rest) - 1;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                poisoned[nt][j] = poisoned[nt][j] || (p >= col_lo[nt][j] && p < col_hi[nt][j]);
+          }
+        }
+      }
+    }
+
+    // ---- the unit's (or piece's) end: the warps' parts merged -----------------------------------
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 4);
+        l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 8);
+        l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 16);
+        if (poisoned[nt][j]) l[nt][j] = __int_as_float(0x7fffffff);
+        float* row = merge + (warp * S::kCols + nt * 8 + 2 * t4 + j) * S::kMergeRow;
+        if (g == 0) { row[D] = m[nt][j]; row[D + 1] = l[nt][j]; }
+        constexpr int kPiece = kC >= 8 ? 16 : 8;
+        constexpr int kElems = kPiece / S::kElem;  // of a lane's piece of a row
+#pragma unroll
+        for (int k = 0; k < S::kSteps; ++k) {
+          // m tile k: elements 2 (k % (kElems / 2)) + {0, 1} of the lane's piece k / (kElems / 2)
+          const int d = (g + 8 * (k / (kElems / 2))) * kElems + 2 * (k % (kElems / 2));
+          *reinterpret_cast<float2*>(row + d) = make_float2(o[k][nt][j], o[k][nt][2 + j]);
+        }
+      }
+    __syncthreads();
+    const int64_t unit0 = plan.before[cw.s] * kvh + int64_t(cw.h) * cw.tiles;  // its first tile
+    const int c0 = share_owner(work, unit0, ctas);
+    const int c1 = share_owner(work, unit0 + cw.tiles - 1, ctas);
+    const int pieces = c1 - c0 + 1;
+    const int cols = cw.n * a.group;
+    constexpr int kVecs = D / 4;  // float4s of a column
+    auto write_out = [&](int col, int v, float4 x, float inv) {
+      const int64_t at = int64_t(cw.row0 + col / a.group) * a.out_stride +
+                         int64_t(cw.h * a.group + col % a.group) * D + v * 4;
+      x = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+      if (a.out_bf16) {
+        __nv_bfloat16* p = static_cast<__nv_bfloat16*>(a.out) + at;
+        if (a.out_vec) {
+          *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
+        } else {
+          p[0] = __float2bfloat16_rn(x.x); p[1] = __float2bfloat16_rn(x.y);
+          p[2] = __float2bfloat16_rn(x.z); p[3] = __float2bfloat16_rn(x.w);
+        }
+      } else {
+        float* p = static_cast<float*>(a.out) + at;
+        if (a.out_vec) *reinterpret_cast<float4*>(p) = x;
+        else { p[0] = x.x; p[1] = x.y; p[2] = x.z; p[3] = x.w; }
+      }
+    };
+    const int slot = 2 * cta + (cta == c0 ? 1 : 0);
+    for (int i = threadIdx.x; i < cols * kVecs; i += kTokThreads) {
+      const int col = i / kVecs, v = i % kVecs;
+      float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kTokWarps; ++w)
+        mm = fmaxf(mm, merge[(w * S::kCols + col) * S::kMergeRow + D]);
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < kTokWarps; ++w) {
+        const float* row = merge + (w * S::kCols + col) * S::kMergeRow;
+        const float f = row[D] == -INFINITY ? 0.0f : exp2_approx(row[D] - mm);
+        // a warp that saw no key has sum 0 (or NaN, which stays)
+        ll += row[D] == -INFINITY ? row[D + 1] : f * row[D + 1];
+        const float4 x = *reinterpret_cast<const float4*>(row + 4 * v);
+        acc.x = fmaf(f, x.x, acc.x); acc.y = fmaf(f, x.y, acc.y);
+        acc.z = fmaf(f, x.z, acc.z); acc.w = fmaf(f, x.w, acc.w);
+      }
+      if (pieces == 1) {
+        // a row that sees no key (every page out of range) is zero
+        write_out(col, v, acc, ll == 0.0f ? 0.0f : 1.0f / ll);
+      } else {
+        *reinterpret_cast<float4*>(a.part_o + (int64_t(slot) * kPagedTokenCols + col) * D + 4 * v) = acc;
+        if (v == 0)
+          *reinterpret_cast<float2*>(a.part_ml + (int64_t(slot) * kPagedTokenCols + col) * 2) =
+              make_float2(mm, ll);
+      }
+    }
+    if (pieces > 1) {
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        const int before_me = atomicAdd(&a.counters[c0], 1);
+        arrived = before_me == pieces - 1;
+        if (arrived) a.counters[c0] = 0;
+      }
+      __syncthreads();
+      if (arrived) {
+        __threadfence();
+        for (int i = threadIdx.x; i < cols * kVecs; i += kTokThreads) {
+          const int col = i / kVecs, v = i % kVecs;
+          auto ml_at = [&](int c) {
+            const int64_t at = int64_t(2 * c + (c == c0 ? 1 : 0)) * kPagedTokenCols + col;
+            return __ldcg(reinterpret_cast<const float2*>(a.part_ml + at * 2));
+          };
+          float mm = -INFINITY;
+#pragma unroll 8
+          for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, ml_at(c).x);
+          float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          float ll = 0.0f;
+#pragma unroll 8
+          for (int c = c0; c <= c1; ++c) {
+            const float2 ml = ml_at(c);
+            const float f = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - mm);
+            ll += ml.x == -INFINITY ? ml.y : f * ml.y;
+            const int64_t at = int64_t(2 * c + (c == c0 ? 1 : 0)) * kPagedTokenCols + col;
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(a.part_o + at * D + 4 * v));
+            acc.x = fmaf(f, x.x, acc.x); acc.y = fmaf(f, x.y, acc.y);
+            acc.z = fmaf(f, x.z, acc.z); acc.w = fmaf(f, x.w, acc.w);
+          }
+          write_out(col, v, acc, ll == 0.0f ? 0.0f : 1.0f / ll);
+        }
+      }
+    }
+    __syncthreads();  // the merge rows are free again
+  }
+}
+
+}  // namespace fa

@@ -20,7 +20,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("FA_ATTN_LIB") or os.path.join(_HERE, "libfa_attn.so")
 
 OK, ERR_ARG, ERR_SHAPE, ERR_CAPACITY, ERR_CUDA, ERR_TIMEOUT, ERR_UNSUPPORTED = range(7)
-F32, BF16 = 0, 1
+F32, BF16, Q8 = 0, 1, 2
 MASK_CAUSAL, MASK_WINDOW, MASK_FULL, MASK_GROUPS = range(4)
 ROPE_NONE, ROPE_HALF, ROPE_INTERLEAVED = range(3)
 NORM_NONE, NORM_ROW, NORM_HEAD = range(3)
@@ -105,6 +105,28 @@ class _Prologue(C.Structure):
                 ("rotated_rows", C.c_int32)]
 
 
+class _PagedCache(C.Structure):
+    _fields_ = [("layers", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("pages", C.c_int32), ("page_size", C.c_int32),
+                ("dtype", C.c_int32), ("device", C.c_int32), ("keys", C.c_void_p),
+                ("values", C.c_void_p), ("key_scales", C.c_void_p), ("value_scales", C.c_void_p)]
+
+
+class _PagedBatch(C.Structure):
+    _fields_ = [("sequences", C.c_int32), ("rows", C.c_int32), ("max_rows", C.c_int32),
+                ("table_width", C.c_int32), ("table_stride", C.c_int64),
+                ("row_starts", C.c_void_p), ("firsts", C.c_void_p), ("tables", C.c_void_p),
+                ("mask", C.c_int32), ("window", C.c_int32), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64)]
+
+
+class _PagedRows(C.Structure):
+    _fields_ = [("keys", C.c_void_p), ("values", C.c_void_p), ("row_stride", C.c_int64),
+                ("head_stride", C.c_int64), ("dtype", C.c_int32)]
+
+
+PAGED_COUNTER_BYTES = 8192
+
 _lib = None
 
 # name -> (restype, argtypes) for every entry point of include/fa_attn.h
@@ -147,6 +169,15 @@ SIGNATURES = {
     "fa_attend_relpos": (C.c_int, [_P, _P, _I64, _P]),
     "fa_normalize_and_rotate": (C.c_int, [_P, _P, _I64, _P, _I64, _I32, _P]),
     "fa_gated_attention": (C.c_int, [_P, _I32, _P, _I32, _I32, _P, _P, _P, _I64, _P, _I64, _P]),
+    "fa_paged_workspace_bytes": (C.c_int, [_P, _I32, _I32, C.POINTER(C.c_uint64)]),
+    "fa_paged_check": (C.c_int, [_P, _P]),
+    "fa_attention_input_paged": (C.c_int, [_P, _I32, _P, _I32, _P, _P, _P, _I64, _I32, _P, _I64,
+                                           _P]),
+    "fa_paged_write": (C.c_int, [_P, _I32, _P, _P, _P]),
+    "fa_paged_read": (C.c_int, [_P, _I32, _P, _P, _P]),
+    "fa_attend_paged": (C.c_int, [_P, _I32, _P, _P, _I64, _I32, _P, _I64, _I32, _P]),
+    "fa_attention_paged": (C.c_int, [_P, _I32, _P, _I32, _P, _P, _P, _I64, _I32, _P, _I64, _I32,
+                                     _P]),
     "fa_device_status": (C.c_int, [_P]),
     "fa_rng_fill_normal": (C.c_int, [C.c_uint64, _P, _I64]),
 }
@@ -555,6 +586,154 @@ def normalize_and_rotate(heads: int, head_dim: int, qkv, out, norm: int = NORM_R
                                          out.stride(0), dt, _stream(stream)))
 
 
+def _rows_dtype(t, what):
+    import torch
+    dt = {torch.float32: F32, torch.bfloat16: BF16}.get(t.dtype)
+    if dt is None:
+        raise ValueError(f"{what} of {t.dtype}: float32 or bfloat16")
+    if t.dim() == 0 or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        raise ValueError(f"{what} with unit stride along a row")
+    return dt
+
+
+def _stride0(t):
+    """Elements between rows (of a single row: its width, as torch leaves its stride open)."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t[0].numel() if t.shape[0] else 1)
+
+
+class PagedCache:
+    """A KV cache in pages of one pool (fa_paged_cache): keys and values are device tensors
+    [layers, pages, kv_heads, page_size, head_dim] of bf16 or (Q8) int8, with 8-bit pages beside
+    f32 scales [layers, pages, kv_heads, page_size]. Allocated zeroed here, or the caller's own."""
+
+    def __init__(self, shape: Shape, pages: int, page_size: int = 16, dtype: int = Q8,
+                 device: int | None = None, keys=None, values=None, key_scales=None,
+                 value_scales=None):
+        import torch
+        if dtype not in (BF16, Q8):
+            raise FaError(ERR_UNSUPPORTED, f"pages of dtype {dtype}: BF16 or Q8")
+        self.shape, self.pages, self.page_size, self.dtype = shape, pages, page_size, dtype
+        dims = (shape.layers, pages, shape.kv_heads, page_size, shape.head_dim)
+        elem = torch.int8 if dtype == Q8 else torch.bfloat16
+        if keys is None:
+            if device is None:
+                device = torch.cuda.current_device()
+            where = torch.device("cuda", device)
+            keys = torch.zeros(dims, dtype=elem, device=where)
+            values = torch.zeros(dims, dtype=elem, device=where)
+            if dtype == Q8:
+                key_scales = torch.zeros(dims[:-1], device=where)
+                value_scales = torch.zeros(dims[:-1], device=where)
+        given = [(keys, dims, elem), (values, dims, elem)]
+        if dtype == Q8:
+            given += [(key_scales, dims[:-1], torch.float32), (value_scales, dims[:-1], torch.float32)]
+        for t, want, kind in given:
+            if t is None or tuple(t.shape) != tuple(want) or t.dtype != kind or not t.is_contiguous():
+                raise ShapeError(ERR_SHAPE, f"a pool tensor of {want} {kind}, contiguous")
+        self.keys, self.values = keys, values
+        self.key_scales = key_scales if dtype == Q8 else None
+        self.value_scales = value_scales if dtype == Q8 else None
+        self.device = keys.device.index or 0
+        self._c = _PagedCache(shape.layers, shape.heads, shape.kv_heads, shape.head_dim, pages,
+                              page_size, dtype, self.device, keys.data_ptr(), values.data_ptr(),
+                              key_scales.data_ptr() if dtype == Q8 else None,
+                              value_scales.data_ptr() if dtype == Q8 else None)
+
+    def attention_input(self, layer: int, batch: "PagedBatch", qkv, angles=None,
+                        rope: int = ROPE_HALF, norm=None, q_out=None, stream=None):
+        """RoPE (+ head norm) and keep of the batch's rows into their pages (layer.rs:175-234)."""
+        batch.covers(qkv, q_out, angles)
+        dt = _rows_dtype(qkv, "qkv")
+        if q_out is not None and (_rows_dtype(q_out, "q_out") != dt):
+            raise ValueError("q_out has qkv's dtype")
+        _check(lib().fa_attention_input_paged(
+            C.byref(self._c), layer, C.byref(batch._c), rope if angles is not None else ROPE_NONE,
+            _dptr(angles), _norm(norm), _dptr(qkv), _stride0(qkv), dt, _dptr(q_out),
+            0 if q_out is None else _stride0(q_out), _stream(stream)))
+
+    def _rows(self, batch, keys, values):
+        batch.covers(keys, values)
+        dt = _rows_dtype(keys, "keys")
+        want = (self.shape.kv_heads, self.shape.head_dim)
+        if keys.shape != values.shape or keys.dtype != values.dtype or tuple(keys.shape[1:]) != want:
+            raise ValueError(f"keys and values of one shape (rows, {want[0]}, {want[1]}) and dtype")
+        if keys.stride() != values.stride():
+            raise ValueError("keys and values with the same strides")
+        return _PagedRows(keys.data_ptr(), values.data_ptr(), keys.stride(0), keys.stride(1), dt)
+
+    def write(self, layer: int, batch: "PagedBatch", keys, values, stream=None):
+        """Key and value rows (rows, kv_heads, head_dim) into the batch's pages as they are."""
+        r = self._rows(batch, keys, values)
+        _check(lib().fa_paged_write(C.byref(self._c), layer, C.byref(batch._c), C.byref(r),
+                                    _stream(stream)))
+
+    def read(self, layer: int, batch: "PagedBatch", keys, values, stream=None):
+        """The batch's rows read back into keys and values (rows, kv_heads, head_dim)."""
+        r = self._rows(batch, keys, values)
+        _check(lib().fa_paged_read(C.byref(self._c), layer, C.byref(batch._c), C.byref(r),
+                                   _stream(stream)))
+
+    def attend(self, layer: int, batch: "PagedBatch", q, out, stream=None):
+        """KvCache::attend (transformer.rs:182-219) of rotated queries over the pages."""
+        batch.covers(q, out)
+        _check(lib().fa_attend_paged(
+            C.byref(self._c), layer, C.byref(batch._c), _dptr(q), _stride0(q),
+            _rows_dtype(q, "q"), _dptr(out), _stride0(out), _rows_dtype(out, "out"),
+            _stream(stream)))
+
+    def attention(self, layer: int, batch: "PagedBatch", qkv, out, angles=None,
+                  rope: int = ROPE_HALF, norm=None, stream=None):
+        """The attention phase of one layer: the batch's rows kept, then attended."""
+        batch.covers(qkv, out, angles)
+        _check(lib().fa_attention_paged(
+            C.byref(self._c), layer, C.byref(batch._c), rope if angles is not None else ROPE_NONE,
+            _dptr(angles), _norm(norm), _dptr(qkv), _stride0(qkv), _rows_dtype(qkv, "qkv"),
+            _dptr(out), _stride0(out), _rows_dtype(out, "out"), _stream(stream)))
+
+
+class PagedBatch:
+    """The spans of calls over a paged cache (fa_paged_batch): row_starts (sequences + 1), firsts
+    (sequences) and tables (sequences x table pages) as int32 device tensors, which the kernels
+    read when they run; `rows` rows in the call's arrays, at most `max_rows` of them a sequence's.
+    It owns the attention's workspace: batches that may run at the same time are separate ones."""
+
+    def __init__(self, cache: PagedCache, row_starts, firsts, tables, rows: int, max_rows: int,
+                 mask: Mask = Mask(MASK_CAUSAL)):
+        import torch
+        self.cache, self.mask, self.rows = cache, mask, rows
+        n = firsts.shape[0]
+        for t, size, what in ((row_starts, n + 1, "row_starts"), (firsts, n, "firsts")):
+            if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != size or not t.is_contiguous():
+                raise ValueError(f"{what}: {size} contiguous int32")
+        if tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != n or (
+                tables.shape[1] > 1 and tables.stride(1) != 1):
+            raise ValueError(f"tables: int32 of {n} rows")
+        self.row_starts, self.firsts, self.tables = row_starts, firsts, tables
+        nbytes = C.c_uint64()
+        _check(lib().fa_paged_workspace_bytes(C.byref(cache._c), rows, max_rows, C.byref(nbytes)))
+        where = torch.device("cuda", cache.device)
+        self.workspace = torch.empty(nbytes.value, dtype=torch.uint8, device=where)
+        self.workspace[:PAGED_COUNTER_BYTES].zero_()
+        stride = tables.stride(0) if n > 1 else tables.shape[1]
+        self._c = _PagedBatch(n, rows, max_rows, tables.shape[1], stride, row_starts.data_ptr(),
+                              firsts.data_ptr(), tables.data_ptr(), mask.kind, mask.window,
+                              self.workspace.data_ptr(), nbytes.value)
+
+    def covers(self, *tensors):
+        for t in tensors:
+            if t is not None and t.shape[0] < self.rows:
+                raise ValueError(f"{t.shape[0]} rows in an array of a batch of {self.rows}")
+
+    def check(self):
+        """Raises what the kernels would find out of range in the batch's numbers (a copy of them
+        on the host: it waits for the current stream)."""
+        host = [t.cpu().contiguous() for t in (self.row_starts, self.firsts, self.tables)]
+        b = _PagedBatch.from_buffer_copy(self._c)
+        b.row_starts, b.firsts, b.tables = (t.data_ptr() for t in host)
+        b.table_stride = host[2].shape[1]
+        _check(lib().fa_paged_check(C.byref(self.cache._c), C.byref(b)))
+
+
 class PeerExchange:
     """This rank's exchange buffer for fa_exchange_merge and the mappings of the other ranks'
     (CUDA IPC handles swapped over `group`, a torch.distributed process group of one process per
@@ -634,7 +813,8 @@ class PeerExchange:
 
 
 def device_status(stream=None):
-    """Raises FaError(ERR_TIMEOUT) if a kernel gave up a device-side wait."""
+    """Raises FaError(ERR_TIMEOUT) if a kernel gave up a device-side wait, CapacityError or
+    FaError(ERR_ARG) if a paged call met spans or page ids out of range."""
     _check(lib().fa_device_status(_stream(stream)))
 
 

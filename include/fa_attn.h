@@ -39,6 +39,9 @@ extern "C" {
 /* Element types of the cache and of full-mask operands. */
 #define FA_F32 0
 #define FA_BF16 1
+/* 8-bit pages of a paged cache: integers in -127..127 and one f32 scale for each (position, KV
+ * head) of keys and of values. */
+#define FA_Q8 2
 
 /* transformer::Mask (crates/blocks/src/transformer.rs:97-111). */
 #define FA_MASK_CAUSAL 0
@@ -132,7 +135,8 @@ typedef struct fa_kvcache fa_kvcache;
 const char* fa_last_error(void);
 
 /* The build's capabilities: a bitmask of 1 = f32 cache, 2 = bf16 cache, 4 = tcgen05 prefill /
- * full-mask kernels, 8 = head dims between the powers of two; and the head_dim values with a
+ * full-mask kernels, 8 = head dims between the powers of two, 16 = paged caches (bf16 and 8-bit
+ * pages of head_dim 64, 128 and 256); and the head_dim values with a
  * kernel of their own through *head_dims (may be NULL). With flag 8, a head_dim between 32 and
  * 256 that is a multiple of 4 (f32 rows) or 8 (bf16 rows) runs on the kernel of the next power
  * of two, the lanes past the head idle (Kronos' 52, Iris' 80); the tensor-core kernels take
@@ -419,8 +423,127 @@ int fa_gated_attention(fa_kvcache* cache, int32_t layer, const fa_span* span, in
                        const float* qkv, int64_t qkv_stride, float* out, int64_t out_stride,
                        void* stream);
 
+/* A paged KV cache: the positions of many sequences in pages of one pool, so that a sequence
+ * grows page by page and sequences may share the pages of a common prefix. The pool is the
+ * caller's device memory: keys and values are [layers][pages][kv_heads][page_size][head_dim] of
+ * FA_BF16 or FA_Q8 elements (16-byte aligned), and with FA_Q8 key_scales and value_scales are
+ * [layers][pages][kv_heads][page_size] f32 (NULL otherwise). It stands beside fa_kvcache (one
+ * contiguous block of positions per sequence, transformer.rs:131-162; the reference has no
+ * pages): the same attention phase, over positions that lie where a table says.
+ * head_dim 64, 128 or 256; page_size a power of two, 16 to 4096; heads a multiple of kv_heads, at
+ * most 128 query heads to a KV head. */
+typedef struct {
+  int32_t layers;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t pages;
+  int32_t page_size;
+  int32_t dtype;  /* FA_BF16 or FA_Q8 */
+  int32_t device;
+  void* keys;
+  void* values;
+  float* key_scales;
+  float* value_scales;
+} fa_paged_cache;
+
+/* The spans of a call over a paged cache: the rows of `sequences` sequences (at most 1024) one
+ * after the other, sequence s's rows row_starts[s] .. row_starts[s + 1] of the call's arrays at
+ * the positions from firsts[s] on; its position p lies in slot p % page_size of the page
+ * tables[s * table_stride + p / page_size]. The numbers are DEVICE memory, read by the kernels,
+ * so a captured call follows them when it is replayed (the host's part of a call depends on
+ * rows, max_rows and the mask alone). A sequence may have no rows; rows of the arrays past
+ * row_starts[sequences] are padding and left as they are. The mask is FA_MASK_CAUSAL,
+ * FA_MASK_WINDOW or FA_MASK_FULL (every position up to the sequence's last new row).
+ * Numbers out of range (rows outside the call's, more of them than max_rows, positions past
+ * table_width pages, page ids outside the pool) fault nothing: such a sequence is left out of the
+ * call, a position on such a page is not written and not seen, and fa_device_status returns
+ * FA_ERR_CAPACITY (spans) or FA_ERR_ARG (page ids). fa_paged_check finds them on the host.
+ * Pages that a call writes belong to one sequence each. */
+typedef struct {
+  int32_t sequences;
+  int32_t rows;         /* rows of the call's arrays */
+  int32_t max_rows;     /* no sequence has more */
+  int32_t table_width;  /* page ids of a sequence's table */
+  int64_t table_stride; /* from one sequence's table to the next */
+  const int32_t* row_starts; /* sequences + 1 */
+  const int32_t* firsts;     /* sequences */
+  const int32_t* tables;
+  int32_t mask;
+  int32_t window;
+  /* Scratch of the attention entry points: fa_paged_workspace_bytes of it, 256-byte aligned, its
+   * first FA_PAGED_COUNTER_BYTES zeroed once before its first call (calls leave them zero; zero
+   * them again after FA_ERR_TIMEOUT). Calls, and replays of captured calls, that may run at the
+   * same time need a workspace each. NULL for the other entry points. */
+  void* workspace;
+  uint64_t workspace_bytes;
+} fa_paged_batch;
+
+#define FA_PAGED_COUNTER_BYTES 8192
+
+/* The workspace of fa_attend_paged and fa_attention_paged for batches of at most `rows` rows, no
+ * sequence of which has more than `max_rows`. */
+int fa_paged_workspace_bytes(const fa_paged_cache* cache, int32_t rows, int32_t max_rows,
+                             uint64_t* bytes);
+
+/* Checks a batch whose row_starts, firsts and tables are HOST copies, as the kernels check theirs:
+ * FA_ERR_CAPACITY for positions past a table, FA_ERR_ARG for rows or page ids out of range, or for
+ * a row whose slot another row of the call writes too. Touches no device. */
+int fa_paged_check(const fa_paged_cache* cache, const fa_paged_batch* batch);
+
+/* fa_attention_input over a paged cache (Stack::attention_input after the projection,
+ * layer.rs:175-234): each row of qkv (dtype FA_F32 or FA_BF16, qkv_stride apart: query, key and
+ * value heads) head-normed (optional) and rotated by `angles` (rows x head_dim f32), the keys and
+ * values kept in the pages, the rotated queries into q_out (rows q_out_stride apart, of dtype; may
+ * be NULL). The arithmetic is f32; FA_BF16 pages round to nearest even, FA_Q8 pages keep
+ * round(x * 127 / max|x|) of each head with the scale max|x| / 127 (a head below 2^-100
+ * everywhere as zeros; one with an infinity or a NaN as NaN throughout). */
+int fa_attention_input_paged(const fa_paged_cache* cache, int32_t layer,
+                             const fa_paged_batch* batch, int32_t rope, const float* angles,
+                             const fa_head_norm* norm, const void* qkv, int64_t qkv_stride,
+                             int32_t dtype, void* q_out, int64_t q_out_stride, void* stream);
+
+/* Keys and values of the batch's rows into a layer's pages as they are (no norm, no RoPE), rounded
+ * or quantised as above: row r's KV head h at keys + r * row_stride + h * head_stride (elements of
+ * dtype, FA_F32 or FA_BF16). A block of a fa_kvcache is such rows (row_stride head_dim, head_stride
+ * capacity * head_dim), as are the new rows of a projection. Keys and values share the strides. */
+typedef struct {
+  void* keys;
+  void* values;
+  int64_t row_stride;
+  int64_t head_stride;
+  int32_t dtype;
+} fa_paged_rows;
+
+int fa_paged_write(const fa_paged_cache* cache, int32_t layer, const fa_paged_batch* batch,
+                   const fa_paged_rows* rows, void* stream);
+
+/* The batch's rows read back out of a layer's pages (KvCache::copy_rows over pages,
+ * transformer.rs:221-239): the values that the pages stand for, in f32 or rounded to bf16. A batch
+ * with firsts 0 and every position as a row reads whole sequences. */
+int fa_paged_read(const fa_paged_cache* cache, int32_t layer, const fa_paged_batch* batch,
+                  const fa_paged_rows* rows, void* stream);
+
+/* fa_attend over a paged cache (KvCache::attend, transformer.rs:182-219): the batch's rows'
+ * rotated queries (rows q_stride apart, heads x head_dim of dtype FA_F32 or FA_BF16) over their
+ * sequences' pages under the mask, into out (rows out_stride apart, of out_dtype), scores scaled
+ * by 1/sqrt(head_dim). Any number of rows to a sequence: single tokens, chunks, and both in one
+ * call. Queries and probabilities are rounded to 16 bits for the tensor cores, scores, sums and
+ * outputs accumulated in f32. A row that sees no position (its pages out of range) is zero. */
+int fa_attend_paged(const fa_paged_cache* cache, int32_t layer, const fa_paged_batch* batch,
+                    const void* q, int64_t q_stride, int32_t dtype, void* out,
+                    int64_t out_stride, int32_t out_dtype, void* stream);
+
+/* fa_attention over a paged cache: fa_attention_input_paged, then fa_attend_paged over the pages
+ * with the new rows in them. */
+int fa_attention_paged(const fa_paged_cache* cache, int32_t layer, const fa_paged_batch* batch,
+                       int32_t rope, const float* angles, const fa_head_norm* norm,
+                       const void* qkv, int64_t qkv_stride, int32_t dtype, void* out,
+                       int64_t out_stride, int32_t out_dtype, void* stream);
+
 /* Waits for `stream` and reports whether any kernel of this library gave up a device-side wait
- * since the last call (FA_ERR_TIMEOUT, clearing the flag) or FA_OK. */
+ * since the last call (FA_ERR_TIMEOUT, clearing the flag), whether a paged call met spans
+ * (FA_ERR_CAPACITY) or page ids (FA_ERR_ARG) out of range, or FA_OK. */
 int fa_device_status(void* stream);
 
 /* The reference's seeded generator (crates/kernels/src/rng.rs:5-52: xoshiro256** seeded by

@@ -24,6 +24,16 @@ use std::ffi::{c_char, c_void};
 #[repr(C)] pub struct FaPrologue { pub tokens: i32, pub heads: i32, pub head_dim: i32, pub norm: i32,
                                   pub q_norm: *const f32, pub k_norm: *const f32, pub eps: f32, pub rope: i32,
                                   pub angles: *const f32, pub rotated_rows: i32 }
+#[repr(C)] pub struct FaPagedCache { pub layers: i32, pub heads: i32, pub kv_heads: i32, pub head_dim: i32,
+                                    pub pages: i32, pub page_size: i32, pub dtype: i32, pub device: i32,
+                                    pub keys: *mut c_void, pub values: *mut c_void,
+                                    pub key_scales: *mut f32, pub value_scales: *mut f32 }
+#[repr(C)] pub struct FaPagedBatch { pub sequences: i32, pub rows: i32, pub max_rows: i32, pub table_width: i32,
+                                    pub table_stride: i64, pub row_starts: *const i32, pub firsts: *const i32,
+                                    pub tables: *const i32, pub mask: i32, pub window: i32,
+                                    pub workspace: *mut c_void, pub workspace_bytes: u64 }
+#[repr(C)] pub struct FaPagedRows { pub keys: *mut c_void, pub values: *mut c_void, pub row_stride: i64,
+                                   pub head_stride: i64, pub dtype: i32 }
 #[repr(C)] pub struct FaKvCache { _private: [u8; 0] }
 
 #[link(name = "fa_attn")]
@@ -120,4 +130,24 @@ unsafe extern "C" {
     pub fn fa_normalize_and_rotate(prologue: *const FaPrologue, qkv: *const f32, qkv_stride: i64,
                                    out: *mut c_void, out_stride: i64, out_dtype: i32,
                                    stream: *mut c_void) -> i32;
+
+    // the paged cache: rows into pages and back, and the attention phase over them
+    pub fn fa_paged_workspace_bytes(cache: *const FaPagedCache, rows: i32, max_rows: i32,
+                                    bytes: *mut u64) -> i32;
+    pub fn fa_paged_check(cache: *const FaPagedCache, batch: *const FaPagedBatch) -> i32;
+    pub fn fa_attention_input_paged(cache: *const FaPagedCache, layer: i32, batch: *const FaPagedBatch,
+                                    rope: i32, angles: *const f32, norm: *const FaHeadNorm,
+                                    qkv: *const c_void, qkv_stride: i64, dtype: i32,
+                                    q_out: *mut c_void, q_out_stride: i64, stream: *mut c_void) -> i32;
+    pub fn fa_paged_write(cache: *const FaPagedCache, layer: i32, batch: *const FaPagedBatch,
+                          rows: *const FaPagedRows, stream: *mut c_void) -> i32;
+    pub fn fa_paged_read(cache: *const FaPagedCache, layer: i32, batch: *const FaPagedBatch,
+                         rows: *const FaPagedRows, stream: *mut c_void) -> i32;
+    pub fn fa_attend_paged(cache: *const FaPagedCache, layer: i32, batch: *const FaPagedBatch,
+                           q: *const c_void, q_stride: i64, dtype: i32, out: *mut c_void,
+                           out_stride: i64, out_dtype: i32, stream: *mut c_void) -> i32;
+    pub fn fa_attention_paged(cache: *const FaPagedCache, layer: i32, batch: *const FaPagedBatch,
+                              rope: i32, angles: *const f32, norm: *const FaHeadNorm,
+                              qkv: *const c_void, qkv_stride: i64, dtype: i32, out: *mut c_void,
+                              out_stride: i64, out_dtype: i32, stream: *mut c_void) -> i32;
 }
