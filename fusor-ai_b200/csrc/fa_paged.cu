@@ -300,7 +300,6 @@ int attend(const fa_paged_cache* c, int layer, const fa_paged_batch* b, const vo
     ca.counters += w.chunk_counters;
     if (!tokens) ca.token_cols = 0;
     const cudaError_t rc = fa::launch_paged_chunk(ca, sms, s);
-    if (rc == cudaErrorNotSupported) return fail(FA_ERR_UNSUPPORTED, "more than %d rows x heads", a.token_cols);
     if (rc != cudaSuccess) return cuda_fail(rc, "paged chunk launch");
   }
   if (tokens) {
