@@ -12,17 +12,27 @@
 //   softmax groups (4 warps for each query tile; thread = packed row = TMEM lane): Q rows into
 //     shared memory, then per key tile the scores from TMEM, masked where the tile is on an edge,
 //     online softmax with a lazy maximum, probabilities back to TMEM as bf16, and the output;
-//   loaders (4 warps): the pages' rows into the swizzled tiles that the products read. bf16 pages
-//     by cp.async straight to their places; 8-bit pages by cp.async into a raw buffer, then
-//     converted by the thread that fetched them: keys to f16 and values to bf16 integers (both
-//     exact), two pairs a word without a byte permutation: a word's bytes come out as 0, 2, 1, 3,
-//     and Q's rows (keys) and the output's columns (values) follow that order;
+//   loaders (two warps for the keys and two for the values; four and four over 8-bit pages): the pages' rows into the swizzled tiles
+//     that the products read. bf16 pages by cp.async straight to their places; 8-bit pages through
+//     registers, a tile's bytes loaded while the one before it is converted to f16;
 //   one warp: TMEM and the MMA issue (one thread).
-// 8-bit pages: a key's scale multiplies its score before the maximum, a value's scale its
-// probability before that is rounded to bf16; a query row is scaled by a power of two to f16's
-// range. Two tiles: as fmha2_kernel (fa_fmha2.cuh) the order per key tile is PV0, S0', PV1, S1',
-// so that one group's exponentials overlap the other's products. One tile: two score buffers,
-// S' is issued before PV.
+// 8-bit pages are dequantised to f16 (2^-12 of the value, an eighth of bf16's rounding) with each
+// tile's scales divided by a power of two, 2^k for the keys and 2^v for the values, that takes the
+// largest to [1, 2): no scale overflows, and one far below its tile's largest loses only what is
+// far below that one's products. 2^k multiplies the tile's scores (with the softmax's scale), v is
+// added to their base-2 exponents, so that the probabilities carry 2^v and the outputs of all
+// tiles stay in one unit; the row's sum takes 2^-v back out. A per-key multiplication of the
+// scores and of the probabilities instead (exact integers in the products) costs every softmax
+// thread 64 16-byte shared loads a tile. Probabilities are f16 too, up to 2^15 (the maximum is
+// lazy by 2^8, and 2^7 are added for f16's small end). A word's bytes come out as 0, 2, 1, 3
+// (two pairs without a byte permutation): Q's rows and the output's columns follow that order.
+//
+// A tile's scores are one product of 128 keys (of 64, the tensor core takes as long for each MMA:
+// it waits for Q's rows out of shared memory; 0.75 against 0.57 ms for 2048 rows of 32/8 heads of
+// 128 after 14336 positions of bf16 pages). The softmax and P.V go 64 keys at a time, so that P.V
+// of the first half runs during the second half's exponentials: per tile the order is PV0, S0',
+// PV1, S1' as in fmha2_kernel (fa_fmha2.cuh), one group's exponentials beside the other's
+// products. One query tile (head_dim 256): tiles of 64 keys, two score buffers, S' before PV.
 //
 // Keys that no row of a unit sees come as zeros (a page's stale end may hold anything). On edge
 // tiles, where some rows see a key and others do not, a value that is not finite would reach all
@@ -40,24 +50,23 @@ template <int D, bool Q8>
 struct ChunkShape {
   static constexpr int NQ = D == 256 ? 1 : 2;     // query tiles of a unit
   static constexpr int BM = 128;
-  static constexpr int BN = D == 256 ? 64 : 128;  // keys of a tile
-  static constexpr int kThreads = NQ == 2 ? 512 : 384;
+  static constexpr int BN = D == 256 ? 64 : 128;  // keys of a tile (a stage)
+  static constexpr int kSubs = BN / 64;           // blocks of 64 keys: the softmax's steps and P.V's
+  static constexpr int kLoad = Q8 ? 128 : 64;     // loaders of the keys, and of the values
+  static constexpr int kThreads = 2 * kLoad + NQ * 128 + 128;  // loaders, softmax, issuer
+  // Two query tiles: the registers of the warpgroups, which add up to the launch's (16 or 20 warps
+  // of 128 or 96): 2 x 88 + 2 x 112 + 80 = 5 x 96 and 128 + 2 x 144 + 96 = 4 x 128.
+  static constexpr int kLoadRegs = Q8 ? 88 : 128, kSoftmaxRegs = Q8 ? 112 : 144, kIssueRegs = Q8 ? 80 : 96;
   static constexpr int kDBlocks = D / 64;         // 128-byte swizzled blocks of a row
   static constexpr int kKStages = 2;
-  static constexpr int kVStages = Q8 && D >= 128 ? 1 : 2;  // what shared memory holds
+  static constexpr int kVStages = 2;
   static constexpr int kQBytes = BM * D * 2;
   static constexpr int kTileBytes = BN * D * 2;   // of a converted (or bf16) K or V tile
-  static constexpr int kRawBytes = Q8 ? BN * D : 0;
-  // scales of keys and of values, of four tiles: a tile's keys may arrive while a softmax group is
-  // still at the tile two before it, never three (its scores wait for that group's products)
-  static constexpr int kScaleBytes = Q8 ? 4 * 2 * BN * 4 : 0;
   static constexpr int kAt_K = NQ * kQBytes;
   static constexpr int kAt_V = kAt_K + kKStages * kTileBytes;
-  static constexpr int kAt_Raw = kAt_V + kVStages * kTileBytes;
-  static constexpr int kAt_Scales = kAt_Raw + 2 * kRawBytes;
-  static constexpr int kAt_Bars = kAt_Scales + kScaleBytes;
+  static constexpr int kAt_Bars = kAt_V + kVStages * kTileBytes;
   static constexpr size_t kSmemBytes = size_t(kAt_Bars) + 512 + 1024 /* alignment */;
-  static constexpr int kO = 128;  // TMEM column of O, after S (or the two S of 64 keys)
+  static constexpr int kO = 128;  // TMEM column of O, after 128 keys' scores or two of 64 keys'
   static_assert(kSmemBytes + 16 * 1024 <= 227 * 1024, "with the plan's static shared memory");
 };
 
@@ -65,8 +74,8 @@ struct ChunkShape {
 struct ChunkUnit {
   int row0, n, first;    // the sequence's span
   int q0;                // row offset of query tile 0 within the span
-  int tb[2], te[2];      // key tiles of each query tile (empty: tb == te)
-  int ub, ue;            // their union
+  int tb[2], te[2];      // 64-key blocks that each query tile sees (empty: tb == te)
+  int ub, ue;            // the key tiles that hold them
 };
 
 struct ChunkWalk {
@@ -106,11 +115,12 @@ __device__ __forceinline__ void chunk_unit(const PagedAttendArgs& a, const Paged
     int lo, hi, x;
     paged_keys(a.kind, a.window, sp.first + r0, end, &lo, &x);
     paged_keys(a.kind, a.window, sp.first + r1 - 1, end, &x, &hi);
-    u->tb[i] = lo / S::BN;
-    u->te[i] = (hi + S::BN - 1) / S::BN;
+    u->tb[i] = lo / 64;
+    u->te[i] = (hi + 63) / 64;
   }
-  u->ub = u->tb[0];
-  u->ue = max(u->te[0], u->te[1]);  // later rows see later keys
+  // later rows see later keys, without a gap
+  u->ub = u->tb[0] / S::kSubs;
+  u->ue = (max(u->te[0], u->te[1]) + S::kSubs - 1) / S::kSubs;
 }
 
 // Tiles of a whole unit.
@@ -159,23 +169,29 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
     paged_chunk_kernel(const __grid_constant__ PagedAttendArgs a) {
   using S = ChunkShape<D, Q8>;
   constexpr int NQ = S::NQ, BM = S::BM, BN = S::BN;
-  constexpr uint32_t kFmtS = Q8 ? 0u : 1u;  // f16 or bf16
-  constexpr uint32_t kIdescQK = tc::instr_desc(kFmtS, false, BN, BM);
-  constexpr uint32_t kIdescPV = tc::instr_desc(1u, true, D, BM);
+  constexpr uint32_t kFmt = Q8 ? 0u : 1u;  // f16 or bf16
+  constexpr uint32_t kIdescQK = tc::instr_desc(kFmt, false, BN, BM);
+  constexpr uint32_t kIdescPV = tc::instr_desc(kFmt, true, D, BM);
   constexpr int kTileCols = 256;  // TMEM columns of a query tile (two of them)
 
   extern __shared__ __align__(128) unsigned char smem_raw[];
   __shared__ int64_t before[kMaxPagedSequences + 1];
   __shared__ int64_t scratch[S::kThreads / 32];
-  __shared__ ChunkWalk start;
+  // each warp's walk and piece live in shared memory: the softmax needs its registers for a row
+  // of scores
+  __shared__ ChunkWalk walks[S::kThreads / 32];
+  __shared__ ChunkPiece pieces[S::kThreads / 32];
   __shared__ uint32_t poison[2][BN / 32];  // by V stage: keys with a value that is not finite
-  __shared__ uint32_t absent[4];  // by tile % 4: a bit per 16 keys whose page is out of range
+  // by tile % 4 (a tile's keys may arrive while a softmax group is still at the tile two before
+  // it, never three: its scores wait for that group's products): a bit per 16 keys whose page is
+  // out of range, and 8-bit pages' 2^k, v and 2^-v
+  __shared__ uint32_t absent[4];
+  __shared__ float4 units[4];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* sQ = smem;
   unsigned char* sK = smem + S::kAt_K;
   unsigned char* sV = smem + S::kAt_V;
-  float* scales = reinterpret_cast<float*>(smem + S::kAt_Scales);  // [tile % 4][K, V][BN]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kAt_Bars);
   uint64_t* q_full = bars;                     // [2]: by query tile, once a piece it is part of
   uint64_t* k_full = bars + 2;                 // [2]
@@ -183,24 +199,26 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
   uint64_t* v_full = k_empty + 2;              // [2]
   uint64_t* v_empty = v_full + 2;              // [2]
   uint64_t* s_full = v_empty + 2;              // [2]: by query tile, or by score buffer
-  uint64_t* p_full = s_full + 2;               // [2]: by query tile
-  uint64_t* o_done = p_full + 2;               // [2]: each P.V
+  uint64_t* p_full = s_full + 2;               // [4]: by query tile and block of the tile, or by
+                                               // score buffer
+  uint64_t* o_done = p_full + 4;               // [2]: each P.V
   uint64_t* o_final = o_done + 2;              // [2]: a piece's last P.V
   uint64_t* drained = o_final + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kLoader0 = NQ * 4, kMmaWarp = kLoader0 + 4;
+  constexpr int kSoftmax0 = 2 * S::kLoad / 32, kMmaWarp = kSoftmax0 + NQ * 4;  // the first warps load
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 128);
-      mbar_init(&k_full[i], 128);
+      mbar_init(&k_full[i], S::kLoad);
       mbar_init(&k_empty[i], 1);
-      mbar_init(&v_full[i], 128);
+      mbar_init(&v_full[i], S::kLoad);
       mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+      mbar_init(&p_full[2 * i], 128);
+      mbar_init(&p_full[2 * i + 1], 128);
       mbar_init(&o_done[i], 1);
       mbar_init(&o_final[i], 1);
     }
@@ -281,7 +299,7 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
       w.qt += 32;
     }
     w.unit0 = w.t - off;
-    if (lane == 0) start = w;
+    if (lane < S::kThreads / 32) walks[lane] = w;
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -289,31 +307,40 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
   const uint32_t tmem = *tmem_slot;
 
   if (!idle) {
-    ChunkWalk walk = start;
-    ChunkPiece pc;
+    const ChunkWalk& walk = walks[warp];
+    const ChunkPiece& pc = pieces[warp];
+    // the warp's next piece (the whole warp, except the MMA issuer's one thread)
+    auto next_piece = [&]() {
+      __syncwarp();
+      int more = 0;
+      if (lane == 0) more = chunk_next<D, Q8>(a, &walks[warp], &pieces[warp]);
+      return __shfl_sync(0xffffffffu, more, 0) != 0;
+    };
     if (warp >= kMmaWarp) {
       // ---- MMA issuer ------------------------------------------------------------------------
-      if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+      if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kIssueRegs));
       if (warp == kMmaWarp && lane == 0) {
         const uint64_t q_desc = tc::smem_desc_sw128(smem_u32(sQ), 16, 1024);
         const uint64_t k_desc = tc::smem_desc_sw128(smem_u32(sK), 16, 1024);
         const uint64_t v_desc = tc::smem_desc(smem_u32(sV), BN * 128, 1024, tc::kSwizzle128B);
         uint32_t tile = 0;        // K (and V) tiles consumed so far
         uint32_t queries[2] = {0, 0};  // pieces that each query tile was part of
-        uint32_t pv[2] = {0, 0};  // P.V products of each query tile so far
-        uint32_t sb = 0;          // one query tile: score products so far
+        uint32_t pv[2][2] = {{0, 0}, {0, 0}};  // P.V products by block of a tile and query tile
+        uint32_t sb = 0;                       // score products
         bool ok = true;
-        while (ok && chunk_next<D, Q8>(a, &walk, &pc)) {
-          const int n_tiles = pc.end - pc.begin;
+        while (ok && chunk_next<D, Q8>(a, &walks[warp], &pieces[warp])) {
+          const int n_tiles = pc.end - pc.begin, n = n_tiles * S::kSubs;  // 64-key blocks
+          const int at0 = pc.begin * S::kSubs;
           bool first[2] = {true, true};
-          auto part = [&](int i, int L) {
-            return pc.begin + L >= pc.u.tb[i] && pc.begin + L < pc.u.te[i];
-          };
+          const int b0 = pc.u.tb[0] - at0, e0 = pc.u.te[0] - at0;
+          const int b1 = pc.u.tb[1] - at0, e1 = pc.u.te[1] - at0;
+          auto part = [&](int i, int u) { return i == 0 ? u >= b0 && u < e0 : u >= b1 && u < e1; };
+          // scores of tile L (score buffer sb & 1 where there are two)
           auto issue_s = [&](int i, int L) {
             const uint64_t qd = q_desc + uint64_t(i * S::kQBytes >> 4);
             const uint64_t kd = k_desc + uint64_t((tile + L) % S::kKStages) * uint64_t(S::kTileBytes >> 4);
-            const int b = NQ == 2 ? i : int(sb & 1);
-            const uint32_t dst = tmem + (NQ == 2 ? i * kTileCols : b * BN);
+            const uint32_t b = NQ == 2 ? uint32_t(i) : sb & 1;
+            const uint32_t dst = tmem + (NQ == 2 ? uint32_t(i * kTileCols) : b * 64);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
               const int db = k / 4, koff = (k % 4) * 32;
@@ -323,21 +350,25 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
             tc::commit(&s_full[b]);
             ++sb;
           };
-          auto issue_pv = [&](int i, int L) {
-            if (!mbar_wait(&p_full[i], pv[i] & 1, a.err)) return false;
+          // block h of tile L: its probabilities are in columns 32 h of the scores' 128, or at the
+          // start of its score buffer
+          auto issue_pv = [&](int i, int L, int h) {
             const uint32_t vt = tile + L;
+            const uint32_t pb = NQ == 2 ? uint32_t(2 * i + h) : vt & 1;
+            if (!mbar_wait(&p_full[pb], NQ == 2 ? pv[h][i] & 1 : (vt >> 1) & 1, a.err)) return false;
+            ++pv[h][i];
             if (!mbar_wait(&v_full[vt % S::kVStages], (vt / S::kVStages) & 1, a.err)) return false;
             tc::fence_after_sync();
-            const uint32_t p_tmem = tmem + (NQ == 2 ? i * kTileCols : int(pv[i] & 1) * BN);
-            const uint32_t o_tmem = tmem + (NQ == 2 ? i * kTileCols : 0) + S::kO;
-            const uint64_t vd = v_desc + uint64_t(vt % S::kVStages) * uint64_t(S::kTileBytes >> 4);
+            const uint32_t p_tmem = tmem + (NQ == 2 ? uint32_t(i * kTileCols + h * 32) : pb * 64);
+            const uint32_t o_tmem = tmem + i * kTileCols + S::kO;
+            const uint64_t vd = v_desc + uint64_t(vt % S::kVStages) * uint64_t(S::kTileBytes >> 4) +
+                                uint64_t(h * (64 * 128) >> 4);
 #pragma unroll
-            for (int k = 0; k < BN / 16; ++k)
+            for (int k = 0; k < 4; ++k)
               tc::mma_ts<false>(o_tmem, p_tmem + k * 8, vd + uint64_t((k * 16 * 128) >> 4), kIdescPV,
                                 (!first[i] || k > 0) ? 1u : 0u);
             tc::commit(&o_done[i]);
             first[i] = false;
-            ++pv[i];
             return true;
           };
           auto wait_k = [&](int L) {
@@ -346,31 +377,40 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
             tc::fence_after_sync();
             return true;
           };
+          auto part_tile = [&](int i, int L) {
+            const int u0 = L * S::kSubs, u1 = u0 + S::kSubs;
+            return i == 0 ? u1 > b0 && u0 < e0 : u1 > b1 && u0 < e1;
+          };
 #pragma unroll
           for (int i = 0; i < NQ; ++i) {
-            if (min(pc.end, pc.u.te[i]) <= max(pc.begin, pc.u.tb[i])) continue;
+            if ((i == 0 ? min(n, e0) <= max(0, b0) : min(n, e1) <= max(0, b1))) continue;
             ok = ok && mbar_wait(&q_full[i], queries[i] & 1, a.err);
             ++queries[i];
           }
-          if (!ok) break;
-          ok = wait_k(0);
+          ok = ok && wait_k(0);
           if (!ok) break;
 #pragma unroll
           for (int i = 0; i < NQ; ++i)
-            if (part(i, 0)) issue_s(i, 0);
+            if (part_tile(i, 0)) issue_s(i, 0);
           tc::commit(&k_empty[tile % S::kKStages]);
           for (int L = 0; ok && L < n_tiles; ++L) {
             const bool next = L + 1 < n_tiles;
-            if (next && !wait_k(L + 1)) { ok = false; break; }
-            if constexpr (NQ == 2) {
-              if (part(0, L) && !issue_pv(0, L)) { ok = false; break; }
-              if (next && part(0, L + 1)) issue_s(0, L + 1);
-              if (part(1, L) && !issue_pv(1, L)) { ok = false; break; }
-              if (next && part(1, L + 1)) issue_s(1, L + 1);
-            } else {
-              if (next) issue_s(0, L + 1);
-              if (!issue_pv(0, L)) { ok = false; break; }
+            if constexpr (NQ == 1) {
+              // the next scores go to the other buffer before this tile's P.V
+              ok = !next || wait_k(L + 1);
+              if (ok && next) issue_s(0, L + 1);
             }
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+#pragma unroll
+              for (int h = 0; h < S::kSubs; ++h)
+                if (ok && part(i, L * S::kSubs + h)) ok = issue_pv(i, L, h);
+              if constexpr (NQ == 2) {
+                if (ok && next && i == 0) ok = wait_k(L + 1);
+                if (ok && next && part_tile(i, L + 1)) issue_s(i, L + 1);
+              }
+            }
+            if (!ok) break;
             if (next) tc::commit(&k_empty[(tile + L + 1) % S::kKStages]);
             tc::commit(&v_empty[(tile + L) % S::kVStages]);
           }
@@ -384,246 +424,258 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
         tc::commit(drained);
         mbar_wait(drained, 0, a.err);
       }
-    } else if (warp >= kLoader0) {
-      // ---- loaders ---------------------------------------------------------------------------
-      if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-      const int tid = threadIdx.x - kLoader0 * 32;
+    } else if (warp < kSoftmax0) {
+      // ---- loaders: the first half brings the keys, the other the values ----------------------
+      if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kLoadRegs));
+      const bool is_v = warp >= S::kLoad / 32;
+      const int tid = threadIdx.x & (S::kLoad - 1);
       constexpr int kRB = D * (Q8 ? 1 : 2), kCR = kRB / 16;  // a page row's bytes and chunks
-      constexpr int kPass = 128 / kCR;                       // rows of one pass of the threads
-      constexpr int kPasses = BN / kPass;
+      constexpr int kPass = S::kLoad / kCR;                  // rows of one pass of the threads (bf16)
+      constexpr int kSub = 16 / kPass, kGroups = BN / 16;    // passes of 16 keys, 16s of a tile
       const int shift = a.pool.page_shift;
       const int chunk = tid % kCR, prow = tid / kCR;
+      const unsigned char* pool = is_v ? a.pool.values : a.pool.keys;
+      uint64_t* full = is_v ? v_full : k_full;
+      uint64_t* empty = is_v ? v_empty : k_empty;
+      unsigned char* tiles = is_v ? sV : sK;
       uint32_t tile = 0;
-      bool ok = true, more = chunk_next<D, Q8>(a, &walk, &pc);
+      bool ok = true, more = next_piece();
       // one key tile's numbers: its first position, the keys that rows of the unit see, and lane
-      // i's page of keys 16 i .. 16 i + 15 (-1: none seen; -2: out of range, a bit of `absent`)
-      struct Tile {
-        int pos, lo, hi, lo_all, hi_all, h, page;
-        uint32_t absent;
-      };
-      auto look = [&](int at, Tile* t) {
+      // i's page of keys 16 i .. 16 i + 15 (-1: none seen; -2: out of range, a bit of `gone`)
+      int pos = 0, lo = 0, hi = 0, page = -1;
+      uint32_t gone = 0;
+      bool edge = false;
+      int ahead = -1, ahead_at = -1;  // the table's entry for the lane of the tile after the last
+      auto look = [&](int at) {
         const ChunkUnit& u = pc.u;
-        const int last = min(u.q0 + NQ * chunk_rows(a), u.n) - 1;
-        const int end = u.first + u.n;
-        paged_keys(a.kind, a.window, u.first + u.q0, end, &t->lo, &t->hi_all);
-        paged_keys(a.kind, a.window, u.first + last, end, &t->lo_all, &t->hi);
-        t->pos = at * BN;
-        t->h = pc.h;
-        t->page = -1;
-        const int p = t->pos + lane * 16;
-        if (lane < BN / 16 && p < t->hi && p + 16 > t->lo) {
-          // the span's table row: found by its sequence
-          t->page = __ldg(a.spans.tables + int64_t(walk.s) * a.spans.table_stride + (p >> shift));
-          if (!paged_page_ok(t->page, a.pool.pages)) {
+        const int last = min(u.q0 + NQ * chunk_rows(a), u.n) - 1, end = u.first + u.n;
+        int lo_all, hi_all;
+        paged_keys(a.kind, a.window, u.first + u.q0, end, &lo, &hi_all);
+        paged_keys(a.kind, a.window, u.first + last, end, &lo_all, &hi);
+        pos = at * BN;
+        edge = pos < lo_all || pos + BN > hi_all;
+        page = -1;
+        const int p = pos + lane * 16;
+        const int* table = a.spans.tables + int64_t(walk.s) * a.spans.table_stride;
+        const int read = ahead_at == at ? ahead : -3;
+        // the next tile's entries are fetched now (within the piece: its own sequence's)
+        ahead_at = at + 1 < pc.end ? at + 1 : -1;
+        const int pn = p + BN;
+        ahead = -1;
+        if (ahead_at >= 0 && lane < kGroups && pn < hi && pn + 16 > lo) ahead = __ldg(table + (pn >> shift));
+        if (lane < kGroups && p < hi && p + 16 > lo) {
+          page = read != -3 ? read : __ldg(table + (p >> shift));
+          if (!paged_page_ok(page, a.pool.pages)) {
             atomicOr(a.err, kErrPagedPage);
-            t->page = -2;
+            page = -2;
           }
         }
-        t->absent = __ballot_sync(0xffffffffu, t->page == -2);
+        gone = __ballot_sync(0xffffffffu, page == -2);
       };
-      // the thread's chunks of the tile's key (or value) rows, as one group of copies
-      auto fetch = [&](const Tile& t, const unsigned char* base, uint32_t dst) {
-#pragma unroll
-        for (int i = 0; i < kPasses; ++i) {
-          const int row = prow + i * kPass;
-          const int page = __shfl_sync(0xffffffffu, t.page, row >> 4);
-          const int p = t.pos + row;
-          const bool there = page >= 0 && p >= t.lo && p < t.hi;
-          const int64_t at = ((int64_t(max(page, 0)) * kvh + t.h) << shift) + (p & ((1 << shift) - 1));
-          const uint32_t to = Q8 ? uint32_t((tid + i * 128) * 16)
-                                 : uint32_t((chunk / 8) * (BN * 128) + row * 128 +
-                                            (((chunk % 8) ^ (row & 7)) * 16));
-          cp_async16(dst + to, base + (there ? at * kRB + chunk * 16 : 0), there ? 16u : 0u);
-        }
-        cp_async_commit();
+      // Row `row` of 16 keys from position p0 is seen by some row of the unit.
+      auto seen = [&](int p0, int row) { return p0 + row >= lo && p0 + row < hi; };
+      // A stage's products are done (its marks are cleared). The value loaders decide as one, so
+      // that a wait that gave up cannot leave the others at their barrier; the key loaders need
+      // none.
+      auto vacant = [&](int st, uint32_t parity) {
+        const bool there = mbar_wait(&empty[st], parity, a.err);
+        if (!is_v) return __all_sync(0xffffffffu, there) != 0;
+        if (there && tid < BN / 32) poison[st][tid] = 0;
+        return !named_sync_or(1, S::kLoad, !there);
       };
-      // a value tile on an edge: what is not finite taken out, its key marked
-      auto scrub_bf16 = [&](unsigned char* dst, int stage) {
-#pragma unroll 1
-        for (int i = 0; i < kPasses; ++i) {
-          const int row = prow + i * kPass;
-          uint4* p = reinterpret_cast<uint4*>(dst + (chunk / 8) * (BN * 128) + row * 128 +
-                                              (((chunk % 8) ^ (row & 7)) * 16));
-          uint4 v = *p;
-          uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          bool bad = false;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            if ((w[x] & 0x7F80u) == 0x7F80u) { w[x] &= 0xFFFF0000u; bad = true; }
-            if ((w[x] & 0x7F800000u) == 0x7F800000u) { w[x] &= 0xFFFFu; bad = true; }
-          }
-          if (bad) {
-            *p = make_uint4(w[0], w[1], w[2], w[3]);
-            atomicOr(&poison[stage][row >> 5], 1u << (row & 31));
-          }
-        }
-      };
-      auto publish = [&](uint64_t* bar) {
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(bar);
-      };
-      // A stage's products are done (its marks are cleared): decided by all loaders as one, so that
-      // a wait that gave up cannot leave the others at this barrier.
-      auto vacant = [&](uint64_t* bar, uint32_t parity, int marks = -1) {
-        const bool there = mbar_wait(bar, parity, a.err);
-        if (there && marks >= 0 && tid < BN / 32) poison[marks][tid] = 0;
-        return !named_sync_or(1, 128, !there);
-      };
-      auto edge = [&](const Tile& t) { return t.pos < t.lo_all || t.pos + BN > t.hi_all; };
-
+      auto stage_of = [&]() { return int(tile % (is_v ? S::kVStages : S::kKStages)); };
+      auto phase_of = [&]() { return ((tile / (is_v ? S::kVStages : S::kKStages)) & 1) ^ 1; };
       if constexpr (!Q8) {
-        // slots K0, V0, K1, V1, ...: each published when the next one's copies are on their way
-        uint64_t* pending = nullptr;
-        unsigned char* pending_v = nullptr;  // a V tile on an edge, to be scrubbed
-        int pending_stage = 0;
-        auto finish = [&]() {
-          if (pending == nullptr) return;
-          if (pending_v != nullptr) scrub_bf16(pending_v, pending_stage);
-          publish(pending);
-        };
-        Tile t;
-        if (more) look(pc.begin, &t);
         while (more && ok) {
-          for (int at = pc.begin; at < pc.end; ++at, ++tile) {
-            const int ks = tile % S::kKStages, vs = tile % S::kVStages;
-            if (!vacant(&k_empty[ks], ((tile / S::kKStages) & 1) ^ 1)) { ok = false; break; }
-            fetch(t, a.pool.keys, smem_u32(sK) + ks * S::kTileBytes);
-            if (tid == 0) absent[tile & 3] = t.absent;
-            cp_async_wait<1>();
-            finish();
-            pending = &k_full[ks];
-            pending_v = nullptr;
-            if (!vacant(&v_empty[vs], ((tile / S::kVStages) & 1) ^ 1, vs)) { ok = false; break; }
-            fetch(t, a.pool.values, smem_u32(sV) + vs * S::kTileBytes);
-            const bool e = edge(t);
-            if (at + 1 < pc.end) look(at + 1, &t);
-            cp_async_wait<1>();
-            finish();
-            pending = &v_full[vs];
-            pending_v = e ? sV + vs * S::kTileBytes : nullptr;
-            pending_stage = vs;
+          const int begin = pc.begin, end = pc.end;
+          for (int at = begin; at < end; ++at, ++tile) {
+            look(at);
+            const int st = stage_of();
+            if (!vacant(st, phase_of())) { ok = false; break; }
+            const uint32_t dst = smem_u32(tiles) + st * S::kTileBytes + (chunk / 8) * (BN * 128);
+#pragma unroll
+            for (int gr = 0; gr < kGroups; ++gr) {
+              const int pg = __shfl_sync(0xffffffffu, page, gr), p0 = pos + gr * 16;
+              const int64_t row0 = ((int64_t(max(pg, 0)) * kvh + pc.h) << shift) + (p0 & ((1 << shift) - 1));
+              const unsigned char* src = pool + (row0 + prow) * kRB + chunk * 16;
+#pragma unroll
+              for (int j = 0; j < kSub; ++j) {
+                const int row = gr * 16 + prow + j * kPass;
+                const bool there = pg >= 0 && seen(p0, prow + j * kPass);
+                cp_async16(dst + row * 128 + (((chunk % 8) ^ (row & 7)) * 16), src + j * kPass * kRB,
+                           there ? 16u : 0u);
+              }
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
+            if (is_v && edge) {
+              // what is not finite taken out, its key marked
+#pragma unroll 1
+              for (int i = 0; i < kGroups * kSub; ++i) {
+                const int row = prow + i * kPass;
+                uint4* p = reinterpret_cast<uint4*>(tiles + st * S::kTileBytes + (chunk / 8) * (BN * 128) +
+                                                    row * 128 + (((chunk % 8) ^ (row & 7)) * 16));
+                const uint4 v = *p;
+                uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                bool bad = false;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                  if ((w[x] & 0x7F80u) == 0x7F80u) { w[x] &= 0xFFFF0000u; bad = true; }
+                  if ((w[x] & 0x7F800000u) == 0x7F800000u) { w[x] &= 0xFFFFu; bad = true; }
+                }
+                if (bad) {
+                  *p = make_uint4(w[0], w[1], w[2], w[3]);
+                  atomicOr(&poison[st][row >> 5], 1u << (row & 31));
+                }
+              }
+            }
+            if (!is_v && tid == 0) absent[tile & 3] = gone;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(&full[st]);
           }
-          if (!ok) break;
-          more = chunk_next<D, Q8>(a, &walk, &pc);
-          if (more) look(pc.begin, &t);
+          if (ok) more = next_piece();
         }
-        cp_async_wait<0>();
-        if (ok) finish();
       } else {
-        unsigned char* raw = smem + S::kAt_Raw;  // a key tile, then a value tile
-        // a tile's copies are under way while the one before it is converted
-        Tile t, next;
-        float ksc = 0.0f, vsc = 0.0f;  // thread i: key i's scales of tile t
-        auto begin_tile = [&](const Tile& x, float* k, float* v) {
-          *k = *v = 0.0f;
-          const int page = __shfl_sync(0xffffffffu, x.page, (tid & (BN - 1)) >> 4);
-          const int p = x.pos + (tid & (BN - 1));
-          if (page >= 0 && p >= x.lo && p < x.hi) {
-            const int64_t at = ((int64_t(page) * kvh + x.h) << shift) + (p & ((1 << shift) - 1));
-            *k = __ldcg(a.pool.key_scales + at);
-            *v = __ldcg(a.pool.value_scales + at);
+        // A tile's bytes wait in registers, loaded while the tile before it is converted. A warp
+        // takes 8 rows x 64 bytes at a time (lane: row lane % 8, chunk lane / 8), so that its
+        // 16-byte stores into the swizzled rows meet no bank twice.
+        constexpr int kWide = kCR / 4;              // 64-byte columns of a row: 1, 2 or 4
+        constexpr int kItems = BN / 8 * kWide / 4;  // of a warp
+        constexpr int kKeys = BN / 32;
+        const int w4 = warp & 3, r8 = lane & 7, c4 = lane >> 3;
+        uint4 raw[kItems];
+        float ks[kKeys], vs[kKeys];  // scales of keys lane, lane + 32, ... (ks: key loaders)
+        // item k of the warp: rows 8 rg .. 8 rg + 7, chunks 4 cg .. 4 cg + 3
+        auto rg_of = [&](int k) { return kWide == 1 ? 4 * k + w4 : kWide == 2 ? 2 * k + (w4 >> 1) : k; };
+        const int cg = kWide == 1 ? 0 : kWide == 2 ? w4 & 1 : w4;
+        auto row_of = [&](int gr) {
+          const int pg = __shfl_sync(0xffffffffu, page, gr);
+          return ((int64_t(max(pg, 0)) * kvh + pc.h) << shift) + ((pos + gr * 16) & ((1 << shift) - 1));
+        };
+        // (rows that are not seen get a zero scale: what their bytes are, or page 0's in their
+        // place, does not matter)
+        auto load = [&](int k) {
+          raw[k] = __ldg(reinterpret_cast<const uint4*>(
+              pool + (row_of(rg_of(k) >> 1) + (rg_of(k) & 1) * 8 + r8) * kRB + (cg * 4 + c4) * 16));
+        };
+        auto load_scales = [&]() {
+#pragma unroll
+          for (int x = 0; x < kKeys; ++x) {
+            const int row = lane + 32 * x, p = pos + row;
+            const int pg = __shfl_sync(0xffffffffu, page, row >> 4);
+            const bool there = pg >= 0 && p >= lo && p < hi;
+            const int64_t at = ((int64_t(max(pg, 0)) * kvh + pc.h) << shift) + (p & ((1 << shift) - 1));
+            const float v = __ldg(a.pool.value_scales + at);
+            vs[x] = there ? v : 0.0f;
+            if (!is_v) {
+              const float k = __ldg(a.pool.key_scales + at);
+              ks[x] = there ? k : 0.0f;
+            }
           }
         };
+        // the exponent of the largest finite scale
+        auto exponent = [&](const float (&x)[kKeys]) {
+          float top = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i)
+            top = fmaxf(top, fabsf(x[i]) <= 3.402823466e38f ? fabsf(x[i]) : 0.0f);
+          const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+          return bits == 0 ? 0 : min(max(int(bits >> 23) - 127, -120), 120);
+        };
+        auto power = [](int e) { return __uint_as_float(uint32_t(127 + e) << 23); };
+        int at = pc.begin, end = pc.end;
         if (more) {
-          look(pc.begin, &t);
-          fetch(t, a.pool.keys, smem_u32(raw));
-          fetch(t, a.pool.values, smem_u32(raw) + S::kRawBytes);
-          begin_tile(t, &ksc, &vsc);
+          look(at);
+#pragma unroll
+          for (int k = 0; k < kItems; ++k) load(k);
+          load_scales();
         }
-        while (more && ok) {
-          for (int at = pc.begin; at < pc.end;) {
-            const int ks = tile % S::kKStages, vs = tile % S::kVStages;
-            const bool e = edge(t);
-            // the tile after this one, of this piece or the next
-            ++at;
-            bool have = true;
-            if (at == pc.end) {
-              have = more = chunk_next<D, Q8>(a, &walk, &pc);
-              at = pc.begin;
-            }
-            if (have) look(at, &next);
-            float nk = 0.0f, nv = 0.0f;
-            if (have) begin_tile(next, &nk, &nv);
-            // keys
-            if (!vacant(&k_empty[ks], ((tile / S::kKStages) & 1) ^ 1)) { ok = false; break; }
-            cp_async_wait<1>();
-            {
-              unsigned char* dst = sK + ks * S::kTileBytes;
+        while (more) {
+          const int st = stage_of();
+          const bool was_edge = edge;
+          const uint32_t was_gone = gone;
+          const int ev = exponent(vs), ek = is_v ? 0 : exponent(ks);
+          // this tile's scales as f16 pairs
+          const float down = power(is_v ? -ev : -ek);
+          __half2 hs[kKeys];
+          uint32_t bad = 0;  // keys lane + 32 x whose value scale is not finite
 #pragma unroll
-              for (int i = 0; i < kPasses; ++i) {
-                const int row = prow + i * kPass;
-                const uint4 v = *reinterpret_cast<const uint4*>(raw + (tid + i * 128) * 16);
-                const int c0 = chunk * 2;
-                unsigned char* p = dst + (c0 / 8) * (BN * 128) + row * 128;
-                *reinterpret_cast<uint4*>(p + ((c0 % 8) ^ (row & 7)) * 16) =
-                    make_uint4(bytes_to_f16(v.x), bytes_to_f16(v.x >> 8), bytes_to_f16(v.y),
-                               bytes_to_f16(v.y >> 8));
-                *reinterpret_cast<uint4*>(p + ((c0 % 8 + 1) ^ (row & 7)) * 16) =
-                    make_uint4(bytes_to_f16(v.z), bytes_to_f16(v.z >> 8), bytes_to_f16(v.w),
-                               bytes_to_f16(v.w >> 8));
-              }
-            }
-            if (tid < BN) scales[(tile & 3) * 2 * BN + tid] = ksc;
-            if (tid == 0) absent[tile & 3] = t.absent;
-            publish(&k_full[ks]);
-            if (have) fetch(next, a.pool.keys, smem_u32(raw)); else cp_async_commit();
-            // values
-            if (!vacant(&v_empty[vs], ((tile / S::kVStages) & 1) ^ 1, vs)) { ok = false; break; }
-            cp_async_wait<1>();
-            {
-              unsigned char* dst = sV + vs * S::kTileBytes;
-#pragma unroll
-              for (int i = 0; i < kPasses; ++i) {
-                const int row = prow + i * kPass;
-                const uint4 v = *reinterpret_cast<const uint4*>(raw + S::kRawBytes + (tid + i * 128) * 16);
-                const int c0 = chunk * 2;
-                unsigned char* p = dst + (c0 / 8) * (BN * 128) + row * 128;
-                *reinterpret_cast<uint4*>(p + ((c0 % 8) ^ (row & 7)) * 16) =
-                    make_uint4(bytes_to_bf16(v.x), bytes_to_bf16(v.x >> 8), bytes_to_bf16(v.y),
-                               bytes_to_bf16(v.y >> 8));
-                *reinterpret_cast<uint4*>(p + ((c0 % 8 + 1) ^ (row & 7)) * 16) =
-                    make_uint4(bytes_to_bf16(v.z), bytes_to_bf16(v.z >> 8), bytes_to_bf16(v.w),
-                               bytes_to_bf16(v.w >> 8));
-              }
-            }
-            if (tid < BN) {
-              if (e && !(fabsf(vsc) <= 3.402823466e38f)) {
-                vsc = 0.0f;
-                atomicOr(&poison[vs][tid >> 5], 1u << (tid & 31));
-              }
-              scales[(tile & 3) * 2 * BN + BN + tid] = vsc;
-            }
-            publish(&v_full[vs]);
-            if (have) fetch(next, a.pool.values, smem_u32(raw) + S::kRawBytes); else cp_async_commit();
-            ++tile;
-            t = next;
-            ksc = nk;
-            vsc = nv;
-            if (!have) break;
+          for (int x = 0; x < kKeys; ++x) {
+            const float sc = is_v ? vs[x] : ks[x];
+            const bool drop = is_v && was_edge && !(fabsf(sc) <= 3.402823466e38f);
+            bad |= uint32_t(drop) << x;
+            hs[x] = __float2half2_rn(drop ? 0.0f : sc * down);
           }
+          // the tile after this one, of this piece or the next
+          if (++at == end) {
+            more = next_piece();
+            at = pc.begin;
+            end = pc.end;
+          }
+          if (more) {
+            look(at);
+            load_scales();
+          }
+          if (!vacant(st, phase_of())) { ok = false; break; }
+          unsigned char* dst = tiles + st * S::kTileBytes;
+          const int c0 = (cg * 4 + c4) * 2;
+          dst += (c0 / 8) * (BN * 128) + r8 * 128;
+          const int to0 = ((c0 % 8) ^ r8) * 16, to1 = ((c0 % 8 + 1) ^ r8) * 16;
+#pragma unroll
+          for (int k = 0; k < kItems; ++k) {
+            constexpr int kPer = kWide == 1 ? 1 : kWide == 2 ? 2 : 4;  // items of 32 rows
+            const __half2 h = __shfl_sync(0xffffffffu, hs[k / kPer], (rg_of(k) * 8 + r8) & 31);
+            const uint4 v = raw[k];
+            load(k);  // (this tile's again after the last: no branch around the loads)
+            auto half = [&](uint32_t w) {
+              const uint32_t y = bytes_to_f16(w);
+              const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&y), h);
+              return *reinterpret_cast<const uint32_t*>(&r);
+            };
+            unsigned char* p = dst + rg_of(k) * 1024;
+            *reinterpret_cast<uint4*>(p + to0) =
+                make_uint4(half(v.x), half(v.x >> 8), half(v.y), half(v.y >> 8));
+            *reinterpret_cast<uint4*>(p + to1) =
+                make_uint4(half(v.z), half(v.z >> 8), half(v.w), half(v.w >> 8));
+          }
+          if (is_v && was_edge && warp == 4) {
+#pragma unroll
+            for (int x = 0; x < kKeys; ++x)
+              if ((bad >> x) & 1u) atomicOr(&poison[st][x], 1u << lane);
+          }
+          if (!is_v && tid == 0) {
+            absent[tile & 3] = was_gone;
+            units[tile & 3] = make_float4(power(ek), float(ev), power(-ev), 0.0f);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          mbar_arrive(&full[st]);
+          ++tile;
         }
-        cp_async_wait<0>();
       }
     } else {
       // ---- softmax and output of query tile i ------------------------------------------------
-      if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-      const int i = NQ == 2 ? warp >> 2 : 0;
+      if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftmaxRegs));
+      const int i = NQ == 2 ? (warp - kSoftmax0) >> 2 : 0;
       const int wq = warp & 3;             // the TMEM lane quarter that this warp may access
       const int p = wq * 32 + lane;        // packed row
       const int rows = chunk_rows(a);
       const int pr = p / a.group, ph = p % a.group;
       const uint32_t lane_base = tmem + (NQ == 2 ? i * kTileCols : 0) + (uint32_t(wq * 32) << 16);
       const uint32_t o_base = lane_base + S::kO;
-      uint32_t sc = 0;     // this query tile's score tiles so far
+      uint32_t sc = 0;     // this query tile's blocks so far
+      uint32_t st = 0;     // and score products
       uint32_t finals = 0; // pieces that it took part in
       uint32_t tile = 0;   // K (and V) tiles so far
       bool ok = true;
-      while (ok && chunk_next<D, Q8>(a, &walk, &pc)) {
+      while (ok && next_piece()) {
         const int n_tiles = pc.end - pc.begin;
+        const int n = n_tiles * S::kSubs;  // 64-key blocks
+        const int my_b = pc.u.tb[i] - pc.begin * S::kSubs, my_e = pc.u.te[i] - pc.begin * S::kSubs;
+        const int kp0 = pc.begin * BN;  // the piece's first key
         const int r = pc.u.q0 + i * rows + pr;  // row of the span
         const bool valid = pr < rows && r < pc.u.n;
         float scale = a.scale_log2;
-        if (min(pc.end, pc.u.te[i]) > max(pc.begin, pc.u.tb[i])) {
+        if (min(n, my_e) > max(0, my_b)) {
           // the packed row's query, zeros for a row that is none; over 8-bit pages f16, scaled by
           // a power of two, its elements in the converted keys' order
           const int64_t at = int64_t(pc.u.row0 + r) * a.q_stride + int64_t(pc.h * a.group + ph) * D;
@@ -702,94 +754,84 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
         }
         float m_used = -INFINITY, l_sum = 0.0f;
         bool poisoned = false;
-        int c = 0;  // score tiles of this piece so far
-        for (int L = 0; L < n_tiles; ++L) {
-          const int at = pc.begin + L;
-          if (at < pc.u.tb[i] || at >= pc.u.te[i]) continue;
-          const int kp = at * BN;
-          const uint32_t s_base = lane_base + (NQ == 2 ? 0 : int(sc & 1) * BN);
-          // every decision before a whole-warp tcgen05 instruction is made warp-uniform
-          const bool there = NQ == 2 ? mbar_wait(&s_full[i], sc & 1, a.err)
-                                     : mbar_wait(&s_full[sc & 1], (sc >> 1) & 1, a.err);
-          if (!__all_sync(0xffffffffu, there)) { ok = false; break; }
-          tc::fence_after_sync();
-          uint32_t sreg[BN];
-#pragma unroll
-          for (int x = 0; x < BN / 64; ++x)
-            tc::tmem_ld64_wait(s_base + x * 64, *reinterpret_cast<uint32_t(*)[64]>(&sreg[x * 64]));
-          float* s = reinterpret_cast<float*>(sreg);
-          const float* sc_k = scales + ((tile + L) & 3) * 2 * BN;
-          if constexpr (Q8) {
-#pragma unroll
-            for (int x = 0; x < BN; x += 4) {
-              const float4 k = *reinterpret_cast<const float4*>(sc_k + x);
-              s[x] *= k.x; s[x + 1] *= k.y; s[x + 2] *= k.z; s[x + 3] *= k.w;
-            }
+        int c = 0;  // blocks of this piece so far
+        const int u_end = min(n, my_e);
+        for (int u = max(0, my_b); u < u_end; ++u) {
+          const int L = u / S::kSubs;
+          const int kp = kp0 + u * 64;
+          const int h = u % S::kSubs;
+          const uint32_t buf = (tile + L) & 1;  // one query tile: the score buffer
+          const uint32_t s_base = lane_base + (NQ == 2 ? uint32_t(h) * 64 : buf * 64);
+          const uint32_t p_base = lane_base + (NQ == 2 ? uint32_t(h) * 32 : buf * 64);
+          if (h == 0 || c == 0) {
+            // every decision before a whole-warp tcgen05 instruction is made warp-uniform
+            const bool there = NQ == 2 ? mbar_wait(&s_full[i], st & 1, a.err)
+                                       : mbar_wait(&s_full[buf], ((tile + L) >> 1) & 1, a.err);
+            if (!__all_sync(0xffffffffu, there)) { ok = false; break; }
+            ++st;
+            tc::fence_after_sync();
           }
-          const bool all_in = !valid || (kp >= runs.b0 && kp + BN <= runs.b0 + runs.n0);
-          if (!all_in) mask_scores<BN>(runs, kp, s);
+          // the tile's units: its scores' scale, what its exponents and its sum take besides
+          float scale_t = scale, up_t = 0.0f, down_t = 1.0f;
+          if constexpr (Q8) {
+            const float4 un = units[(tile + L) & 3];
+            scale_t = scale * un.x;
+            up_t = un.y;
+            down_t = un.z;
+          }
           const uint32_t gone = *const_cast<const volatile uint32_t*>(&absent[(tile + L) & 3]);
+          uint32_t sreg[64];
+          tc::tmem_ld64_wait(s_base, sreg);
+          float* s = reinterpret_cast<float*>(sreg);
+          const bool all_in = !valid || (kp >= runs.b0 && kp + 64 <= runs.b0 + runs.n0);
+          if (!all_in) mask_scores<64>(runs, kp, s);
           if (gone != 0) {
 #pragma unroll
-            for (int x = 0; x < BN; ++x)
-              if ((gone >> (x >> 4)) & 1u) s[x] = -INFINITY;
+            for (int x = 0; x < 64; ++x)
+              if ((gone >> (h * 4 + (x >> 4))) & 1u) s[x] = -INFINITY;
           }
-          float mx0 = fmax3(s[0], s[1], s[2]), mx1 = fmax3(s[3], s[4], s[5]);
-          float mx2 = fmax3(s[6], s[7], s[8]), mx3 = fmax3(s[9], s[10], s[11]);
+          float mx0 = s[0], mx1 = s[1], mx2 = s[2], mx3 = s[3];
 #pragma unroll
-          for (int x = 12; x < BN - 4; x += 8) {
+          for (int x = 4; x < 60; x += 8) {
             mx0 = fmax3(mx0, s[x], s[x + 1]);
             mx1 = fmax3(mx1, s[x + 2], s[x + 3]);
             mx2 = fmax3(mx2, s[x + 4], s[x + 5]);
             mx3 = fmax3(mx3, s[x + 6], s[x + 7]);
           }
-          mx0 = fmax3(mx0, s[BN - 4], s[BN - 3]);
-          mx1 = fmax3(mx1, s[BN - 2], s[BN - 1]);
-          const float m_tile = fmax3(mx0, mx1, fmaxf(mx2, mx3)) * scale;
+          mx0 = fmax3(mx0, s[60], s[61]);
+          mx1 = fmax3(mx1, s[62], s[63]);
+          const float m_tile = fmaf(fmax3(mx0, mx1, fmaxf(mx2, mx3)), scale_t, up_t);
           float alpha = 1.0f;
           if (m_tile > m_used + 8.0f || (m_used == -INFINITY && m_tile > -INFINITY)) {
             if (m_used > -INFINITY) alpha = exp2_approx(m_used - m_tile);
             m_used = m_tile;
           }
           const float ms = m_used == -INFINITY ? 0.0f : m_used;
-          const float2 scale2 = make_float2(scale, scale), neg2 = make_float2(-ms, -ms);
+          const float off = Q8 ? up_t - ms + 7.0f : -ms;
+          const float2 scale2 = make_float2(scale_t, scale_t), neg2 = make_float2(off, off);
           float2 sum2a = make_float2(0.0f, 0.0f), sum2b = make_float2(0.0f, 0.0f);
-          const float* sc_v = sc_k + BN;
-          if constexpr (Q8) {
-            // the values' scales are there with the values
-            const uint32_t vt = tile + L;
-            const bool v_there = mbar_wait(&v_full[vt % S::kVStages], (vt / S::kVStages) & 1, a.err);
-            if (!__all_sync(0xffffffffu, v_there)) { ok = false; break; }
-          }
 #pragma unroll
-          for (int x = 0; x < BN; x += 4) {
+          for (int x = 0; x < 64; x += 4) {
             const float2 x0 = __ffma2_rn(make_float2(s[x], s[x + 1]), scale2, neg2);
             const float2 x1 = __ffma2_rn(make_float2(s[x + 2], s[x + 3]), scale2, neg2);
-            float2 p0 = make_float2(exp2_approx(x0.x), exp2_approx(x0.y));
-            float2 p1 = make_float2(exp2_approx(x1.x), exp2_approx(x1.y));
+            const float2 p0 = make_float2(exp2_approx(x0.x), exp2_approx(x0.y));
+            const float2 p1 = make_float2(exp2_approx(x1.x), exp2_approx(x1.y));
             sum2a = __fadd2_rn(sum2a, p0);
             sum2b = __fadd2_rn(sum2b, p1);
-            if constexpr (Q8) {
-              const float4 v = *reinterpret_cast<const float4*>(sc_v + x);
-              p0 = __fmul2_rn(p0, make_float2(v.x, v.y));
-              p1 = __fmul2_rn(p1, make_float2(v.z, v.w));
-            }
-            sreg[x / 2] = tc::pack_bf16(p0.x, p0.y);
-            sreg[x / 2 + 1] = tc::pack_bf16(p1.x, p1.y);
+            sreg[x / 2] = Q8 ? pack_f16(p0.x, p0.y) : tc::pack_bf16(p0.x, p0.y);
+            sreg[x / 2 + 1] = Q8 ? pack_f16(p1.x, p1.y) : tc::pack_bf16(p1.x, p1.y);
           }
-#pragma unroll
-          for (int x = 0; x < BN / 64; ++x)
-            tc::tmem_st32(s_base + x * 32, *reinterpret_cast<const uint32_t(*)[32]>(&sreg[x * 32]));
-          l_sum = l_sum * alpha + ((sum2a.x + sum2a.y) + (sum2b.x + sum2b.y));
-          if (kp < lo_all || kp + BN > hi_all) {
+          tc::tmem_st32(p_base, *reinterpret_cast<const uint32_t(*)[32]>(&sreg[0]));
+          l_sum = l_sum * alpha + ((sum2a.x + sum2a.y) + (sum2b.x + sum2b.y)) * down_t;
+          if (kp0 + L * BN < lo_all || kp0 + (L + 1) * BN > hi_all) {
             // an edge tile (of the unit, as the loaders see it): keys that they marked
             const uint32_t vt = tile + L;
             const bool v_there = mbar_wait(&v_full[vt % S::kVStages], (vt / S::kVStages) & 1, a.err);
             if (!__all_sync(0xffffffffu, v_there)) { ok = false; break; }
             const volatile uint32_t* marks = poison[vt % S::kVStages];
 #pragma unroll
-            for (int w = 0; w < BN / 32; ++w)
-              if (marks[w] & run_word(runs.b0, runs.n0, kp, w)) poisoned = true;
+            for (int w = 0; w < 2; ++w)
+              if (marks[h * 2 + w] & run_word(runs.b0, runs.n0, kp, w)) poisoned = true;
           }
           if (__any_sync(0xffffffffu, alpha != 1.0f) && c > 0) {
             // O holds the products of this piece's earlier tiles, the last of which may still run
@@ -807,7 +849,7 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
           }
           tc::tmem_wait_st();
           tc::fence_before_sync();
-          mbar_arrive(&p_full[i]);
+          mbar_arrive(&p_full[NQ == 2 ? uint32_t(2 * i + h) : buf]);
           ++c;
           ++sc;
         }

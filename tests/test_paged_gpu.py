@@ -305,8 +305,6 @@ def run_attend(shape, spans, dtype, mask, rows_dt="bf16", out_dt="bf16", layer=0
     cache.attend(layer, batch, q, out)
     fa.device_status()
     bits = 0.0 if rows_dt == "bf16" else (2.0 ** -11 if dtype == fa.Q8 else HALF16)
-    if rows_dt == "f32" and spans.max_rows * (shape.heads // shape.kv_heads) > 16:
-        bits = HALF16  # chunks round their queries to bf16
     want, tol = reference(cache, layer, spans, q.double(), mask, bits)
     n = spans.real_rows
     check_close(out[:n], want[:n], tol[:n], out_dt == "bf16")
