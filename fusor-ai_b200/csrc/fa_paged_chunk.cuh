@@ -12,14 +12,15 @@
 //   softmax groups (4 warps for each query tile; thread = packed row = TMEM lane): Q rows into
 //     shared memory, then per key tile the scores from TMEM, masked where the tile is on an edge,
 //     online softmax with a lazy maximum, probabilities back to TMEM as bf16, and the output;
-//   loaders (two warps for the keys and two for the values; four and four over 8-bit pages): the pages' rows into the swizzled tiles
-//     that the products read. bf16 pages by cp.async straight to their places; 8-bit pages through
-//     registers, a tile's bytes loaded while the one before it is converted to f16;
+//   loaders (two warps for the keys and two for the values; four and four over 8-bit pages): the
+//     pages' rows into the swizzled tiles that the products read. bf16 pages by cp.async straight
+//     to their places; 8-bit pages through registers, a tile's bytes loaded while the one before
+//     it is converted to f16;
 //   one warp: TMEM and the MMA issue (one thread).
 // 8-bit pages are dequantised to f16 (2^-12 of the value, an eighth of bf16's rounding) with each
 // tile's scales divided by a power of two, 2^k for the keys and 2^v for the values, that takes the
-// largest to [1, 2): no scale overflows, and one far below its tile's largest loses only what is
-// far below that one's products. 2^k multiplies the tile's scores (with the softmax's scale), v is
+// largest to [2^8, 2^9): none overflows, and one keeps f16's precision down to 2^-22 of its tile's
+// largest. 2^k multiplies the tile's scores (with the softmax's scale), v is
 // added to their base-2 exponents, so that the probabilities carry 2^v and the outputs of all
 // tiles stay in one unit; the row's sum takes 2^-v back out. A per-key multiplication of the
 // scores and of the probabilities instead (exact integers in the products) costs every softmax
@@ -573,14 +574,14 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
             }
           }
         };
-        // the exponent of the largest finite scale
+        // the exponent that takes the largest finite scale to [2^8, 2^9): 127 of it stay in f16
         auto exponent = [&](const float (&x)[kKeys]) {
           float top = 0.0f;
 #pragma unroll
           for (int i = 0; i < kKeys; ++i)
             top = fmaxf(top, fabsf(x[i]) <= 3.402823466e38f ? fabsf(x[i]) : 0.0f);
           const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-          return bits == 0 ? 0 : min(max(int(bits >> 23) - 127, -120), 120);
+          return bits == 0 ? 0 : min(max(int(bits >> 23) - 127, -110), 120) - 8;
         };
         auto power = [](int e) { return __uint_as_float(uint32_t(127 + e) << 23); };
         int at = pc.begin, end = pc.end;

@@ -485,6 +485,35 @@ def test_scores_of_any_size():
     fa.device_status()
 
 
+@pytest.mark.parametrize("rows", [2, 60])
+@pytest.mark.parametrize("dims", [(14, 2, 64), (32, 8, 128), (8, 2, 256)], ids=str)
+def test_huge_heads_leave_the_others_their_precision(dims, rows):
+    """One position's keys and values a million times its neighbours' over 8-bit pages: the rows
+    before it are as precise as ever, and so are the rows that give it no weight."""
+    torch = torch_()
+    shape = fa.Shape(1, *dims)
+    spans = Spans([(rows, 90)], 16)
+    cache = make_cache(shape, spans, fa.Q8)
+    page, slot = spans.places(0, 91, 92)
+    cache.value_scales[0, page, :, slot] *= 1e6
+    run_attend(shape, spans, fa.Q8, fa.Mask.causal(), cache=cache)
+    cache.key_scales[0, page, :, slot] *= 1e6  # each row gives it all of its weight, or none
+    q = torch.randn((spans.rows, shape.width), device="cuda").bfloat16()
+    out = torch.empty_like(q)
+    cache.attend(0, spans.batch(cache), q, out)
+    want, tol = reference(cache, 0, spans, q.double(), fa.Mask.causal(), 0.0)
+    # (the bound's part for the scores is the huge key's: a row's other scores are not off by it)
+    d, group = dims[2], dims[0] // dims[1]
+    k, _ = held(cache, 0, page, slot)
+    for h in range(dims[0]):
+        at = slice(h * d, (h + 1) * d)
+        huge = (q[:, at].double() @ k[0, h // group]) / math.sqrt(d)
+        clear = (huge < -100) | (torch.arange(rows, device="cuda") == 0)
+        got, ref = out[clear, at].double(), want[clear, at]
+        if len(got):
+            assert ((got - ref).norm() / ref.norm()).item() < 2 * HALF16
+
+
 @pytest.mark.parametrize("sp", BOTH, ids=["tokens", "chunks"])
 @pytest.mark.parametrize("dims", [(14, 2, 64), (32, 8, 128), (8, 2, 256)], ids=str)
 @pytest.mark.parametrize("dtype", [fa.Q8, fa.BF16], ids=["q8", "bf16"])
