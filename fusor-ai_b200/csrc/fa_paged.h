@@ -124,6 +124,7 @@ struct PagedAttendArgs {
   int heads, group;      // query heads; query heads of a KV head
   int kind, window;      // mask: 0 causal, 1 window, 2 full
   int token_cols;        // packed rows up to which a sequence runs on the token kernel
+  int merge_cols;        // token kernel: the most packed rows that a sequence of it can have
   int q_bf16, q_vec, out_bf16, out_vec;
   const void* q;         // row r, head h at q + r * q_stride + h * head_dim
   int64_t q_stride;

@@ -10,13 +10,17 @@ namespace fa {
 namespace {
 
 template <int D, bool Q8, int NT>
-cudaError_t launch_tokens(const PagedAttendArgs& a, int sms, cudaStream_t stream) {
+cudaError_t launch_tokens(PagedAttendArgs a, int sms, cudaStream_t stream) {
   using S = TokShape<D, Q8, NT>;
   auto kernel = paged_tokens_kernel<D, Q8, NT>;
   static std::atomic<bool> configured[64];  // per instantiation, per device
-  cudaError_t e = smem_limit_once(kernel, S::kSmem, configured);
+  cudaError_t e = smem_limit_once(kernel, S::smem(S::kCols, kMaxPagedSequences), configured);
   if (e != cudaSuccess) return e;
-  return launch_pdl(kernel, dim3(unsigned(sms * S::kCtas)), dim3(kTokThreads), S::kSmem, stream, a);
+  a.merge_cols = int(std::min<int64_t>(S::kCols, int64_t(a.spans.max_rows) * a.group));
+  const int smem = S::smem(a.merge_cols, a.spans.sequences);
+  // the CTAs that an SM holds: 228 KB, of which each takes 1 KB besides its own (and its statics)
+  const int fit = std::max(1, std::min(S::kCtas, (228 * 1024) / (smem + 1024 + 128)));
+  return launch_pdl(kernel, dim3(unsigned(sms * fit)), dim3(kTokThreads), size_t(smem), stream, a);
 }
 
 template <int D>

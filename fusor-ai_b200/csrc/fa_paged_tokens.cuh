@@ -1,27 +1,31 @@
 // Attention of a few packed rows over a paged cache: single tokens, and spans whose rows x query
 // heads of a KV head fit in 16 columns (bound by the bytes of the pages: each is read once).
 //
-// The products run transposed on mma.sync m16n8k16, so that the keys fill the 16 rows and a KV
-// head's packed rows (column c = row offset x group + query head) the 8 or 16 columns:
+// The products run transposed on mma.sync, so that the keys fill the 16 rows and a KV head's packed
+// rows (column c = row offset x group + query head) the 8 or 16 columns:
 //   S^T (16 keys x columns) = K Q^T, then O^T (head_dim x columns) += V^T P^T.
 // Each product's A operand comes straight from a page's rows: the order of the elements within
 // the sums is free (Q is laid out to match, O is written back by the same order), so a thread's
-// fragments are 16-byte vectors of its keys' rows, and an 8-bit page's bytes become f16 (keys) or
-// bf16 (values) integers in registers, at one and a half to two instructions an element. tcgen05
-// would want the converted tile written to shared memory and read again; at 16 columns the tensor
-// pipe is idle either way.
-//   keys: integers are exact in f16; the queries are scaled by a power of two to f16's range, the
-//     key's scale multiplies the score;
-//   values: the probability times the value's scale is rounded to bf16 (a f16 would lose weights
-//     below 2^-24 of the largest); integers up to 127 are exact in bf16.
+// fragments are 16-byte vectors of its keys' rows. tcgen05 would want converted tiles written to
+// shared memory and read again; at 16 columns the tensor pipe is idle either way, and what counts
+// is instructions per byte:
+//   8-bit keys go into m16n8k32 as they are; a query row is held in 15 bits as two 8-bit parts
+//     (q = 128 hi + lo, scaled to its largest element), whose products are exact integers, so
+//     that a score is off by at most half a step, 2^-15 of |q|max, of each element;
+//   8-bit values become f16 integers in registers (exact, three instructions a pair: the bytes of
+//     two keys side by side, 1024 + 128 put under them by one logical operation, subtracted), and
+//     the probabilities take the values' scales: w = 2^(score + log2 scale - M) in f16, M the
+//     running maximum of that exponent (the row's sum keeps the scores' own maximum), so that
+//     the weights that matter are in f16's range whatever the scales;
+//   bf16 keys and values as they are (values by transposing loads), probabilities in bf16.
 // Scores, maxima, sums and outputs are f32. The maximum is lazy: moved when a score exceeds it by
 // 2^8.
 //
-// A CTA has 4 warps, each with its own ring of 16-key stages filled by cp.async (16 consecutive
-// keys lie in one page, so a stage is one contiguous block of keys, one of values, and 16 scales
-// of each): no barrier among the warps until a unit ends, and a warp loads ahead across units.
-// Rows of a stage are swizzled by 16-byte chunks so that both products' reads are free of bank
-// conflicts. Work is shared out as fa_paged_work.cuh says.
+// A CTA has 4 warps, each with its own ring of stages of 32 (or 16) keys filled by cp.async (16
+// consecutive keys lie in one page, so a stage holds contiguous blocks of keys, of values, and
+// their scales): no barrier among the warps until a unit ends, and a warp loads ahead across
+// units. Rows of a stage are swizzled by 16-byte chunks so that both products' reads are free of
+// bank conflicts. Work is shared out as fa_paged_work.cuh says.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -33,7 +37,6 @@ namespace fa {
 
 constexpr int kTokWarps = 4;
 constexpr int kTokThreads = kTokWarps * 32;
-constexpr int kTokTile = 16 * kTokWarps;  // keys of a CTA's tile
 
 template <int D, bool Q8, int NT>
 struct TokShape {
@@ -42,17 +45,21 @@ struct TokShape {
   static constexpr int kRowBytes = D * kElem;
   static constexpr int kChunks = kRowBytes / 16;        // 16-byte chunks of a row
   static constexpr int kPer = 16 / kElem;               // elements of a chunk
-  static constexpr int kBlock = 16 * kRowBytes;         // keys (or values) of a stage
-  static constexpr int kStageBytes = 2 * kBlock + (Q8 ? 128 : 0);
-  static constexpr int kStages = kRowBytes >= 512 ? 2 : 3;  // what shared memory holds
-  static constexpr int kSteps = D / 16;                 // k steps of S, and m tiles of O
+  static constexpr int kBlock = 16 * kRowBytes;         // 16 keys (or values)
+  static constexpr int kHalves = kRowBytes <= 128 ? 2 : 1;  // blocks of 16 keys in a stage
+  static constexpr int kTile = 16 * kHalves * kTokWarps;    // keys of a CTA's tile
+  static constexpr int kHalfBytes = 2 * kBlock + (Q8 ? 128 : 0);
+  static constexpr int kStageBytes = kHalves * kHalfBytes;
+  static constexpr int kStages = kRowBytes <= 64 ? 3 : 2;
+  static constexpr int kSteps = D / 16;                 // m tiles of O (and 16-bit k steps of S)
   static constexpr int kRing = kTokWarps * kStages * kStageBytes;
   static constexpr int kMergeRow = D + 4;               // floats: O, then max and sum (16-byte rows)
-  static constexpr int kMerge = kTokWarps * kCols * kMergeRow * 4;
-  static constexpr int kSmem = kRing + kMerge;
-  // resident CTAs per SM: what 227 KB hold (1 KB each is the system's), at most three
-  static constexpr int kFit = (227 * 1024) / (kSmem + 10240);
-  static constexpr int kCtas = kFit > 3 ? 3 : (kFit < 1 ? 1 : kFit);
+  // resident CTAs per SM that the registers allow
+  static constexpr int kCtas = D == 256 ? (NT == 1 ? 2 : 1) : (NT == 1 ? 3 : 2);
+  // dynamic shared memory for batches of `cols` packed rows and `sequences` sequences
+  static int smem(int cols, int sequences) {
+    return kRing + kTokWarps * cols * kMergeRow * 4 + (sequences + 1) * 8;
+  }
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
@@ -95,6 +102,12 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   return y;
 }
 
+__device__ __forceinline__ float log2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Two signed bytes, at bits 0-7 and 16-23 of w, as f16: the byte plus 128 becomes the low bits of
 // 1024 + (byte + 128), less 1152 (all exact). Bits 8-15 and 24-31 are ignored.
 __device__ __forceinline__ uint32_t bytes_to_f16(uint32_t w) {
@@ -103,13 +116,22 @@ __device__ __forceinline__ uint32_t bytes_to_f16(uint32_t w) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// The same as bf16: 128 + (the low 7 bits), less 128 or, for a negative byte, 256 (all exact).
-__device__ __forceinline__ uint32_t bytes_to_bf16(uint32_t w) {
-  const uint32_t x = (w & 0x007F007Fu) | 0x43004300u;
-  const uint32_t y = (w & 0x00800080u) | 0x43004300u;
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x),
-                                   *reinterpret_cast<const __nv_bfloat162*>(&y));
-  return *reinterpret_cast<const uint32_t*>(&r);
+// m16n8k32 of signed bytes.
+__device__ __forceinline__ void mma16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Four 8 x 8 matrices of 16-bit elements, transposed: lane l gives row l % 8 of matrix l / 8.
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
 }
 
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
@@ -139,6 +161,7 @@ struct TokPlan {
 
 // A sequence's part in the token kernel: its span, the keys that its rows see and their tiles
 // (0 if it is empty, out of range or the chunk kernel's).
+template <int kTile>
 __device__ __forceinline__ int token_tiles(const PagedAttendArgs& a, int s, TokWalk* w) {
   PagedSpan sp;
   if (!paged_span(a.spans, a.pool.page_shift, s, &sp)) return -1;
@@ -153,15 +176,16 @@ __device__ __forceinline__ int token_tiles(const PagedAttendArgs& a, int s, TokW
     w->lo = lo;
     w->hi = hi;
   }
-  return (hi + kTokTile - 1) / kTokTile - lo / kTokTile;
+  return (hi + kTile - 1) / kTile - lo / kTile;
 }
 
 // Moves the walk to the unit that holds global tile w->t (w->s at or before it); false at the
 // share's end.
+template <int kTile>
 __device__ __forceinline__ bool token_seek(const PagedAttendArgs& a, const TokPlan& plan, TokWalk* w) {
   if (w->t >= w->t_end) return false;
   while (plan.before[w->s + 1] * plan.kvh <= w->t) ++w->s;
-  w->tiles = token_tiles(a, w->s, w);
+  w->tiles = token_tiles<kTile>(a, w->s, w);
   const int64_t rest = w->t - plan.before[w->s] * plan.kvh;
   w->h = int(rest / w->tiles);
   w->tile = int(rest - int64_t(w->h) * w->tiles);
@@ -174,11 +198,13 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
     paged_tokens_kernel(const __grid_constant__ PagedAttendArgs a) {
   using S = TokShape<D, Q8, NT>;
   constexpr int kRB = S::kRowBytes, kC = S::kChunks, kPer = S::kPer;
+  constexpr int KH = S::kHalves, kTile = S::kTile;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int64_t before[kMaxPagedSequences + 1];
   __shared__ int64_t scratch[kTokWarps];
   __shared__ int arrived;
+  const int mcols = a.merge_cols;  // packed rows that any sequence has
   float* merge = reinterpret_cast<float*>(smem + S::kRing);
+  int64_t* before = reinterpret_cast<int64_t*>(merge + kTokWarps * mcols * S::kMergeRow);
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
@@ -194,7 +220,7 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
     const int s0 = min(nseq, int(threadIdx.x) * each), s1 = min(nseq, s0 + each);
     int64_t sum = 0;
     for (int s = s0; s < s1; ++s) {
-      const int n = token_tiles(a, s, nullptr);
+      const int n = token_tiles<kTile>(a, s, nullptr);
       if (n < 0) atomicOr(a.err, kErrPagedSpan);
       sum += max(n, 0);
       before[s] = sum;  // inclusive within the thread's sequences, for now
@@ -230,43 +256,51 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
     lw.s = cw.s = s0;
   }
 
-  // ---- loads: one 16-key stage at a time ------------------------------------------------------
+  // ---- loads: one stage at a time --------------------------------------------------------------
   const int shift = a.pool.page_shift;
-  bool more = token_seek(a, plan, &lw);
-  int next_page = -1;  // the page of the next stage's keys (-1: none of them is seen)
-  auto fetch_page = [&]() {
-    next_page = -1;
-    if (!more) return;
-    const int pos = (lw.lo / kTokTile + lw.tile) * kTokTile + warp * 16;
-    if (pos < lw.hi && pos + 16 > lw.lo)
-      next_page = __ldg(a.spans.tables + int64_t(lw.s) * a.spans.table_stride + (pos >> shift));
+  bool more = token_seek<kTile>(a, plan, &lw);
+  int next_page[KH];  // the pages of the next stage's 16s of keys (-1: none of them is seen)
+  auto stage_pos = [&](const TokWalk& w) { return (w.lo / kTile + w.tile) * kTile + warp * (16 * KH); };
+  auto fetch_pages = [&]() {
+#pragma unroll
+    for (int h = 0; h < KH; ++h) {
+      next_page[h] = -1;
+      if (!more) continue;
+      const int pos = stage_pos(lw) + 16 * h;
+      if (pos < lw.hi && pos + 16 > lw.lo)
+        next_page[h] = __ldg(a.spans.tables + int64_t(lw.s) * a.spans.table_stride + (pos >> shift));
+    }
   };
-  fetch_page();
-  uint32_t ring_live = 0;  // a bit per stage: its keys are there (a page in range, some key seen)
+  fetch_pages();
+  uint32_t ring_live = 0;  // a bit per 16s: its keys are there (a page in range, some key seen)
+  // chunk q = lane + 32 i of a block: its row and its place in the stage, by i's parity where the
+  // swizzle's row bits change
+  const int q_key = lane / kC, q_c = lane % kC;
   auto issue = [&](int stage) {
     if (!more) return;
-    bool live = next_page >= 0;
-    const int pos = (lw.lo / kTokTile + lw.tile) * kTokTile + warp * 16;
-    if (!paged_page_ok(next_page, a.pool.pages)) {
-      if (pos < lw.hi && pos + 16 > lw.lo && lane == 0) atomicOr(a.err, kErrPagedPage);
-      live = false;
-    }
-    ring_live = (ring_live & ~(1u << stage)) | (uint32_t(live) << stage);
-    if (live) {
-      const int64_t row = ((int64_t(next_page) * kvh + lw.h) << shift) + (pos & ((1 << shift) - 1));
-      const unsigned char* ks = a.pool.keys + row * kRB;
-      const unsigned char* vs = a.pool.values + row * kRB;
-      const uint32_t kd = smem_u32(ring + stage * S::kStageBytes), vd = kd + S::kBlock;
+#pragma unroll
+    for (int h = 0; h < KH; ++h) {
+      const int pos = stage_pos(lw) + 16 * h;
+      const bool some = pos < lw.hi && pos + 16 > lw.lo;
+      const bool live = some && paged_page_ok(next_page[h], a.pool.pages);
+      if (some && !live && lane == 0) atomicOr(a.err, kErrPagedPage);
+      const uint32_t bit = 1u << (stage * KH + h);
+      ring_live = live ? ring_live | bit : ring_live & ~bit;
+      if (!live) continue;
+      const int64_t row = ((int64_t(next_page[h]) * kvh + lw.h) << shift) + (pos & ((1 << shift) - 1));
+      const unsigned char* ks = a.pool.keys + row * kRB + lane * 16;
+      const unsigned char* vs = a.pool.values + row * kRB + lane * 16;
+      const uint32_t kd = smem_u32(ring + stage * S::kStageBytes + h * S::kHalfBytes), vd = kd + S::kBlock;
+      const bool all = pos >= lw.lo && pos + 16 <= lw.hi;
 #pragma unroll
       for (int i = 0; i < kC / 2; ++i) {
-        const int q = lane + 32 * i;  // the block's 16-byte chunk
-        const int key = q / kC, c = q % kC;
+        const int key = q_key + i * (32 / kC < 1 ? 1 : 32 / kC);  // (kC <= 32)
+        const int ck = kC >= 8 ? q_c ^ ((key & 1) << 2) : q_c;
+        const int cv = kC < 8 ? q_c : Q8 ? q_c ^ (((key >> 1) & 3) << 1) : q_c ^ (key & 7);
         // rows outside the keys seen (a page's stale end, or before the window) come as zeros
-        const uint32_t bytes = pos + key >= lw.lo && pos + key < lw.hi ? 16u : 0u;
-        const int ck = kC >= 8 ? c ^ ((key & 1) << 2) : c;
-        const int cv = kC >= 8 ? c ^ (((key >> 1) & 3) << 1) : c;
-        cp_async16(kd + key * kRB + ck * 16, ks + q * 16, bytes);
-        cp_async16(vd + key * kRB + cv * 16, vs + q * 16, bytes);
+        const uint32_t bytes = all || (pos + key >= lw.lo && pos + key < lw.hi) ? 16u : 0u;
+        cp_async16(kd + key * kRB + ck * 16, ks + i * 512, bytes);
+        cp_async16(vd + key * kRB + cv * 16, vs + i * 512, bytes);
       }
       if constexpr (Q8) {
         const int key = lane & 15;
@@ -276,8 +310,8 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
       }
     }
     ++lw.t;
-    if (++lw.tile == lw.tile_end) more = token_seek(a, plan, &lw);
-    fetch_page();
+    if (++lw.tile == lw.tile_end) more = token_seek<kTile>(a, plan, &lw);
+    fetch_pages();
   };
 #pragma unroll
   for (int i = 0; i < S::kStages - 1; ++i) {
@@ -287,9 +321,11 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
 
   // ---- the products ---------------------------------------------------------------------------
   int stage = 0;
-  while (token_seek(a, plan, &cw)) {
-    // this lane's query column g (+ 8): its fragments, scaled to f16's range for 8-bit pages
-    uint32_t qf[NT][S::kSteps][2];
+  while (token_seek<kTile>(a, plan, &cw)) {
+    // This lane's query column g (+ 8): its fragments. 8-bit pages: bytes of hi and lo for the
+    // lane's chunks, two words for each product of 32 elements; bf16: pairs.
+    constexpr int kFrags = Q8 ? D / 32 : S::kSteps;
+    uint32_t qf[NT][kFrags][2], ql[NT][Q8 ? kFrags : 1][2];
     float qscale[NT][2];  // of this lane's score columns 2 t4, 2 t4 + 1
     int col_lo[NT][2], col_hi[NT][2];
     int lo_max = 0, hi_min = 0x7fffffff;  // keys that every column sees
@@ -298,12 +334,11 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
       const int col = nt * 8 + g;
       const int r = col / a.group;
       const bool valid = r < cw.n;
-      float top = 0.0f;
       float x[S::kSteps][4];
       const int64_t at = int64_t(cw.row0 + r) * a.q_stride +
                          int64_t(cw.h * a.group + col % a.group) * D;
 #pragma unroll
-      for (int i = 0; i < kC / 4 + (kC < 4); ++i) {
+      for (int i = 0; i < kC / 4; ++i) {
         const int64_t e0 = at + (t4 + 4 * i) * kPer;
 #pragma unroll
         for (int j = 0; j < kPer / 4; ++j) {
@@ -331,25 +366,41 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
           }
         }
       }
-      float up = 1.0f, down = 1.0f;
+      float down = 1.0f;
       if constexpr (Q8) {
+        float top = 0.0f, total = 0.0f;  // (total: NaN if an element is)
 #pragma unroll
         for (int k = 0; k < S::kSteps; ++k)
-          top = fmaxf(top, fmaxf(fmaxf(fabsf(x[k][0]), fabsf(x[k][1])), fmaxf(fabsf(x[k][2]), fabsf(x[k][3]))));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the power of two that takes the largest element to [1, 2): exponents within 2^+-126
-        const int e = min(max(int(__float_as_uint(top) >> 23), 1), 253);
-        up = __uint_as_float(uint32_t(254 - e) << 23);
-        down = __uint_as_float(uint32_t(e) << 23);
-      }
 #pragma unroll
-      for (int k = 0; k < S::kSteps; ++k) {
-        if constexpr (Q8) {
-          // 8-bit keys come as bytes 0, 2 then 1, 3 of a word
-          qf[nt][k][0] = pack_f16(x[k][0] * up, x[k][2] * up);
-          qf[nt][k][1] = pack_f16(x[k][1] * up, x[k][3] * up);
-        } else {
+          for (int e = 0; e < 4; ++e) {
+            top = fmaxf(top, fabsf(x[k][e]));
+            total += x[k][e] * 0.0f;
+          }
+#pragma unroll
+        for (int off = 1; off <= 2; off <<= 1) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          total += __shfl_xor_sync(0xffffffffu, total, off);
+        }
+        // steps of top / 16256 (hi up to 127); elements below 1e-33 throughout are kept as zeros
+        top = fmaxf(top, 1e-33f);
+        const float up = 16256.0f / top;
+        down = top / 16256.0f + total;  // a row with an infinity or a NaN scores NaN
+#pragma unroll
+        for (int k = 0; k < S::kSteps; ++k) {
+          uint32_t hw = 0, lw_ = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int v = __float2int_rn(fminf(fmaxf(x[k][e] * up, -16256.0f), 16256.0f));
+            const int hi = (v + 64) >> 7, lo = v - (hi << 7);
+            hw |= uint32_t(hi & 0xff) << (8 * e);
+            lw_ |= uint32_t(lo & 0xff) << (8 * e);
+          }
+          qf[nt][k / 2][k & 1] = hw;
+          ql[nt][k / 2][k & 1] = lw_;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < S::kSteps; ++k) {
           qf[nt][k][0] = pack_bf16x2(x[k][0], x[k][1]);
           qf[nt][k][1] = pack_bf16x2(x[k][2], x[k][3]);
         }
@@ -372,18 +423,18 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
 
     float o[S::kSteps][NT][4];
     float m[NT][2], l[NT][2];
+    float mo[NT][2];  // 8-bit pages: the maximum of the weights' exponents (O is in its unit)
+    bool poisoned[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = -INFINITY;
+      m[nt][0] = m[nt][1] = mo[nt][0] = mo[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = 0.0f;
+      poisoned[nt][0] = poisoned[nt][1] = false;
 #pragma unroll
       for (int k = 0; k < S::kSteps; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[k][nt][e] = 0.0f;
     }
-    bool poisoned[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) poisoned[nt][0] = poisoned[nt][1] = false;
 
     for (; cw.tile < cw.tile_end; ++cw.tile, ++cw.t) {
       cp_async_wait<S::kStages - 2>();
@@ -391,86 +442,130 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
       const int fill = stage == 0 ? S::kStages - 1 : stage - 1;  // the stage read last time
       issue(fill);
       cp_async_commit();
-      const unsigned char* kb = ring + stage * S::kStageBytes;
-      const unsigned char* vb = kb + S::kBlock;
-      const float* scales = reinterpret_cast<const float*>(vb + S::kBlock);
-      const bool live = (ring_live >> stage) & 1u;
+      const unsigned char* base = ring + stage * S::kStageBytes;
+      const uint32_t live = (ring_live >> (stage * KH)) & ((1u << KH) - 1);
       stage = stage + 1 == S::kStages ? 0 : stage + 1;
-      if (!live) continue;  // uniform over the warp
-      const int pos = (cw.lo / kTokTile + cw.tile) * kTokTile + warp * 16;
+      if (live == 0) continue;  // uniform over the warp
+      const int pos0 = stage_pos(cw);
 
-      // S^T: keys g and g + 8 of the stage
-      float sc[NT][2][4];
+      // S^T: keys g and g + 8 of each 16
+      float s[KH][NT][4];  // e: key g + 8 (e / 2), column 2 t4 + e % 2
+      bool whole[KH];
+      bool grow = false;
+#pragma unroll
+      for (int h = 0; h < KH; ++h) {
+        const unsigned char* kb = base + h * S::kHalfBytes;
+        const int pos = pos0 + 16 * h;
+        whole[h] = pos >= lo_max && pos + 16 <= hi_min && ((live >> h) & 1u);
+        float f[NT][4];
+        if constexpr (Q8) {
+          int ch[NT][4], cl[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ch[nt][e] = cl[nt][e] = 0;
+#pragma unroll
+          for (int i = 0; i < kC / 4; ++i) {
+            const int c = t4 + 4 * i, cs = kC >= 8 ? c ^ ((g & 1) << 2) : c;
+            const uint4 ra = *reinterpret_cast<const uint4*>(kb + g * kRB + cs * 16);
+            const uint4 rb = *reinterpret_cast<const uint4*>(kb + (g + 8) * kRB + cs * 16);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16832(ch[nt], ra.x, rb.x, ra.y, rb.y, qf[nt][2 * i][0], qf[nt][2 * i][1]);
+              mma16832(cl[nt], ra.x, rb.x, ra.y, rb.y, ql[nt][2 * i][0], ql[nt][2 * i][1]);
+              mma16832(ch[nt], ra.z, rb.z, ra.w, rb.w, qf[nt][2 * i + 1][0], qf[nt][2 * i + 1][1]);
+              mma16832(cl[nt], ra.z, rb.z, ra.w, rb.w, ql[nt][2 * i + 1][0], ql[nt][2 * i + 1][1]);
+            }
+          }
+          const float* sk = reinterpret_cast<const float*>(kb + 2 * S::kBlock);
+          const float ks[2] = {sk[g], sk[g + 8]};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              f[nt][e] = float(ch[nt][e] * 128 + cl[nt][e]) * (qscale[nt][e & 1] * ks[e >> 1]);
+        } else {
+          float sc[NT][2][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[nt][0][e] = sc[nt][1][e] = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kC / 4; ++i) {
+            const int c = t4 + 4 * i, cs = kC >= 8 ? c ^ ((g & 1) << 2) : c;
+            const uint4 ra = *reinterpret_cast<const uint4*>(kb + g * kRB + cs * 16);
+            const uint4 rb = *reinterpret_cast<const uint4*>(kb + (g + 8) * kRB + cs * 16);
+            const uint32_t fa_[4] = {ra.x, rb.x, ra.y, rb.y}, fb_[4] = {ra.z, rb.z, ra.w, rb.w};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816<false>(sc[nt][0], fa_, qf[nt][2 * i][0], qf[nt][2 * i][1]);
+              mma16816<false>(sc[nt][1], fb_, qf[nt][2 * i + 1][0], qf[nt][2 * i + 1][1]);
+            }
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[nt][e] = (sc[nt][0][e] + sc[nt][1][e]) * qscale[nt][e & 1];
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            bool see = whole[h];
+            if (!see) {
+              const int p = pos + g + 8 * (e >> 1);
+              see = ((live >> h) & 1u) && p >= col_lo[nt][e & 1] && p < col_hi[nt][e & 1];
+            }
+            s[h][nt][e] = see ? f[nt][e] : -INFINITY;
+          }
+      }
+      // the weights' exponents: over 8-bit pages with the values' scales
+      float y[Q8 ? KH : 1][Q8 ? NT : 1][4];
+      if constexpr (Q8) {
+#pragma unroll
+        for (int h = 0; h < KH; ++h) {
+          const float* sv = reinterpret_cast<const float*>(base + h * S::kHalfBytes + 2 * S::kBlock) + 16;
+          const float lv[2] = {log2_approx(sv[g]), log2_approx(sv[g + 8])};  // (stale if not live)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              y[h][nt][e] = s[h][nt][e] > -INFINITY ? s[h][nt][e] + lv[e >> 1] : -INFINITY;
+        }
+      }
+      auto top_of = [&](const auto& x, int nt, int j) {
+        float top = fmaxf(x[0][nt][j], x[0][nt][2 + j]);
+        if constexpr (KH == 2) top = fmaxf(top, fmaxf(x[1][nt][j], x[1][nt][2 + j]));
+        return top;
+      };
+      auto moves = [](float top, float m) { return top > m + 8.0f || (m == -INFINITY && top > -INFINITY); };
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[nt][0][e] = sc[nt][1][e] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kC / 4; ++i) {
-        const int c = t4 + 4 * i;
-        const int cs = kC >= 8 ? c ^ ((g & 1) << 2) : c;
-        const uint4 ra = *reinterpret_cast<const uint4*>(kb + g * kRB + cs * 16);
-        const uint4 rb = *reinterpret_cast<const uint4*>(kb + (g + 8) * kRB + cs * 16);
-        const uint32_t wa[4] = {ra.x, ra.y, ra.z, ra.w}, wb[4] = {rb.x, rb.y, rb.z, rb.w};
-        if constexpr (Q8) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t fr[4] = {bytes_to_f16(wa[j]), bytes_to_f16(wb[j]),
-                                    bytes_to_f16(wa[j] >> 8), bytes_to_f16(wb[j] >> 8)};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma16816<true>(sc[nt][j & 1], fr, qf[nt][4 * i + j][0], qf[nt][4 * i + j][1]);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint32_t fr[4] = {wa[2 * j], wb[2 * j], wa[2 * j + 1], wb[2 * j + 1]};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma16816<false>(sc[nt][j & 1], fr, qf[nt][2 * i + j][0], qf[nt][2 * i + j][1]);
-          }
-        }
-      }
-      float ks[2] = {1.0f, 1.0f}, vs[2] = {1.0f, 1.0f};
-      if constexpr (Q8) {
-        ks[0] = scales[g];
-        ks[1] = scales[g + 8];
-        vs[0] = scales[16 + g];
-        vs[1] = scales[16 + g + 8];
-      }
-      const bool whole = pos >= lo_max && pos + 16 <= hi_min;
-      float s[NT][4];  // e: key g + 8 (e / 2), column 2 t4 + e % 2
-      bool grow = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = (sc[nt][0][e] + sc[nt][1][e]) * (qscale[nt][e & 1] * ks[e >> 1]);
-          const int p = pos + g + 8 * (e >> 1);
-          s[nt][e] = whole || (p >= col_lo[nt][e & 1] && p < col_hi[nt][e & 1]) ? x : -INFINITY;
-        }
-#pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const float top = fmaxf(s[nt][j], s[nt][2 + j]);
-          grow = grow || top > m[nt][j] + 8.0f || (m[nt][j] == -INFINITY && top > -INFINITY);
+          grow = grow || moves(top_of(s, nt, j), m[nt][j]);
+          if constexpr (Q8) grow = grow || moves(top_of(y, nt, j), mo[nt][j]);
         }
-      }
       if (__any_sync(0xffffffffu, grow)) {
+        // a maximum moves to its column's largest over the warp; what it was gets the ratio
+        auto move = [&](float top, float& m) {
+#pragma unroll
+          for (int off = 4; off <= 16; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          float alpha = 1.0f;
+          if (top > m) {
+            if (m > -INFINITY) alpha = exp2_approx(m - top);
+            m = top;
+          }
+          return alpha;
+        };
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float alpha[2];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float top = fmaxf(s[nt][j], s[nt][2 + j]);
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            alpha[j] = 1.0f;
-            if (top > m[nt][j]) {
-              if (m[nt][j] > -INFINITY) alpha[j] = exp2_approx(m[nt][j] - top);
-              m[nt][j] = top;
-            }
+            alpha[j] = move(top_of(s, nt, j), m[nt][j]);
             l[nt][j] *= alpha[j];
+            if constexpr (Q8) alpha[j] = move(top_of(y, nt, j), mo[nt][j]);
           }
 #pragma unroll
           for (int k = 0; k < S::kSteps; ++k)
@@ -478,97 +573,105 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
             for (int e = 0; e < 4; ++e) o[k][nt][e] *= alpha[e & 1];
         }
       }
-      uint32_t pf[NT][2];
+      uint32_t pf[KH][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float w[4];
+        float off[2], off_o[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float ms = m[nt][e & 1] == -INFINITY ? 0.0f : m[nt][e & 1];
-          const float p = exp2_approx(s[nt][e] - ms);
-          l[nt][e & 1] += p;
-          // a key that the column does not see keeps its scale out (it may be infinite or NaN)
-          w[e] = Q8 ? (s[nt][e] > -INFINITY ? p * vs[e >> 1] : 0.0f) : p;
+        for (int j = 0; j < 2; ++j) {
+          off[j] = m[nt][j] == -INFINITY ? 0.0f : m[nt][j];
+          off_o[j] = Q8 ? (mo[nt][j] == -INFINITY ? 0.0f : mo[nt][j]) - 6.0f : 0.0f;
         }
-        pf[nt][0] = movmatrix(pack_bf16x2(w[0], w[1]));
-        pf[nt][1] = movmatrix(pack_bf16x2(w[2], w[3]));
+#pragma unroll
+        for (int h = 0; h < KH; ++h) {
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p = exp2_approx(s[h][nt][e] - off[e & 1]);
+            l[nt][e & 1] += p;
+            if constexpr (Q8) w[e] = exp2_approx(y[h][nt][e] - off_o[e & 1]);
+            else w[e] = p;
+          }
+          pf[h][nt][0] = movmatrix(Q8 ? pack_f16(w[0], w[1]) : pack_bf16x2(w[0], w[1]));
+          pf[h][nt][1] = movmatrix(Q8 ? pack_f16(w[2], w[3]) : pack_bf16x2(w[2], w[3]));
+        }
       }
 
-      // O^T: values of keys 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9
-      constexpr int kPiece = kC >= 8 ? 16 : 8;             // bytes a lane takes of a row at a time
-      constexpr int kPieces = kRB / (8 * kPiece);
-      constexpr int kWords = kPiece / 4;
-      uint32_t bad = 0;  // bf16: which of the lane's four keys has a value that is not finite
+      // O^T
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        uint32_t wv[4][kWords];
+      for (int h = 0; h < KH; ++h) {
+        if (!((live >> h) & 1u)) continue;  // (stale bytes: not to be multiplied even by zero)
+        const unsigned char* vb = base + h * S::kHalfBytes + S::kBlock;
+        if constexpr (Q8) {
+          // values of keys 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9
+          constexpr int kPiece = kC >= 8 ? 16 : 8;  // bytes a lane takes of a row at a time
+          constexpr int kPieces = kRB / (8 * kPiece), kWords = kPiece / 4;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int key = 2 * t4 + (q & 1) + 8 * (q >> 1);
-          if constexpr (kPiece == 16) {
-            const int c = (g + 8 * i) ^ (((key >> 1) & 3) << 1);
-            const uint4 r = *reinterpret_cast<const uint4*>(vb + key * kRB + c * 16);
-            wv[q][0] = r.x; wv[q][1] = r.y; wv[q][2] = r.z; wv[q][3] = r.w;
-          } else {
-            const uint2 r = *reinterpret_cast<const uint2*>(vb + key * kRB + g * 8);
-            wv[q][0] = r.x; wv[q][1] = r.y;
-          }
-        }
-        if constexpr (!Q8) {
-          if (!whole) {
-            // a value that is not finite would reach columns that do not see its key (0 x inf):
-            // it is taken out here and every column that sees it marked below
+          for (int i = 0; i < kPieces; ++i) {
+            uint32_t wv[4][kWords];
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+            for (int q = 0; q < 4; ++q) {
+              const int key = 2 * t4 + (q & 1) + 8 * (q >> 1);
+              if constexpr (kPiece == 16) {
+                const int c = (g + 8 * i) ^ (((key >> 1) & 3) << 1);
+                const uint4 r = *reinterpret_cast<const uint4*>(vb + key * kRB + c * 16);
+                wv[q][0] = r.x; wv[q][1] = r.y; wv[q][2] = r.z; wv[q][3] = r.w;
+              } else {
+                const uint2 r = *reinterpret_cast<const uint2*>(vb + key * kRB + g * 8);
+                wv[q][0] = r.x; wv[q][1] = r.y;
+              }
+            }
 #pragma unroll
-              for (int x = 0; x < kWords; ++x) {
-                if ((wv[q][x] & 0x7F80u) == 0x7F80u) { wv[q][x] &= 0xFFFF0000u; bad |= 1u << q; }
-                if ((wv[q][x] & 0x7F800000u) == 0x7F800000u) { wv[q][x] &= 0xFFFFu; bad |= 1u << q; }
+            for (int x = 0; x < kWords; ++x)
+#pragma unroll
+              for (int b = 0; b < 2; ++b) {
+                // bytes 2 b and 2 b + 1 of word x: two elements, an m tile
+                const uint32_t sel0 = b == 0 ? 0x0400u : 0x0602u, sel1 = b == 0 ? 0x0501u : 0x0703u;
+                const uint32_t fr[4] = {bytes_to_f16(__byte_perm(wv[0][x], wv[1][x], sel0)),
+                                        bytes_to_f16(__byte_perm(wv[0][x], wv[1][x], sel1)),
+                                        bytes_to_f16(__byte_perm(wv[2][x], wv[3][x], sel0)),
+                                        bytes_to_f16(__byte_perm(wv[2][x], wv[3][x], sel1))};
+                const int mt = i * (kPiece / 2) + 2 * x + b;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma16816<true>(o[mt][nt], fr, pf[h][nt][0], pf[h][nt][1]);
               }
           }
-        }
+        } else {
+          // lane: row lane % 8 of matrix lane / 8 (elements 0-7 and 8-15 of keys 0-7, then of 8-15)
+          const int key = (lane & 7) + 8 * (lane >> 4), half = (lane >> 3) & 1;
+          const uint32_t row = smem_u32(vb) + key * kRB;
+          uint32_t bad = 0;  // which of the lane's four keys has a value that is not finite
 #pragma unroll
-        for (int x = 0; x < kWords; ++x) {
-          if constexpr (Q8) {
-            // bytes 0..3 of word x: elements 4x .. 4x + 3 of the piece, two m tiles
+          for (int mt = 0; mt < S::kSteps; ++mt) {
+            uint32_t fr[4];
+            ldmatrix4_trans(fr, row + (((2 * mt + half) ^ (key & 7)) * 16));
+            if (!whole[h]) {
+              // a value that is not finite would reach columns that do not see its key (0 x inf):
+              // it is taken out here and every column that sees it marked below
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-              const uint32_t sel0 = b == 0 ? 0x0400u : 0x0602u;  // bytes 2b of both keys
-              const uint32_t sel1 = b == 0 ? 0x0501u : 0x0703u;  // bytes 2b + 1
-              const uint32_t fr[4] = {bytes_to_bf16(__byte_perm(wv[0][x], wv[1][x], sel0)),
-                                      bytes_to_bf16(__byte_perm(wv[0][x], wv[1][x], sel1)),
-                                      bytes_to_bf16(__byte_perm(wv[2][x], wv[3][x], sel0)),
-                                      bytes_to_bf16(__byte_perm(wv[2][x], wv[3][x], sel1))};
-              const int mt = i * (kPiece / 2) + 2 * x + b;
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma16816<false>(o[mt][nt], fr, pf[nt][0], pf[nt][1]);
+              for (int x = 0; x < 4; ++x) {
+                if ((fr[x] & 0x7F80u) == 0x7F80u) { fr[x] &= 0xFFFF0000u; bad |= 1u << (x & 2); }
+                if ((fr[x] & 0x7F800000u) == 0x7F800000u) { fr[x] &= 0xFFFFu; bad |= 2u << (x & 2); }
+              }
             }
-          } else {
-            const uint32_t fr[4] = {__byte_perm(wv[0][x], wv[1][x], 0x5410),
-                                    __byte_perm(wv[0][x], wv[1][x], 0x7632),
-                                    __byte_perm(wv[2][x], wv[3][x], 0x5410),
-                                    __byte_perm(wv[2][x], wv[3][x], 0x7632)};
-            const int mt = i * (kPiece / 4) + x;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16816<false>(o[mt][nt], fr, pf[nt][0], pf[nt][1]);
+            for (int nt = 0; nt < NT; ++nt) mma16816<false>(o[mt][nt], fr, pf[h][nt][0], pf[h][nt][1]);
           }
-        }
-      }
-      if constexpr (!Q8) {
-        if (!whole) {
-          // the keys with such a value, over the warp: bit k for key k of the stage
-          uint32_t keys = 0;
+          if (!whole[h]) {
+            // the keys with such a value, over the warp: bit k for key k of the 16
+            uint32_t keys = 0;
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if ((bad >> q) & 1u) keys |= 1u << (2 * t4 + (q & 1) + 8 * (q >> 1));
-          keys = __reduce_or_sync(0xffffffffu, keys);
-          for (uint32_t rest = keys; rest != 0; rest &= rest - 1) {
-            const int p = pos + __ffs(rest) - 1;
+            for (int q = 0; q < 4; ++q)
+              if ((bad >> q) & 1u) keys |= 1u << (2 * t4 + (q & 1) + 8 * (q >> 1));
+            keys = __reduce_or_sync(0xffffffffu, keys);
+            for (uint32_t rest = keys; rest != 0; rest &= rest - 1) {
+              const int p = pos0 + 16 * h + __ffs(rest) - 1;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+              for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int j = 0; j < 2; ++j)
-                poisoned[nt][j] = poisoned[nt][j] || (p >= col_lo[nt][j] && p < col_hi[nt][j]);
+                for (int j = 0; j < 2; ++j)
+                  poisoned[nt][j] = poisoned[nt][j] || (p >= col_lo[nt][j] && p < col_hi[nt][j]);
+            }
           }
         }
       }
@@ -583,15 +686,31 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
         l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 8);
         l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 16);
         if (poisoned[nt][j]) l[nt][j] = __int_as_float(0x7fffffff);
-        float* row = merge + (warp * S::kCols + nt * 8 + 2 * t4 + j) * S::kMergeRow;
+        const int col = nt * 8 + 2 * t4 + j;
+        if (col >= mcols) continue;
+        if constexpr (Q8) {
+          // O to the sum's unit
+          const float f = mo[nt][j] == -INFINITY || m[nt][j] == -INFINITY
+                              ? 0.0f : exp2_approx(mo[nt][j] - m[nt][j] - 6.0f);
+#pragma unroll
+          for (int k = 0; k < S::kSteps; ++k) {
+            o[k][nt][j] *= f;
+            o[k][nt][2 + j] *= f;
+          }
+        }
+        float* row = merge + (warp * mcols + col) * S::kMergeRow;
         if (g == 0) { row[D] = m[nt][j]; row[D + 1] = l[nt][j]; }
-        constexpr int kPiece = kC >= 8 ? 16 : 8;
-        constexpr int kElems = kPiece / S::kElem;  // of a lane's piece of a row
 #pragma unroll
         for (int k = 0; k < S::kSteps; ++k) {
-          // m tile k: elements 2 (k % (kElems / 2)) + {0, 1} of the lane's piece k / (kElems / 2)
-          const int d = (g + 8 * (k / (kElems / 2))) * kElems + 2 * (k % (kElems / 2));
-          *reinterpret_cast<float2*>(row + d) = make_float2(o[k][nt][j], o[k][nt][2 + j]);
+          if constexpr (Q8) {
+            // m tile k: elements 2 (k % (kElems / 2)) + {0, 1} of the lane's piece k / (kElems / 2)
+            constexpr int kElems = kC >= 8 ? 16 : 8;  // of a lane's piece of a row
+            const int d = (g + 8 * (k / (kElems / 2))) * kElems + 2 * (k % (kElems / 2));
+            *reinterpret_cast<float2*>(row + d) = make_float2(o[k][nt][j], o[k][nt][2 + j]);
+          } else {
+            row[16 * k + g] = o[k][nt][j];
+            row[16 * k + g + 8] = o[k][nt][2 + j];
+          }
         }
       }
     __syncthreads();
@@ -625,11 +744,11 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
       float mm = -INFINITY, ll = 0.0f;
 #pragma unroll
       for (int w = 0; w < kTokWarps; ++w)
-        mm = fmaxf(mm, merge[(w * S::kCols + col) * S::kMergeRow + D]);
+        mm = fmaxf(mm, merge[(w * mcols + col) * S::kMergeRow + D]);
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int w = 0; w < kTokWarps; ++w) {
-        const float* row = merge + (w * S::kCols + col) * S::kMergeRow;
+        const float* row = merge + (w * mcols + col) * S::kMergeRow;
         const float f = row[D] == -INFINITY ? 0.0f : exp2_approx(row[D] - mm);
         // a warp that saw no key has sum 0 (or NaN, which stays)
         ll += row[D] == -INFINITY ? row[D + 1] : f * row[D + 1];
