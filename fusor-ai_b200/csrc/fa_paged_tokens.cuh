@@ -291,23 +291,27 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
       const unsigned char* ks = a.pool.keys + row * kRB + lane * 16;
       const unsigned char* vs = a.pool.values + row * kRB + lane * 16;
       const uint32_t kd = smem_u32(ring + stage * S::kStageBytes + h * S::kHalfBytes), vd = kd + S::kBlock;
-      const bool all = pos >= lw.lo && pos + 16 <= lw.hi;
+      const int64_t at = row + (lane & 15);
+      const float* sc = lane < 16 ? a.pool.key_scales : a.pool.value_scales;
+      auto copy = [&](bool all) {
 #pragma unroll
-      for (int i = 0; i < kC / 2; ++i) {
-        const int key = q_key + i * (32 / kC < 1 ? 1 : 32 / kC);  // (kC <= 32)
-        const int ck = kC >= 8 ? q_c ^ ((key & 1) << 2) : q_c;
-        const int cv = kC < 8 ? q_c : Q8 ? q_c ^ (((key >> 1) & 3) << 1) : q_c ^ (key & 7);
-        // rows outside the keys seen (a page's stale end, or before the window) come as zeros
-        const uint32_t bytes = all || (pos + key >= lw.lo && pos + key < lw.hi) ? 16u : 0u;
-        cp_async16(kd + key * kRB + ck * 16, ks + i * 512, bytes);
-        cp_async16(vd + key * kRB + cv * 16, vs + i * 512, bytes);
-      }
-      if constexpr (Q8) {
-        const int key = lane & 15;
-        const uint32_t bytes = pos + key >= lw.lo && pos + key < lw.hi ? 4u : 0u;
-        const float* sc = lane < 16 ? a.pool.key_scales : a.pool.value_scales;
-        cp_async4(vd + S::kBlock + lane * 4, sc + row + key, bytes);
-      }
+        for (int i = 0; i < kC / 2; ++i) {
+          const int key = q_key + i * (32 / kC);
+          const int ck = kC >= 8 ? q_c ^ ((key & 1) << 2) : q_c;
+          const int cv = kC < 8 ? q_c : Q8 ? q_c ^ (((key >> 1) & 3) << 1) : q_c ^ (key & 7);
+          const uint32_t bytes = all || (pos + key >= lw.lo && pos + key < lw.hi) ? 16u : 0u;
+          cp_async16(kd + key * kRB + ck * 16, ks + i * 512, bytes);
+          cp_async16(vd + key * kRB + cv * 16, vs + i * 512, bytes);
+        }
+        if constexpr (Q8) {
+          const int key = lane & 15;
+          const uint32_t bytes = all || (pos + key >= lw.lo && pos + key < lw.hi) ? 4u : 0u;
+          cp_async4(vd + S::kBlock + lane * 4, sc + at, bytes);
+        }
+      };
+      // rows outside the keys seen (a page's stale end, or before the window) come as zeros
+      if (pos >= lw.lo && pos + 16 <= lw.hi) copy(true);
+      else copy(false);
     }
     ++lw.t;
     if (++lw.tile == lw.tile_end) more = token_seek<kTile>(a, plan, &lw);
@@ -510,14 +514,17 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            bool see = whole[h];
-            if (!see) {
+          for (int e = 0; e < 4; ++e) s[h][nt][e] = f[nt][e];
+        if (!whole[h]) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
               const int p = pos + g + 8 * (e >> 1);
-              see = ((live >> h) & 1u) && p >= col_lo[nt][e & 1] && p < col_hi[nt][e & 1];
+              if (!((live >> h) & 1u) || p < col_lo[nt][e & 1] || p >= col_hi[nt][e & 1])
+                s[h][nt][e] = -INFINITY;
             }
-            s[h][nt][e] = see ? f[nt][e] : -INFINITY;
-          }
+        }
       }
       // the weights' exponents: over 8-bit pages with the values' scales
       float y[Q8 ? KH : 1][Q8 ? NT : 1][4];
@@ -530,7 +537,14 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              y[h][nt][e] = s[h][nt][e] > -INFINITY ? s[h][nt][e] + lv[e >> 1] : -INFINITY;
+              y[h][nt][e] = s[h][nt][e] + lv[e >> 1];
+          if (!whole[h]) {  // (a scale that is not finite stays out of the columns that do not see it)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (!(s[h][nt][e] > -INFINITY)) y[h][nt][e] = s[h][nt][e];
+          }
         }
       }
       auto top_of = [&](const auto& x, int nt, int j) {
