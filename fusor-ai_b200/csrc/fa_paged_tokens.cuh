@@ -54,11 +54,13 @@ struct TokShape {
   static constexpr int kSteps = D / 16;                 // m tiles of O (and 16-bit k steps of S)
   static constexpr int kRing = kTokWarps * kStages * kStageBytes;
   static constexpr int kMergeRow = D + 4;               // floats: O, then max and sum (16-byte rows)
+  // At a unit's end each warp leaves its rows in the stage that it read last, if they fit there.
+  static constexpr bool kInStage = kCols * kMergeRow * 4 <= kStageBytes;
   // resident CTAs per SM that the registers allow
   static constexpr int kCtas = D == 256 ? (NT == 1 ? 2 : 1) : (NT == 1 ? 3 : 2);
   // dynamic shared memory for batches of `cols` packed rows and `sequences` sequences
   static int smem(int cols, int sequences) {
-    return kRing + kTokWarps * cols * kMergeRow * 4 + (sequences + 1) * 8;
+    return kRing + (kInStage ? 0 : kTokWarps * cols * kMergeRow * 4) + sequences * 24 + 8;
   }
 };
 
@@ -156,41 +158,126 @@ struct TokWalk {
 
 struct TokPlan {
   const int64_t* before;  // [sequences + 1]: tiles of the sequences before, of one KV head each
+  const int4* spans;      // [sequences]: first row, rows, first position, first key seen
   int kvh;
 };
 
-// A sequence's part in the token kernel: its span, the keys that its rows see and their tiles
-// (0 if it is empty, out of range or the chunk kernel's).
+// A sequence's part in the token kernel: its span, the first key that its rows see, and their
+// tiles (0 if it is empty or the chunk kernel's, -1 if it is out of range).
 template <int kTile>
-__device__ __forceinline__ int token_tiles(const PagedAttendArgs& a, int s, TokWalk* w) {
+__device__ __forceinline__ int token_tiles(const PagedAttendArgs& a, int s, int4* span) {
   PagedSpan sp;
+  *span = make_int4(0, 0, 0, 0);
   if (!paged_span(a.spans, a.pool.page_shift, s, &sp)) return -1;
   if (sp.n == 0 || int64_t(sp.n) * a.group > a.token_cols) return 0;
-  int lo, hi, unused;
+  int lo, unused;
   paged_keys(a.kind, a.window, sp.first, sp.first + sp.n, &lo, &unused);
-  hi = sp.first + sp.n;
-  if (w != nullptr) {
-    w->row0 = sp.row0;
-    w->n = sp.n;
-    w->first = sp.first;
-    w->lo = lo;
-    w->hi = hi;
-  }
-  return (hi + kTile - 1) / kTile - lo / kTile;
+  *span = make_int4(sp.row0, sp.n, sp.first, lo);
+  return (sp.first + sp.n + kTile - 1) / kTile - lo / kTile;
 }
 
 // Moves the walk to the unit that holds global tile w->t (w->s at or before it); false at the
 // share's end.
-template <int kTile>
-__device__ __forceinline__ bool token_seek(const PagedAttendArgs& a, const TokPlan& plan, TokWalk* w) {
+__device__ __forceinline__ bool token_seek(const TokPlan& plan, TokWalk* w) {
   if (w->t >= w->t_end) return false;
   while (plan.before[w->s + 1] * plan.kvh <= w->t) ++w->s;
-  w->tiles = token_tiles<kTile>(a, w->s, w);
+  const int4 sp = plan.spans[w->s];
+  w->row0 = sp.x;
+  w->n = sp.y;
+  w->first = sp.z;
+  w->lo = sp.w;
+  w->hi = sp.z + sp.y;
+  w->tiles = int(plan.before[w->s + 1] - plan.before[w->s]);
   const int64_t rest = w->t - plan.before[w->s] * plan.kvh;
   w->h = int(rest / w->tiles);
   w->tile = int(rest - int64_t(w->h) * w->tiles);
   w->tile_end = int(min(int64_t(w->tiles), int64_t(w->tile) + (w->t_end - w->t)));
   return true;
+}
+
+// Elements 4 v .. 4 v + 3 of a packed row's output: o / l (a row that sees no key, its pages out of
+// range, is zero).
+template <int D>
+__device__ __forceinline__ void token_write(const PagedAttendArgs& a, int row0, int h, int col, int v,
+                                            float4 o, float l) {
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  const int64_t at = int64_t(row0 + col / a.group) * a.out_stride +
+                     int64_t(h * a.group + col % a.group) * D + v * 4;
+  if (a.out_bf16) {
+    uint16_t* p = static_cast<uint16_t*>(a.out) + at;
+    const uint2 w = make_uint2(pack_bf16x2(o.x, o.y), pack_bf16x2(o.z, o.w));
+    if (a.out_vec) {
+      *reinterpret_cast<uint2*>(p) = w;
+    } else {
+      p[0] = uint16_t(w.x); p[1] = uint16_t(w.x >> 16);
+      p[2] = uint16_t(w.y); p[3] = uint16_t(w.y >> 16);
+    }
+  } else {
+    float* p = static_cast<float*>(a.out) + at;
+    if (a.out_vec) *reinterpret_cast<float4*>(p) = o;
+    else { p[0] = o.x; p[1] = o.y; p[2] = o.z; p[3] = o.w; }
+  }
+}
+
+// The partials of a unit's pieces (of CTAs c0 ..) merged into the output, by the whole CTA of the
+// piece that arrived last. Bound by trips to L2, one for each group of loads: four lanes share a
+// vector of the output, each with a quarter of the pieces, eight at a time, and a piece's maximum
+// is loaded beside its output (the sums are rescaled as the maximum grows), so that 32 pieces
+// cost one trip; in an order that does not depend on who arrived last. Not inlined: the loop over
+// the keys has its registers to itself.
+template <int D>
+__device__ __noinline__ void token_merge(const PagedAttendArgs& a, int row0, int h, int cols, int c0,
+                                         int pieces) {
+  constexpr int kVecs = D / 4, kGroup = 8;
+  const int sub = threadIdx.x & 3;
+  for (int i = threadIdx.x / 4; i < cols * kVecs; i += kTokThreads / 4) {
+    const int col = i / kVecs, v = i % kVecs;
+    float mm = -INFINITY, ll = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+    for (int b = 0; b < pieces; b += 4 * kGroup) {
+      float2 ml[kGroup];
+      float4 x[kGroup];
+#pragma unroll
+      for (int k = 0; k < kGroup; ++k) {
+        // (past the end the last piece's again, without a weight)
+        const int c = c0 + min(b + 4 * k + sub, pieces - 1);
+        const int64_t at = int64_t(2 * c + (c == c0 ? 1 : 0)) * kPagedTokenCols + col;
+        ml[k] = __ldcg(reinterpret_cast<const float2*>(a.part_ml + at * 2));
+        x[k] = __ldcg(reinterpret_cast<const float4*>(a.part_o + at * D + 4 * v));
+      }
+#pragma unroll
+      for (int k = 0; k < kGroup; ++k) {
+        if (b + 4 * k + sub >= pieces) break;
+        // a piece that saw no key has sum 0 (or NaN, which stays)
+        if (ml[k].x == -INFINITY) { ll += ml[k].y; continue; }
+        const float top = fmaxf(mm, ml[k].x);
+        const float f = exp2_approx(ml[k].x - top);
+        const float e = mm == -INFINITY ? 1.0f : exp2_approx(mm - top);
+        mm = top;
+        ll = fmaf(ll, e, f * ml[k].y);
+        acc.x = fmaf(acc.x, e, f * x[k].x); acc.y = fmaf(acc.y, e, f * x[k].y);
+        acc.z = fmaf(acc.z, e, f * x[k].z); acc.w = fmaf(acc.w, e, f * x[k].w);
+      }
+    }
+    __syncwarp();
+    float top = mm;
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const float f = mm == -INFINITY ? 1.0f : exp2_approx(mm - top);
+    ll *= f;
+    acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+#pragma unroll
+    for (int off = 1; off <= 2; off <<= 1) {
+      ll += __shfl_xor_sync(0xffffffffu, ll, off);
+      acc.x += __shfl_xor_sync(0xffffffffu, acc.x, off);
+      acc.y += __shfl_xor_sync(0xffffffffu, acc.y, off);
+      acc.z += __shfl_xor_sync(0xffffffffu, acc.z, off);
+      acc.w += __shfl_xor_sync(0xffffffffu, acc.w, off);
+    }
+    if (sub == 0) token_write<D>(a, row0, h, col, v, acc, ll);
+  }
 }
 
 template <int D, bool Q8, int NT>
@@ -203,8 +290,9 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
   __shared__ int64_t scratch[kTokWarps];
   __shared__ int arrived;
   const int mcols = a.merge_cols;  // packed rows that any sequence has
-  float* merge = reinterpret_cast<float*>(smem + S::kRing);
-  int64_t* before = reinterpret_cast<int64_t*>(merge + kTokWarps * mcols * S::kMergeRow);
+  int4* spans = reinterpret_cast<int4*>(
+      smem + S::kRing + (S::kInStage ? 0 : kTokWarps * mcols * S::kMergeRow * 4));
+  int64_t* before = reinterpret_cast<int64_t*>(spans + a.spans.sequences);
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
@@ -220,7 +308,7 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
     const int s0 = min(nseq, int(threadIdx.x) * each), s1 = min(nseq, s0 + each);
     int64_t sum = 0;
     for (int s = s0; s < s1; ++s) {
-      const int n = token_tiles<kTile>(a, s, nullptr);
+      const int n = token_tiles<kTile>(a, s, &spans[s]);
       if (n < 0) atomicOr(a.err, kErrPagedSpan);
       sum += max(n, 0);
       before[s] = sum;  // inclusive within the thread's sequences, for now
@@ -236,7 +324,7 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
     if (threadIdx.x == 0) before[nseq] = total;
     __syncthreads();
   }
-  const TokPlan plan{before, kvh};
+  const TokPlan plan{before, spans, kvh};
   const int64_t work = before[nseq] * kvh;
   if (work == 0) return;
   // at least two tiles a CTA: a piece costs about as much as streaming one
@@ -258,7 +346,7 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
 
   // ---- loads: one stage at a time --------------------------------------------------------------
   const int shift = a.pool.page_shift;
-  bool more = token_seek<kTile>(a, plan, &lw);
+  bool more = token_seek(plan, &lw);
   int next_page[KH];  // the pages of the next stage's 16s of keys (-1: none of them is seen)
   auto stage_pos = [&](const TokWalk& w) { return (w.lo / kTile + w.tile) * kTile + warp * (16 * KH); };
   auto fetch_pages = [&]() {
@@ -314,7 +402,7 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
       else copy(false);
     }
     ++lw.t;
-    if (++lw.tile == lw.tile_end) more = token_seek<kTile>(a, plan, &lw);
+    if (++lw.tile == lw.tile_end) more = token_seek(plan, &lw);
     fetch_pages();
   };
 #pragma unroll
@@ -325,7 +413,7 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
 
   // ---- the products ---------------------------------------------------------------------------
   int stage = 0;
-  while (token_seek<kTile>(a, plan, &cw)) {
+  while (token_seek(plan, &cw)) {
     // This lane's query column g (+ 8): its fragments. 8-bit pages: bytes of hi and lo for the
     // lane's chunks, two words for each product of 32 elements; bf16: pairs.
     constexpr int kFrags = Q8 ? D / 32 : S::kSteps;
@@ -691,6 +779,15 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
       }
     }
 
+    // every warp's rows: in its stage read last (the same for all, as are the tiles)
+    const int done = stage == 0 ? S::kStages - 1 : stage - 1;
+    auto merge_of = [&](int w) {
+      return reinterpret_cast<float*>(
+          S::kInStage ? smem + w * (S::kStages * S::kStageBytes) + done * S::kStageBytes
+                      : smem + S::kRing + w * (mcols * S::kMergeRow * 4));
+    };
+    __syncwarp();  // (the stage's last reads are done)
+
     // ---- the unit's (or piece's) end: the warps' parts merged -----------------------------------
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -712,7 +809,7 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
             o[k][nt][2 + j] *= f;
           }
         }
-        float* row = merge + (warp * mcols + col) * S::kMergeRow;
+        float* row = merge_of(warp) + col * S::kMergeRow;
         if (g == 0) { row[D] = m[nt][j]; row[D + 1] = l[nt][j]; }
 #pragma unroll
         for (int k = 0; k < S::kSteps; ++k) {
@@ -734,35 +831,17 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
     const int pieces = c1 - c0 + 1;
     const int cols = cw.n * a.group;
     constexpr int kVecs = D / 4;  // float4s of a column
-    auto write_out = [&](int col, int v, float4 x, float inv) {
-      const int64_t at = int64_t(cw.row0 + col / a.group) * a.out_stride +
-                         int64_t(cw.h * a.group + col % a.group) * D + v * 4;
-      x = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-      if (a.out_bf16) {
-        __nv_bfloat16* p = static_cast<__nv_bfloat16*>(a.out) + at;
-        if (a.out_vec) {
-          *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
-        } else {
-          p[0] = __float2bfloat16_rn(x.x); p[1] = __float2bfloat16_rn(x.y);
-          p[2] = __float2bfloat16_rn(x.z); p[3] = __float2bfloat16_rn(x.w);
-        }
-      } else {
-        float* p = static_cast<float*>(a.out) + at;
-        if (a.out_vec) *reinterpret_cast<float4*>(p) = x;
-        else { p[0] = x.x; p[1] = x.y; p[2] = x.z; p[3] = x.w; }
-      }
-    };
     const int slot = 2 * cta + (cta == c0 ? 1 : 0);
     for (int i = threadIdx.x; i < cols * kVecs; i += kTokThreads) {
       const int col = i / kVecs, v = i % kVecs;
       float mm = -INFINITY, ll = 0.0f;
 #pragma unroll
       for (int w = 0; w < kTokWarps; ++w)
-        mm = fmaxf(mm, merge[(w * mcols + col) * S::kMergeRow + D]);
+        mm = fmaxf(mm, merge_of(w)[col * S::kMergeRow + D]);
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int w = 0; w < kTokWarps; ++w) {
-        const float* row = merge + (w * mcols + col) * S::kMergeRow;
+        const float* row = merge_of(w) + col * S::kMergeRow;
         const float f = row[D] == -INFINITY ? 0.0f : exp2_approx(row[D] - mm);
         // a warp that saw no key has sum 0 (or NaN, which stays)
         ll += row[D] == -INFINITY ? row[D + 1] : f * row[D + 1];
@@ -772,7 +851,7 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
       }
       if (pieces == 1) {
         // a row that sees no key (every page out of range) is zero
-        write_out(col, v, acc, ll == 0.0f ? 0.0f : 1.0f / ll);
+        token_write<D>(a, cw.row0, cw.h, col, v, acc, ll);
       } else {
         *reinterpret_cast<float4*>(a.part_o + (int64_t(slot) * kPagedTokenCols + col) * D + 4 * v) = acc;
         if (v == 0)
@@ -791,29 +870,7 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
       __syncthreads();
       if (arrived) {
         __threadfence();
-        for (int i = threadIdx.x; i < cols * kVecs; i += kTokThreads) {
-          const int col = i / kVecs, v = i % kVecs;
-          auto ml_at = [&](int c) {
-            const int64_t at = int64_t(2 * c + (c == c0 ? 1 : 0)) * kPagedTokenCols + col;
-            return __ldcg(reinterpret_cast<const float2*>(a.part_ml + at * 2));
-          };
-          float mm = -INFINITY;
-#pragma unroll 8
-          for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, ml_at(c).x);
-          float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          float ll = 0.0f;
-#pragma unroll 8
-          for (int c = c0; c <= c1; ++c) {
-            const float2 ml = ml_at(c);
-            const float f = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - mm);
-            ll += ml.x == -INFINITY ? ml.y : f * ml.y;
-            const int64_t at = int64_t(2 * c + (c == c0 ? 1 : 0)) * kPagedTokenCols + col;
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(a.part_o + at * D + 4 * v));
-            acc.x = fmaf(f, x.x, acc.x); acc.y = fmaf(f, x.y, acc.y);
-            acc.z = fmaf(f, x.z, acc.z); acc.w = fmaf(f, x.w, acc.w);
-          }
-          write_out(col, v, acc, ll == 0.0f ? 0.0f : 1.0f / ll);
-        }
+        token_merge<D>(a, cw.row0, cw.h, cols, c0, pieces);
       }
     }
     __syncthreads();  // the merge rows are free again
