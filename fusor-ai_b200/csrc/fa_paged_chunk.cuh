@@ -278,7 +278,7 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
     w.nq = chunk_units<NQ>(a, s0, &sp);
     const int64_t per = before[s0 + 1] - before[s0];
     const int64_t rest = w.t - before[s0] * kvh;
-    w.h = int(rest / per);
+    w.h = whole_times(rest, per);
     int64_t off = rest - int64_t(w.h) * per;  // tiles into the head
     w.qt = 0;
     for (;;) {  // 32 units at a time

@@ -189,7 +189,7 @@ __device__ __forceinline__ bool token_seek(const TokPlan& plan, TokWalk* w) {
   w->hi = sp.z + sp.y;
   w->tiles = int(plan.before[w->s + 1] - plan.before[w->s]);
   const int64_t rest = w->t - plan.before[w->s] * plan.kvh;
-  w->h = int(rest / w->tiles);
+  w->h = whole_times(rest, w->tiles);
   w->tile = int(rest - int64_t(w->h) * w->tiles);
   w->tile_end = int(min(int64_t(w->tiles), int64_t(w->tile) + (w->t_end - w->t)));
   return true;
@@ -221,55 +221,68 @@ __device__ __forceinline__ void token_write(const PagedAttendArgs& a, int row0, 
 }
 
 // The partials of a unit's pieces (of CTAs c0 ..) merged into the output, by the whole CTA of the
-// piece that arrived last. Bound by trips to L2, one for each group of loads: four lanes share a
-// vector of the output, each with a quarter of the pieces, eight at a time, and a piece's maximum
-// is loaded beside its output (the sums are rescaled as the maximum grows), so that 32 pieces
-// cost one trip; in an order that does not depend on who arrived last. Not inlined: the loop over
-// the keys has its registers to itself.
+// piece that arrived last. Bound by trips to L2, one for each group of loads: of more than eight
+// pieces four lanes share a vector of the output, each with a quarter of the pieces, and a piece's
+// maximum is loaded beside its output (the sums are rescaled as the maximum grows), so that 8
+// pieces, or 32, cost one trip; in an order that does not depend on who arrived last. Not inlined:
+// the loop over the keys has its registers to itself.
 template <int D>
 __device__ __noinline__ void token_merge(const PagedAttendArgs& a, int row0, int h, int cols, int c0,
                                          int pieces) {
   constexpr int kVecs = D / 4, kGroup = 8;
-  const int sub = threadIdx.x & 3;
-  for (int i = threadIdx.x / 4; i < cols * kVecs; i += kTokThreads / 4) {
+  const int lanes = pieces > 8 ? 4 : 1;
+  const int sub = threadIdx.x & (lanes - 1);
+  for (int i = threadIdx.x / lanes; i < cols * kVecs; i += kTokThreads / lanes) {
     const int col = i / kVecs, v = i % kVecs;
+    // piece j's row, in slot 2 (c0 + j), or 2 c0 + 1 for j = 0
+    const int64_t at0 = int64_t(2 * c0) * kPagedTokenCols + col;
+    const float* const o0 = a.part_o + at0 * D + 4 * v;
+    const float* const ml0 = a.part_ml + at0 * 2;
     float mm = -INFINITY, ll = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 1
-    for (int b = 0; b < pieces; b += 4 * kGroup) {
+    for (int b = sub; b < pieces; b += lanes * kGroup) {
       float2 ml[kGroup];
       float4 x[kGroup];
 #pragma unroll
       for (int k = 0; k < kGroup; ++k) {
         // (past the end the last piece's again, without a weight)
-        const int c = c0 + min(b + 4 * k + sub, pieces - 1);
-        const int64_t at = int64_t(2 * c + (c == c0 ? 1 : 0)) * kPagedTokenCols + col;
-        ml[k] = __ldcg(reinterpret_cast<const float2*>(a.part_ml + at * 2));
-        x[k] = __ldcg(reinterpret_cast<const float4*>(a.part_o + at * D + 4 * v));
+        const int j = min(b + lanes * k, pieces - 1);
+        const int row = (j == 0 ? 1 : 2 * j) * kPagedTokenCols;
+        ml[k] = __ldcg(reinterpret_cast<const float2*>(ml0 + row * 2));
+        x[k] = __ldcg(reinterpret_cast<const float4*>(o0 + row * D));
       }
+      float top = mm;
 #pragma unroll
       for (int k = 0; k < kGroup; ++k) {
-        if (b + 4 * k + sub >= pieces) break;
+        if (b + lanes * k >= pieces) ml[k] = make_float2(-INFINITY, 0.0f);
+        top = fmaxf(top, ml[k].x);
+      }
+      const float e = mm == -INFINITY ? 1.0f : exp2_approx(mm - top);
+      mm = top;
+      ll *= e;
+      acc = make_float4(acc.x * e, acc.y * e, acc.z * e, acc.w * e);
+#pragma unroll
+      for (int k = 0; k < kGroup; ++k) {
         // a piece that saw no key has sum 0 (or NaN, which stays)
-        if (ml[k].x == -INFINITY) { ll += ml[k].y; continue; }
-        const float top = fmaxf(mm, ml[k].x);
-        const float f = exp2_approx(ml[k].x - top);
-        const float e = mm == -INFINITY ? 1.0f : exp2_approx(mm - top);
-        mm = top;
-        ll = fmaf(ll, e, f * ml[k].y);
-        acc.x = fmaf(acc.x, e, f * x[k].x); acc.y = fmaf(acc.y, e, f * x[k].y);
-        acc.z = fmaf(acc.z, e, f * x[k].z); acc.w = fmaf(acc.w, e, f * x[k].w);
+        const float f = ml[k].x == -INFINITY ? 0.0f : exp2_approx(ml[k].x - mm);
+        ll += ml[k].x == -INFINITY ? ml[k].y : f * ml[k].y;
+        acc.x = fmaf(f, x[k].x, acc.x); acc.y = fmaf(f, x[k].y, acc.y);
+        acc.z = fmaf(f, x[k].z, acc.z); acc.w = fmaf(f, x[k].w, acc.w);
       }
     }
-    __syncwarp();
-    float top = mm;
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const float f = mm == -INFINITY ? 1.0f : exp2_approx(mm - top);
-    ll *= f;
-    acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+    if (lanes == 4) {  // (whole warps have the same items)
+      __syncwarp();
+      float top = mm;
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float f = mm == -INFINITY ? 1.0f : exp2_approx(mm - top);
+      ll *= f;
+      acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+    }
 #pragma unroll
-    for (int off = 1; off <= 2; off <<= 1) {
+    for (int off = 1; off < 4; off <<= 1) {
+      if (lanes == 1) break;
       ll += __shfl_xor_sync(0xffffffffu, ll, off);
       acc.x += __shfl_xor_sync(0xffffffffu, acc.x, off);
       acc.y += __shfl_xor_sync(0xffffffffu, acc.y, off);
@@ -327,8 +340,7 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
   const TokPlan plan{before, spans, kvh};
   const int64_t work = before[nseq] * kvh;
   if (work == 0) return;
-  // at least two tiles a CTA: a piece costs about as much as streaming one
-  const int ctas = int(min(int64_t(gridDim.x), (work + 1) / 2));
+  const int ctas = int(min(int64_t(gridDim.x), work));  // a tile each at least
   const int cta = blockIdx.x;
   if (cta >= ctas) return;
 

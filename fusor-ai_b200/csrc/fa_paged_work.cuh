@@ -16,14 +16,22 @@
 
 namespace fa {
 
-// CTA c's first tile of W shared among n.
+// CTA c's first tile of W shared among n. (A 64-bit division takes some hundred instructions, which
+// short calls wait for: 32 bits where they do, n being at most 4096.)
 __device__ __forceinline__ int64_t share_begin(int64_t w, int c, int n) {
+  if (w < (1 << 20)) return int64_t(uint32_t(w) * uint32_t(c) / uint32_t(n));
   return int64_t((unsigned long long)(w) * (unsigned long long)(c) / (unsigned long long)(n));
 }
 
 // The CTA whose share holds tile t.
 __device__ __forceinline__ int share_owner(int64_t w, int64_t t, int n) {
+  if (w < (1 << 20)) return int(((uint32_t(t) + 1) * uint32_t(n) - 1) / uint32_t(w));
   return int((((unsigned long long)(t) + 1) * (unsigned long long)(n)-1) / (unsigned long long)(w));
+}
+
+// How many times `per` goes into t.
+__device__ __forceinline__ int whole_times(int64_t t, int64_t per) {
+  return t < (1 << 30) ? int(uint32_t(t) / uint32_t(per)) : int(t / per);
 }
 
 // Exclusive prefix sums over the CTA's threads of one value each, and the total (every thread);
