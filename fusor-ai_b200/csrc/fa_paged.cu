@@ -298,7 +298,11 @@ int attend(const fa_paged_cache* c, int layer, const fa_paged_batch* b, const vo
   if (chunks) {
     fa::PagedAttendArgs ca = a;
     ca.counters += w.chunk_counters;
+    // Beside the chunk kernel the token kernel takes sequences of one 8-column product alone (its
+    // 16-column form holds twice the accumulators and two CTAs an SM, not three: 59 against 37 us
+    // for 24 single tokens of 2000 positions each), where a token fits in it.
     if (!tokens) ca.token_cols = 0;
+    else if (a.group <= 8) ca.token_cols = a.token_cols = 8;
     const cudaError_t rc = fa::launch_paged_chunk(ca, sms, s);
     if (rc != cudaSuccess) return cuda_fail(rc, "paged chunk launch");
   }

@@ -50,11 +50,11 @@ struct PagedSpan {
   int row0, n, first;
 };
 
-// Sequence s's span, or false if it is out of range: rows that are not within the call's or run
-// backwards, more rows than max_rows, a negative position or positions past its table. Nothing
-// of such a sequence is read or written.
-FA_HD bool paged_span(const PagedSpans& b, int page_shift, int s, PagedSpan* out) {
-  const int r0 = b.row_starts[s], r1 = b.row_starts[s + 1], first = b.firsts[s];
+// The span of rows r0 .. r1 from position `first` on, or false if it is out of range: rows that are
+// not within the call's or run backwards, more rows than max_rows, a negative position or positions
+// past its table. Nothing of such a sequence is read or written.
+FA_HD bool paged_span_of(const PagedSpans& b, int page_shift, int r0, int r1, int first,
+                         PagedSpan* out) {
   out->row0 = r0;
   out->n = 0;
   out->first = first;
@@ -63,6 +63,11 @@ FA_HD bool paged_span(const PagedSpans& b, int page_shift, int s, PagedSpan* out
   if (int64_t(first) + (r1 - r0) > 0x7fffff00) return false;  // positions stay 32-bit integers
   out->n = r1 - r0;
   return true;
+}
+
+// Sequence s's span.
+FA_HD bool paged_span(const PagedSpans& b, int page_shift, int s, PagedSpan* out) {
+  return paged_span_of(b, page_shift, b.row_starts[s], b.row_starts[s + 1], b.firsts[s], out);
 }
 
 // Whether a page id names a page of the pool.

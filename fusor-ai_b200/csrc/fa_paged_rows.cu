@@ -16,29 +16,34 @@ namespace {
 
 constexpr int kRowWarps = 8;
 
-// The sequence that holds row r: the number of sequences that end at or before it (one warp;
-// row_starts rises, or the span check refuses what is found). Up to 32 sequences take one load,
-// up to 1024 two.
-__device__ __forceinline__ int sequence_of(const PagedSpans& b, int r, int lane) {
+// Row r's place: its page and slot, or false (with the error word set) if the batch's numbers are
+// out of range. Rows past the last sequence's are left alone. One warp; two trips to memory (three
+// for more than 32 sequences): the row's sequence s is the number of sequences that end at or
+// before it (row_starts rises, or the span check refuses what is found), and each lane has its
+// sequence's span at hand when s is known.
+__device__ __forceinline__ bool place_of(const PagedSpans& b, const PagedPool& pool, int r,
+                                         int lane, int* page, int* slot, unsigned* err) {
   int base = 0;
   if (b.sequences > 32) {
     const int at = (lane + 1) * 32;  // the end of block `lane` of 32 sequences
     const bool past = at <= b.sequences && b.row_starts[at] <= r;
     base = 32 * __popc(__ballot_sync(0xffffffffu, past));
   }
-  const int at = base + lane + 1;
-  const bool past = at <= b.sequences && b.row_starts[at] <= r;
-  return base + __popc(__ballot_sync(0xffffffffu, past));
-}
-
-// Row r's place: its page and slot and its sequence's span, or false (with the error word set)
-// if the batch's numbers are out of range. Rows past the last sequence's are left alone.
-__device__ __forceinline__ bool place_of(const PagedSpans& b, const PagedPool& pool, int r,
-                                         int lane, int* page, int* slot, unsigned* err) {
-  const int s = sequence_of(b, r, lane);
+  const int mine = base + lane;
+  int r0 = 0, r1 = 0x7fffffff, first = 0;
+  if (mine < b.sequences) {
+    r0 = b.row_starts[mine];
+    r1 = b.row_starts[mine + 1];
+    first = b.firsts[mine];
+  }
+  const int in = __popc(__ballot_sync(0xffffffffu, mine < b.sequences && r1 <= r));
+  const int s = base + in;
   if (s >= b.sequences) return false;
+  r0 = __shfl_sync(0xffffffffu, r0, in & 31);
+  r1 = __shfl_sync(0xffffffffu, r1, in & 31);
+  first = __shfl_sync(0xffffffffu, first, in & 31);
   PagedSpan span;
-  const bool ok = paged_span(b, pool.page_shift, s, &span);
+  const bool ok = in < 32 && paged_span_of(b, pool.page_shift, r0, r1, first, &span);
   if (!ok || r < span.row0 || r >= span.row0 + span.n) {
     if (lane == 0) atomicOr(err, kErrPagedSpan);
     return false;
@@ -144,7 +149,9 @@ __device__ __forceinline__ void keep_head(const PagedPool& pool, bool is_key, in
 }
 
 // One CTA per row; a warp takes every kRowWarps-th head unit (query heads, key heads, value
-// heads), two at a time so that their loads are in flight together. Lane l holds elements lE ..
+// heads), U at a time so that their loads are in flight together, the first of them while the
+// row's place is looked up. Bound by memory: 10 thousand rows of 32/8 heads of 128 (bf16 rows, 8-bit
+// pages) move 231 MB. Lane l holds elements lE ..
 // lE + E - 1 of a head: RoPE by halves finds the partner of e in lane l ^ 16, interleaved RoPE
 // within the lane, and the row's cosines and sines are loaded once for all of the warp's heads.
 // Arithmetic of the rotation: each product rounded, then the difference or sum (ops.rs:77-95).
@@ -152,29 +159,15 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kRowWarps * 32)
     paged_write_kernel(const __grid_constant__ PagedWriteArgs a) {
   constexpr int E = D / 32;
-  constexpr int U = 2;
+  constexpr int U = D == 256 ? 4 : 6;
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r = blockIdx.x;
   const int kvh = a.pool.kv_heads;
   const int units = a.heads + 2 * kvh;
-  int page, slot;
-  if (!place_of(a.spans, a.pool, r, lane, &page, &slot, a.err)) return;  // the warp's, as one
-  float c[E], s[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) c[e] = s[e] = 0.0f;
-  if (a.rope == 1) {
-    const float* cs = a.angles + int64_t(r) * D + (lane & 15) * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) { c[e] = cs[e]; s[e] = cs[D / 2 + e]; }
-  } else if (a.rope == 2) {
-    const float* cs = a.angles + int64_t(r) * D + lane * (E / 2);
-#pragma unroll
-    for (int e = 0; e < E / 2; ++e) { c[e] = cs[e]; s[e] = cs[D / 2 + e]; }
-  }
-  for (int u0 = warp; u0 < units; u0 += U * kRowWarps) {
-    float xs[U][E];
+  float xs[U][E];
+  auto load = [&](int u0) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int u = u0 + i * kRowWarps;
@@ -189,6 +182,24 @@ __global__ void __launch_bounds__(kRowWarps * 32)
             int64_t(u - a.heads - kvh) * a.v_head_stride;
       load_elems<T, E>(p + lane * E, a.vec != 0, xs[i]);
     }
+  };
+  load(warp);
+  float c[E], s[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) c[e] = s[e] = 0.0f;
+  if (a.rope == 1) {
+    const float* cs = a.angles + int64_t(r) * D + (lane & 15) * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) { c[e] = cs[e]; s[e] = cs[D / 2 + e]; }
+  } else if (a.rope == 2) {
+    const float* cs = a.angles + int64_t(r) * D + lane * (E / 2);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) { c[e] = cs[e]; s[e] = cs[D / 2 + e]; }
+  }
+  int page, slot;
+  if (!place_of(a.spans, a.pool, r, lane, &page, &slot, a.err)) return;  // the warp's, as one
+  for (int u0 = warp; u0 < units; u0 += U * kRowWarps) {
+    if (u0 != warp) load(u0);
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int u = u0 + i * kRowWarps;
@@ -233,76 +244,78 @@ __global__ void __launch_bounds__(kRowWarps * 32)
   }
 }
 
-// 16 rows a CTA: their places once, then every thread 16 bytes of a page's row at a time (keys
-// and values), four such loads in flight.
-constexpr int kReadRows = 16;
+// A warp takes two rows: their places, then 16 bytes of them a lane at a time, eight such loads in
+// flight (two vectors of keys and of values of each row). Bound by memory.
+constexpr int kReadWarps = 8, kReadRows = 2 * kReadWarps;
 
-__global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__ PagedReadArgs a) {
+template <bool Q8, int D>
+__global__ void __launch_bounds__(kReadWarps * 32)
+    paged_read_kernel(const __grid_constant__ PagedReadArgs a) {
+  constexpr int kElems = Q8 ? 16 : 8;          // of a 16-byte vector
+  constexpr int kPerHead = D / kElems;         // vectors of a head
   pdl_wait();
   pdl_trigger();
-  __shared__ int64_t place[kReadRows];  // (page, slot)'s row of KV head 0, or -1
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int r0 = blockIdx.x * kReadRows;
-  for (int i = warp; i < kReadRows; i += 8) {
+  const int r0 = blockIdx.x * kReadRows + warp;
+  int64_t place[2];  // (page, slot)'s row of KV head 0, or -1
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = r0 + i * kReadWarps;
     int page = 0, slot = 0;
-    const bool ok = r0 + i < a.spans.rows &&
-                    place_of(a.spans, a.pool, r0 + i, lane, &page, &slot, a.err);
-    if (lane == 0)
-      place[i] = ok ? ((int64_t(page) * a.pool.kv_heads) << a.pool.page_shift) + slot : -1;
+    const bool ok = r < a.spans.rows && place_of(a.spans, a.pool, r, lane, &page, &slot, a.err);
+    place[i] = ok ? ((int64_t(page) * a.pool.kv_heads) << a.pool.page_shift) + slot : -1;
   }
-  __syncthreads();
-  const int d = a.pool.head_dim;
-  const int elems = a.pool.q8 ? 16 : 8;  // of a 16-byte vector
-  const int per_head = d / elems, per_row = per_head * a.pool.kv_heads;
-  const int items = kReadRows * per_row * 2;
-  constexpr int U = 4;
-  for (int i0 = threadIdx.x; i0 < items; i0 += 256 * U) {
-    uint4 raw[U];
-    float scale[U];
-    int64_t to[U];
+  const int vectors = a.pool.kv_heads * kPerHead;
+  for (int x0 = lane; x0 < vectors; x0 += 64) {
+    uint4 raw[2][2][2];   // [row][vector][keys, values]
+    float scale[2][2][2];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * 256;
-      to[u] = -1;
-      if (i >= items) continue;
-      const int c = i % per_head, rest = i / per_head;
-      const int h = rest % a.pool.kv_heads, row = (rest / a.pool.kv_heads) % kReadRows;
-      const bool is_key = rest / a.pool.kv_heads < kReadRows;
-      if (place[row] < 0) continue;
-      const int64_t at = place[row] + (int64_t(h) << a.pool.page_shift);
-      const unsigned char* base = is_key ? a.pool.keys : a.pool.values;
-      raw[u] = __ldcs(reinterpret_cast<const uint4*>(base) + at * per_head + c);
-      scale[u] = a.pool.q8 ? (is_key ? a.pool.key_scales : a.pool.value_scales)[at] : 1.0f;
-      to[u] = int64_t(r0 + row) * (is_key ? a.k_stride : a.v_stride) +
-              int64_t(h) * (is_key ? a.k_head_stride : a.v_head_stride) + c * elems;
-    }
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (to[u] < 0) continue;
-      const int i = i0 + u * 256;
-      const bool is_key = i / per_head / a.pool.kv_heads < kReadRows;
-      void* out = is_key ? a.k : a.v;
-      if (a.pool.q8) {
-        const signed char* q = reinterpret_cast<const signed char*>(&raw[u]);
-        float x[8], y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = float(q[e]) * scale[u];
-          y[e] = float(q[8 + e]) * scale[u];
+      for (int j = 0; j < 2; ++j) {
+        const int x = x0 + 32 * j;
+        if (place[i] < 0 || x >= vectors) continue;
+        const int64_t at = place[i] + (int64_t(x / kPerHead) << a.pool.page_shift);
+        raw[i][j][0] = __ldcs(reinterpret_cast<const uint4*>(a.pool.keys) + at * kPerHead + x % kPerHead);
+        raw[i][j][1] = __ldcs(reinterpret_cast<const uint4*>(a.pool.values) + at * kPerHead + x % kPerHead);
+        if constexpr (Q8) {
+          scale[i][j][0] = a.pool.key_scales[at];
+          scale[i][j][1] = a.pool.value_scales[at];
         }
-        store_elems<8>(out, to[u], a.out_bf16 != 0, a.vec != 0, x);
-        store_elems<8>(out, to[u] + 8, a.out_bf16 != 0, a.vec != 0, y);
-      } else {
-        const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[2 * e] = bf16_lo(w[e]);
-          x[2 * e + 1] = bf16_hi(w[e]);
-        }
-        store_elems<8>(out, to[u], a.out_bf16 != 0, a.vec != 0, x);
       }
-    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int x = x0 + 32 * j;
+        if (place[i] < 0 || x >= vectors) continue;
+        const int64_t r = r0 + i * kReadWarps;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          void* out = kv ? a.v : a.k;
+          const int64_t to = r * (kv ? a.v_stride : a.k_stride) +
+                             int64_t(x / kPerHead) * (kv ? a.v_head_stride : a.k_head_stride) +
+                             (x % kPerHead) * kElems;
+          const uint4 w4 = raw[i][j][kv];
+          if constexpr (Q8) {
+            const signed char* q = reinterpret_cast<const signed char*>(&w4);
+            float y[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) y[e] = float(q[e]) * scale[i][j][kv];
+            store_elems<8>(out, to, a.out_bf16 != 0, a.vec != 0, *reinterpret_cast<const float(*)[8]>(&y[0]));
+            store_elems<8>(out, to + 8, a.out_bf16 != 0, a.vec != 0, *reinterpret_cast<const float(*)[8]>(&y[8]));
+          } else {
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              y[2 * e] = bf16_lo(w[e]);
+              y[2 * e + 1] = bf16_hi(w[e]);
+            }
+            store_elems<8>(out, to, a.out_bf16 != 0, a.vec != 0, y);
+          }
+        }
+      }
   }
 }
 
@@ -344,7 +357,15 @@ cudaError_t launch_paged_write(const PagedWriteArgs& a, cudaStream_t stream) {
 
 cudaError_t launch_paged_read(const PagedReadArgs& a, cudaStream_t stream) {
   if (a.spans.rows == 0) return cudaSuccess;
-  return launch(paged_read_kernel, (a.spans.rows + kReadRows - 1) / kReadRows, 256, a, stream);
+  auto go = [&](void (*k)(PagedReadArgs)) {
+    return launch(k, (a.spans.rows + kReadRows - 1) / kReadRows, kReadWarps * 32, a, stream);
+  };
+  switch (a.pool.head_dim) {
+    case 64: return go(a.pool.q8 ? paged_read_kernel<true, 64> : paged_read_kernel<false, 64>);
+    case 128: return go(a.pool.q8 ? paged_read_kernel<true, 128> : paged_read_kernel<false, 128>);
+    case 256: return go(a.pool.q8 ? paged_read_kernel<true, 256> : paged_read_kernel<false, 256>);
+    default: return cudaErrorInvalidValue;
+  }
 }
 
 }  // namespace fa

@@ -16,7 +16,7 @@ cudaError_t launch_tokens(PagedAttendArgs a, int sms, cudaStream_t stream) {
   static std::atomic<bool> configured[64];  // per instantiation, per device
   cudaError_t e = smem_limit_once(kernel, S::smem(S::kCols, kMaxPagedSequences), configured);
   if (e != cudaSuccess) return e;
-  a.merge_cols = int(std::min<int64_t>(S::kCols, int64_t(a.spans.max_rows) * a.group));
+  a.merge_cols = int(std::min<int64_t>(a.token_cols, int64_t(a.spans.max_rows) * a.group));
   const int smem = S::smem(a.merge_cols, a.spans.sequences);
   // the CTAs that an SM holds: 228 KB, of which each takes 1 KB besides its own (and its statics)
   const int fit = std::max(1, std::min(S::kCtas, (228 * 1024) / (smem + 1024 + 128)));
@@ -26,7 +26,7 @@ cudaError_t launch_tokens(PagedAttendArgs a, int sms, cudaStream_t stream) {
 template <int D>
 cudaError_t launch_dim(const PagedAttendArgs& a, int sms, cudaStream_t stream) {
   // 8 columns where no sequence has more: half the products and accumulators
-  const bool wide = int64_t(std::min(a.spans.max_rows, kPagedTokenCols)) * a.group > 8;
+  const bool wide = std::min<int64_t>(int64_t(a.spans.max_rows) * a.group, a.token_cols) > 8;
   if (a.pool.q8)
     return wide ? launch_tokens<D, true, 2>(a, sms, stream) : launch_tokens<D, true, 1>(a, sms, stream);
   return wide ? launch_tokens<D, false, 2>(a, sms, stream) : launch_tokens<D, false, 1>(a, sms, stream);
