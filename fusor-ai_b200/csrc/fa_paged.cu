@@ -247,7 +247,7 @@ int write_input(const fa_paged_cache* c, int layer, const fa_paged_batch* b, int
   a.v = base + int64_t(c->heads + c->kv_heads) * d * e;
   a.q_stride = a.k_stride = a.v_stride = qkv_stride;
   a.k_head_stride = a.v_head_stride = d;
-  a.vec = vectors(qkv, {qkv_stride}, e, std::min(16, d / 32 * e));
+  a.vec = vectors(qkv, {qkv_stride}, e, 16);
   a.angles = angles;
   a.q_norm = norm ? norm->q_norm : nullptr;
   a.k_norm = norm ? norm->k_norm : nullptr;
@@ -255,7 +255,7 @@ int write_input(const fa_paged_cache* c, int layer, const fa_paged_batch* b, int
   a.q_out = q_out;
   a.q_out_stride = q_out_stride;
   const int oe = q_out_dtype == FA_BF16 ? 2 : 4;
-  a.q_out_vec = vectors(q_out, {q_out_stride}, oe, std::min(16, d / 32 * oe));
+  a.q_out_vec = vectors(q_out, {q_out_stride}, oe, 16);
   a.err = err;
   const cudaError_t rc = fa::launch_paged_write(a, s);
   if (rc != cudaSuccess) return cuda_fail(rc, "paged write launch");
@@ -424,9 +424,8 @@ int fa_paged_write(const fa_paged_cache* cache, int32_t layer, const fa_paged_ba
   a.v = rows->values;
   a.k_stride = a.v_stride = rows->row_stride;
   a.k_head_stride = a.v_head_stride = rows->head_stride;
-  const int lane = std::min(16, cache->head_dim / 32 * e);
-  a.vec = vectors(rows->keys, {rows->row_stride, rows->head_stride}, e, lane) &&
-          aligned(rows->values, lane);
+  a.vec = vectors(rows->keys, {rows->row_stride, rows->head_stride}, e, 16) &&
+          aligned(rows->values, 16);
   a.err = err;
   const cudaError_t rc = fa::launch_paged_write(a, static_cast<cudaStream_t>(stream));
   if (rc != cudaSuccess) return cuda_fail(rc, "paged write launch");

@@ -14,7 +14,7 @@ namespace fa {
 
 namespace {
 
-constexpr int kRowWarps = 8;
+constexpr int kRowWarps = 4;
 
 // Row r's place: its page and slot, or false (with the error word set) if the batch's numbers are
 // out of range. Rows past the last sequence's are left alone. One warp; two trips to memory (three
@@ -112,66 +112,36 @@ __device__ __forceinline__ void store_elems(void* base, int64_t at, bool bf16, b
   }
 }
 
-// A head's row kept in its page: E elements a lane, quantised over the warp for 8-bit pages.
-template <int E>
-__device__ __forceinline__ void keep_head(const PagedPool& pool, bool is_key, int page, int kv,
-                                          int slot, int lane, const float (&x)[E]) {
-  const int64_t row = ((int64_t(page) * pool.kv_heads + kv) << pool.page_shift) + slot;
-  unsigned char* base = is_key ? pool.keys : pool.values;
-  if (!pool.q8) {
-    store_elems<E>(base, row * (32 * E) + lane * E, true, true, x);
-    return;
-  }
-  float top = 0.0f;
-  bool finite = true;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    top = fmaxf(top, fabsf(x[e]));
-    finite = finite && fabsf(x[e]) <= 3.402823466e38f;
-  }
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-  finite = __all_sync(0xffffffffu, finite);
-  const bool live = finite && top >= 7.888609052e-31f;  // 2^-100
-  const float inverse = live ? __fdiv_rn(127.0f, top) : 0.0f;
-  const float scale = !finite ? __int_as_float(0x7fffffff) : live ? __fdiv_rn(top, 127.0f) : 0.0f;
-  alignas(8) signed char q[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const float y = finite ? __fmul_rn(x[e], inverse) : 0.0f;
-    q[e] = static_cast<signed char>(max(-127, min(127, __float2int_rn(y))));
-  }
-  unsigned char* p = base + row * (32 * E) + lane * E;
-  if constexpr (E == 2) *reinterpret_cast<uint16_t*>(p) = *reinterpret_cast<uint16_t*>(q);
-  else if constexpr (E == 4) *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<uint32_t*>(q);
-  else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(q);
-  if (lane == 0) (is_key ? pool.key_scales : pool.value_scales)[row] = scale;
-}
-
-// One CTA per row; a warp takes every kRowWarps-th head unit (query heads, key heads, value
-// heads), U at a time so that their loads are in flight together, the first of them while the
-// row's place is looked up. Bound by memory: 10 thousand rows of 32/8 heads of 128 (bf16 rows, 8-bit
-// pages) move 231 MB. Lane l holds elements lE ..
-// lE + E - 1 of a head: RoPE by halves finds the partner of e in lane l ^ 16, interleaved RoPE
-// within the lane, and the row's cosines and sines are loaded once for all of the warp's heads.
-// Arithmetic of the rotation: each product rounded, then the difference or sum (ops.rs:77-95).
+// One CTA per row. A head's elements lie eight to a lane on D / 8 lanes, so that a warp takes 32 / (D
+// / 8) heads at a time (a step); it takes every kRowWarps-th step, U at a time so that their loads
+// are in flight together, the first of them while the row's place is looked up. RoPE by halves
+// finds the partner of an element half a head's lanes away, interleaved RoPE within the lane; the
+// row's cosines and sines are loaded once for all of a warp's heads. Every lane takes part in the
+// shuffles, whatever its head is (a step may hold heads of two kinds). Arithmetic of the rotation:
+// each product rounded, then the difference or sum (ops.rs:77-95).
+// Bound by memory, next by instructions: with four elements a lane, a head to a warp, 10 thousand
+// rows of 32/8 heads of 128 (bf16 rows, 8-bit pages, 231 MB) took 77 us.
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowWarps * 32)
     paged_write_kernel(const __grid_constant__ PagedWriteArgs a) {
-  constexpr int E = D / 32;
-  constexpr int U = D == 256 ? 4 : 6;
+  constexpr int E = 8, LH = D / E, HW = 32 / LH;  // lanes of a head, heads of a step
+  constexpr int U = D == 256 ? 4 : 3;
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sub = lane % LH;
   const int r = blockIdx.x;
   const int kvh = a.pool.kv_heads;
   const int units = a.heads + 2 * kvh;
   float xs[U][E];
+  auto skipped = [&](int u) { return u >= units || (u < a.heads && a.q_out == nullptr); };
   auto load = [&](int u0) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int u = u0 + i * kRowWarps;
-      if (u >= units || (u < a.heads && a.q_out == nullptr)) continue;
+      const int u = u0 + i * (kRowWarps * HW) + lane / LH;
+#pragma unroll
+      for (int e = 0; e < E; ++e) xs[i][e] = 0.0f;
+      if (skipped(u)) continue;
       const T* p;
       if (u < a.heads)
         p = static_cast<const T*>(a.q) + int64_t(r) * a.q_stride + int64_t(u) * D;
@@ -180,53 +150,56 @@ __global__ void __launch_bounds__(kRowWarps * 32)
       else
         p = static_cast<const T*>(a.v) + int64_t(r) * a.v_stride +
             int64_t(u - a.heads - kvh) * a.v_head_stride;
-      load_elems<T, E>(p + lane * E, a.vec != 0, xs[i]);
+      load_elems<T, E>(p + sub * E, a.vec != 0, xs[i]);
     }
   };
-  load(warp);
+  load(warp * HW);
   float c[E], s[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) c[e] = s[e] = 0.0f;
   if (a.rope == 1) {
-    const float* cs = a.angles + int64_t(r) * D + (lane & 15) * E;
+    const float* cs = a.angles + int64_t(r) * D + (sub % (LH / 2)) * E;
 #pragma unroll
     for (int e = 0; e < E; ++e) { c[e] = cs[e]; s[e] = cs[D / 2 + e]; }
   } else if (a.rope == 2) {
-    const float* cs = a.angles + int64_t(r) * D + lane * (E / 2);
+    const float* cs = a.angles + int64_t(r) * D + sub * (E / 2);
 #pragma unroll
     for (int e = 0; e < E / 2; ++e) { c[e] = cs[e]; s[e] = cs[D / 2 + e]; }
   }
   int page, slot;
   if (!place_of(a.spans, a.pool, r, lane, &page, &slot, a.err)) return;  // the warp's, as one
-  for (int u0 = warp; u0 < units; u0 += U * kRowWarps) {
-    if (u0 != warp) load(u0);
+  for (int u0 = warp * HW; u0 < units; u0 += U * kRowWarps * HW) {
+    if (u0 != warp * HW) load(u0);
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int u = u0 + i * kRowWarps;
-      if (u >= units || (u < a.heads && a.q_out == nullptr)) continue;
-      float(&x)[E] = xs[i];
+      const int step = u0 + i * (kRowWarps * HW);  // the step's first head
+      if (step >= units) break;
+      const int u = step + lane / LH;
+      const bool skip = skipped(u);
       const bool is_query = u < a.heads, is_key = !is_query && u < a.heads + kvh;
-      if (is_query || is_key) {
-        const float* weight = is_query ? a.q_norm : a.k_norm;
-        if (weight != nullptr) {
+      float(&x)[E] = xs[i];
+      if (step < a.heads + kvh) {  // (some head of the step is turned)
+        const float* weight = is_query ? a.q_norm : is_key ? a.k_norm : nullptr;
+        if (a.q_norm != nullptr || a.k_norm != nullptr) {
           float ss = 0.0f;
 #pragma unroll
           for (int e = 0; e < E; ++e) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
-          for (int off = 16; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-          const float inverse = 1.0f / sqrtf(ss / float(D) + a.eps);
+          for (int off = LH / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+          if (weight != nullptr) {
+            const float inverse = 1.0f / sqrtf(ss / float(D) + a.eps);
 #pragma unroll
-          for (int e = 0; e < E; ++e)
-            x[e] = __fmul_rn(__fmul_rn(x[e], inverse), weight[lane * E + e]);
+            for (int e = 0; e < E; ++e) x[e] = __fmul_rn(__fmul_rn(x[e], inverse), weight[sub * E + e]);
+          }
         }
         if (a.rope == 1) {
 #pragma unroll
           for (int e = 0; e < E; ++e) {
-            const float o = __shfl_xor_sync(0xffffffffu, x[e], 16);
+            const float o = __shfl_xor_sync(0xffffffffu, x[e], LH / 2);
             const float xc = __fmul_rn(x[e], c[e]), os = __fmul_rn(o, s[e]);
-            x[e] = lane < 16 ? __fsub_rn(xc, os) : __fadd_rn(xc, os);
+            if (is_query || is_key) x[e] = sub < LH / 2 ? __fsub_rn(xc, os) : __fadd_rn(xc, os);
           }
-        } else if (a.rope == 2) {
+        } else if (a.rope == 2 && (is_query || is_key)) {
 #pragma unroll
           for (int e = 0; e < E / 2; ++e) {
             const float y0 = x[2 * e], y1 = x[2 * e + 1];
@@ -235,11 +208,41 @@ __global__ void __launch_bounds__(kRowWarps * 32)
           }
         }
       }
-      if (is_query)
-        store_elems<E>(a.q_out, int64_t(r) * a.q_out_stride + int64_t(u) * D + lane * E,
+      if (is_query && !skip)
+        store_elems<E>(a.q_out, int64_t(r) * a.q_out_stride + int64_t(u) * D + sub * E,
                        a.q_out_bf16 != 0, a.q_out_vec != 0, x);
-      else
-        keep_head<E>(a.pool, is_key, page, is_key ? u - a.heads : u - a.heads - kvh, slot, lane, x);
+      if (step + HW <= a.heads) continue;  // all of the step's heads are queries
+      const int kv = is_key ? u - a.heads : u - a.heads - kvh;
+      const int64_t row = ((int64_t(page) * kvh + kv) << a.pool.page_shift) + slot;
+      unsigned char* base = is_key ? a.pool.keys : a.pool.values;
+      if (!a.pool.q8) {
+        if (!is_query && !skip) store_elems<E>(base, row * D + sub * E, true, true, x);
+        continue;
+      }
+      float top = 0.0f, total = 0.0f;  // (total: NaN if an element is not finite)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        top = fmaxf(top, fabsf(x[e]));
+        total = fmaf(x[e], 0.0f, total);
+      }
+#pragma unroll
+      for (int off = LH / 2; off >= 1; off >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        total += __shfl_xor_sync(0xffffffffu, total, off);
+      }
+      const bool finite = total == 0.0f;
+      const bool live = finite && top >= 7.888609052e-31f;  // 2^-100
+      const float inverse = live ? __fdiv_rn(127.0f, top) : 0.0f;
+      const float scale = !finite ? __int_as_float(0x7fffffff) : live ? __fdiv_rn(top, 127.0f) : 0.0f;
+      uint32_t w[2] = {0, 0};
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float y = finite ? __fmul_rn(x[e], inverse) : 0.0f;  // within +-127 but for a rounding
+        w[e / 4] |= uint32_t(max(-127, min(127, __float2int_rn(y))) & 0xff) << (8 * (e % 4));
+      }
+      if (is_query || skip) continue;
+      *reinterpret_cast<uint2*>(base + row * D + sub * E) = make_uint2(w[0], w[1]);
+      if (sub == 0) (is_key ? a.pool.key_scales : a.pool.value_scales)[row] = scale;
     }
   }
 }
