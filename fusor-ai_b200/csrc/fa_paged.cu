@@ -249,6 +249,7 @@ int write_input(const fa_paged_cache* c, int layer, const fa_paged_batch* b, int
   a.k_head_stride = a.v_head_stride = d;
   a.vec = vectors(qkv, {qkv_stride}, e, 16);
   a.angles = angles;
+  a.angles_vec = aligned(angles, 16);
   a.q_norm = norm ? norm->q_norm : nullptr;
   a.k_norm = norm ? norm->k_norm : nullptr;
   a.eps = norm ? norm->eps : 0.0f;

@@ -93,8 +93,9 @@ struct PagedWriteArgs {
   const void* k;         // row r, head h at k + r * k_stride + h * k_head_stride
   const void* v;
   int64_t q_stride, k_stride, k_head_stride, v_stride, v_head_stride;
-  int vec;               // every head's row starts on a boundary of its lanes' vectors
+  int vec;               // every head's row starts on a 16-byte boundary
   const float* angles;   // row r at angles + r * head_dim: cosines then sines
+  int angles_vec;        // 16-byte aligned
   const float* q_norm;
   const float* k_norm;
   float eps;

@@ -112,55 +112,59 @@ __device__ __forceinline__ void store_elems(void* base, int64_t at, bool bf16, b
   }
 }
 
+// Two words' low bytes, then two more's, as one word.
+__device__ __forceinline__ uint32_t pack_bytes(int a, int b, int c, int d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
 // One CTA per row. A head's elements lie eight to a lane on D / 8 lanes, so that a warp takes 32 / (D
-// / 8) heads at a time (a step); it takes every kRowWarps-th step, U at a time so that their loads
-// are in flight together, the first of them while the row's place is looked up. RoPE by halves
-// finds the partner of an element half a head's lanes away, interleaved RoPE within the lane; the
-// row's cosines and sines are loaded once for all of a warp's heads. Every lane takes part in the
-// shuffles, whatever its head is (a step may hold heads of two kinds). Arithmetic of the rotation:
-// each product rounded, then the difference or sum (ops.rs:77-95).
-// Bound by memory, next by instructions: with four elements a lane, a head to a warp, 10 thousand
-// rows of 32/8 heads of 128 (bf16 rows, 8-bit pages, 231 MB) took 77 us.
+// / 8) heads of one kind (queries, keys, values) at a time (a step); it takes every kRowWarps-th
+// step, the first one's loads issued before the row's place is looked up. RoPE by halves finds the partner of an element half a head's lanes away,
+// interleaved RoPE within the lane; the row's cosines and sines are loaded once for all of a warp's
+// heads. Arithmetic of the rotation: each product rounded, then the difference or sum
+// (ops.rs:77-95; x - y is x + (-y), so that a lane's sign goes into its sine once).
+// Bound by the latency of a row's loads, hidden by many warps: 10 thousand rows of 32/8 heads of 128
+// (bf16 rows, 8-bit pages, 231 MB) take 57 us with 48 warps an SM (40 registers), 76 us with two
+// or three steps' loads in flight and 28 warps.
 template <typename T, int D>
-__global__ void __launch_bounds__(kRowWarps * 32)
+__global__ void __launch_bounds__(kRowWarps * 32, 12)
     paged_write_kernel(const __grid_constant__ PagedWriteArgs a) {
   constexpr int E = 8, LH = D / E, HW = 32 / LH;  // lanes of a head, heads of a step
-  constexpr int U = D == 256 ? 4 : 3;
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int sub = lane % LH;
+  const int sub = lane % LH, which = lane / LH;
   const int r = blockIdx.x;
   const int kvh = a.pool.kv_heads;
-  const int units = a.heads + 2 * kvh;
-  float xs[U][E];
-  auto skipped = [&](int u) { return u >= units || (u < a.heads && a.q_out == nullptr); };
-  auto load = [&](int u0) {
+  const int q_steps = a.q_out == nullptr ? 0 : (a.heads + HW - 1) / HW, kv_steps = (kvh + HW - 1) / HW;
+  const int steps = q_steps + 2 * kv_steps;
+  const T* const q = static_cast<const T*>(a.q) + int64_t(r) * a.q_stride + sub * E;
+  const T* const k = static_cast<const T*>(a.k) + int64_t(r) * a.k_stride + sub * E;
+  const T* const v = static_cast<const T*>(a.v) + int64_t(r) * a.v_stride + sub * E;
+  // a step's kind (0 queries, 1 keys, 2 values) and this lane's head of it
+  auto kind_of = [&](int t) { return t < q_steps ? 0 : t < q_steps + kv_steps ? 1 : 2; };
+  auto head_of = [&](int t, int kind) {
+    return (kind == 0 ? t : kind == 1 ? t - q_steps : t - q_steps - kv_steps) * HW + which;
+  };
+  float x[E];
+  auto load = [&](int t) {
+    const int kind = kind_of(t), h = head_of(t, kind);
+    const T* p = kind == 0 ? q + h * D : kind == 1 ? k + h * a.k_head_stride : v + h * a.v_head_stride;
+    if (h < (kind == 0 ? a.heads : kvh)) {
+      load_elems<T, E>(p, a.vec != 0, x);
+    } else {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int u = u0 + i * (kRowWarps * HW) + lane / LH;
-#pragma unroll
-      for (int e = 0; e < E; ++e) xs[i][e] = 0.0f;
-      if (skipped(u)) continue;
-      const T* p;
-      if (u < a.heads)
-        p = static_cast<const T*>(a.q) + int64_t(r) * a.q_stride + int64_t(u) * D;
-      else if (u < a.heads + kvh)
-        p = static_cast<const T*>(a.k) + int64_t(r) * a.k_stride + int64_t(u - a.heads) * a.k_head_stride;
-      else
-        p = static_cast<const T*>(a.v) + int64_t(r) * a.v_stride +
-            int64_t(u - a.heads - kvh) * a.v_head_stride;
-      load_elems<T, E>(p + sub * E, a.vec != 0, xs[i]);
+      for (int e = 0; e < E; ++e) x[e] = 0.0f;
     }
   };
-  load(warp * HW);
+  if (warp < steps) load(warp);
   float c[E], s[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) c[e] = s[e] = 0.0f;
   if (a.rope == 1) {
     const float* cs = a.angles + int64_t(r) * D + (sub % (LH / 2)) * E;
+    load_elems<float, E>(cs, a.angles_vec != 0, c);
+    load_elems<float, E>(cs + D / 2, a.angles_vec != 0, s);
 #pragma unroll
-    for (int e = 0; e < E; ++e) { c[e] = cs[e]; s[e] = cs[D / 2 + e]; }
+    for (int e = 0; e < E; ++e) s[e] = sub < LH / 2 ? -s[e] : s[e];
   } else if (a.rope == 2) {
     const float* cs = a.angles + int64_t(r) * D + sub * (E / 2);
 #pragma unroll
@@ -168,82 +172,73 @@ __global__ void __launch_bounds__(kRowWarps * 32)
   }
   int page, slot;
   if (!place_of(a.spans, a.pool, r, lane, &page, &slot, a.err)) return;  // the warp's, as one
-  for (int u0 = warp * HW; u0 < units; u0 += U * kRowWarps * HW) {
-    if (u0 != warp * HW) load(u0);
+  for (int t = warp; t < steps; t += kRowWarps) {
+    if (t != warp) load(t);
+    const int kind = kind_of(t), h = head_of(t, kind);  // the kind is the warp's
+    const bool live = h < (kind == 0 ? a.heads : kvh);
+    if (kind < 2) {
+      const float* weight = kind == 0 ? a.q_norm : a.k_norm;
+      if (weight != nullptr) {
+        float ss = 0.0f;
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int step = u0 + i * (kRowWarps * HW);  // the step's first head
-      if (step >= units) break;
-      const int u = step + lane / LH;
-      const bool skip = skipped(u);
-      const bool is_query = u < a.heads, is_key = !is_query && u < a.heads + kvh;
-      float(&x)[E] = xs[i];
-      if (step < a.heads + kvh) {  // (some head of the step is turned)
-        const float* weight = is_query ? a.q_norm : is_key ? a.k_norm : nullptr;
-        if (a.q_norm != nullptr || a.k_norm != nullptr) {
-          float ss = 0.0f;
+        for (int e = 0; e < E; ++e) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
-          for (int e = 0; e < E; ++e) ss = fmaf(x[e], x[e], ss);
+        for (int off = LH / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+        const float inverse = 1.0f / sqrtf(ss / float(D) + a.eps);
 #pragma unroll
-          for (int off = LH / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-          if (weight != nullptr) {
-            const float inverse = 1.0f / sqrtf(ss / float(D) + a.eps);
+        for (int e = 0; e < E; ++e) x[e] = __fmul_rn(__fmul_rn(x[e], inverse), weight[sub * E + e]);
+      }
+      if (a.rope == 1) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = __fmul_rn(__fmul_rn(x[e], inverse), weight[sub * E + e]);
-          }
+        for (int e = 0; e < E; ++e) {
+          const float o = __shfl_xor_sync(0xffffffffu, x[e], LH / 2);
+          x[e] = __fadd_rn(__fmul_rn(x[e], c[e]), __fmul_rn(o, s[e]));
         }
-        if (a.rope == 1) {
+      } else if (a.rope == 2) {
 #pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const float o = __shfl_xor_sync(0xffffffffu, x[e], LH / 2);
-            const float xc = __fmul_rn(x[e], c[e]), os = __fmul_rn(o, s[e]);
-            if (is_query || is_key) x[e] = sub < LH / 2 ? __fsub_rn(xc, os) : __fadd_rn(xc, os);
-          }
-        } else if (a.rope == 2 && (is_query || is_key)) {
-#pragma unroll
-          for (int e = 0; e < E / 2; ++e) {
-            const float y0 = x[2 * e], y1 = x[2 * e + 1];
-            x[2 * e] = __fsub_rn(__fmul_rn(y0, c[e]), __fmul_rn(y1, s[e]));
-            x[2 * e + 1] = __fadd_rn(__fmul_rn(y1, c[e]), __fmul_rn(y0, s[e]));
-          }
+        for (int e = 0; e < E / 2; ++e) {
+          const float y0 = x[2 * e], y1 = x[2 * e + 1];
+          x[2 * e] = __fsub_rn(__fmul_rn(y0, c[e]), __fmul_rn(y1, s[e]));
+          x[2 * e + 1] = __fadd_rn(__fmul_rn(y1, c[e]), __fmul_rn(y0, s[e]));
         }
       }
-      if (is_query && !skip)
-        store_elems<E>(a.q_out, int64_t(r) * a.q_out_stride + int64_t(u) * D + sub * E,
-                       a.q_out_bf16 != 0, a.q_out_vec != 0, x);
-      if (step + HW <= a.heads) continue;  // all of the step's heads are queries
-      const int kv = is_key ? u - a.heads : u - a.heads - kvh;
-      const int64_t row = ((int64_t(page) * kvh + kv) << a.pool.page_shift) + slot;
-      unsigned char* base = is_key ? a.pool.keys : a.pool.values;
-      if (!a.pool.q8) {
-        if (!is_query && !skip) store_elems<E>(base, row * D + sub * E, true, true, x);
-        continue;
-      }
-      float top = 0.0f, total = 0.0f;  // (total: NaN if an element is not finite)
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        top = fmaxf(top, fabsf(x[e]));
-        total = fmaf(x[e], 0.0f, total);
-      }
-#pragma unroll
-      for (int off = LH / 2; off >= 1; off >>= 1) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        total += __shfl_xor_sync(0xffffffffu, total, off);
-      }
-      const bool finite = total == 0.0f;
-      const bool live = finite && top >= 7.888609052e-31f;  // 2^-100
-      const float inverse = live ? __fdiv_rn(127.0f, top) : 0.0f;
-      const float scale = !finite ? __int_as_float(0x7fffffff) : live ? __fdiv_rn(top, 127.0f) : 0.0f;
-      uint32_t w[2] = {0, 0};
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float y = finite ? __fmul_rn(x[e], inverse) : 0.0f;  // within +-127 but for a rounding
-        w[e / 4] |= uint32_t(max(-127, min(127, __float2int_rn(y))) & 0xff) << (8 * (e % 4));
-      }
-      if (is_query || skip) continue;
-      *reinterpret_cast<uint2*>(base + row * D + sub * E) = make_uint2(w[0], w[1]);
-      if (sub == 0) (is_key ? a.pool.key_scales : a.pool.value_scales)[row] = scale;
     }
+    if (kind == 0) {
+      if (live)
+        store_elems<E>(a.q_out, int64_t(r) * a.q_out_stride + h * D + sub * E, a.q_out_bf16 != 0,
+                       a.q_out_vec != 0, x);
+      continue;
+    }
+    const int64_t row = ((int64_t(page) * kvh + h) << a.pool.page_shift) + slot;
+    unsigned char* base = kind == 1 ? a.pool.keys : a.pool.values;
+    if (!a.pool.q8) {
+      if (live) store_elems<E>(base, row * D + sub * E, true, true, x);
+      continue;
+    }
+    float top = 0.0f, total = 0.0f;  // (total: NaN if an element is not finite)
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      top = fmaxf(top, fabsf(x[e]));
+      total = fmaf(x[e], 0.0f, total);
+    }
+#pragma unroll
+    for (int off = LH / 2; off >= 1; off >>= 1) {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      total += __shfl_xor_sync(0xffffffffu, total, off);
+    }
+    const bool finite = total == 0.0f;
+    const bool some = finite && top >= 7.888609052e-31f;  // 2^-100
+    const float inverse = some ? __fdiv_rn(127.0f, top) : 0.0f;
+    const float scale = !finite ? __int_as_float(0x7fffffff) : some ? __fdiv_rn(top, 127.0f) : 0.0f;
+    // x (127 / top) is within +-127 but for two roundings, and so rounds to -127 .. 127; what is
+    // not finite times 0 converts to 0
+    int n[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) n[e] = __float2int_rn(__fmul_rn(x[e], inverse));
+    if (!live) continue;
+    *reinterpret_cast<uint2*>(base + row * D + sub * E) =
+        make_uint2(pack_bytes(n[0], n[1], n[2], n[3]), pack_bytes(n[4], n[5], n[6], n[7]));
+    if (sub == 0) (kind == 1 ? a.pool.key_scales : a.pool.value_scales)[row] = scale;
   }
 }
 
