@@ -68,7 +68,7 @@ struct ChunkShape {
   static constexpr int kAt_Bars = kAt_V + kVStages * kTileBytes;
   static constexpr size_t kSmemBytes = size_t(kAt_Bars) + 512 + 1024 /* alignment */;
   static constexpr int kO = 128;  // TMEM column of O, after 128 keys' scores or two of 64 keys'
-  static_assert(kSmemBytes + 16 * 1024 <= 227 * 1024, "with the plan's static shared memory");
+  static_assert(kSmemBytes + 26 * 1024 <= 227 * 1024, "with the plan's static shared memory");
 };
 
 // One unit: rows q0 .. of sequence s, KV head h, and each query tile's key tiles.
@@ -140,19 +140,21 @@ struct ChunkPiece {
   int cost;        // the whole unit's tiles
 };
 
-// The next piece of the CTA's share, or false at its end.
+// The next piece of the CTA's share, or false at its end. spans: every sequence's row0, rows (0 if
+// none are this kernel's) and first position.
 template <int D, bool Q8>
-__device__ __forceinline__ bool chunk_next(const PagedAttendArgs& a, ChunkWalk* w, ChunkPiece* p) {
+__device__ __forceinline__ bool chunk_next(const PagedAttendArgs& a, const int3* spans, ChunkWalk* w,
+                                           ChunkPiece* p) {
   if (w->t >= w->t_end) return false;
-  PagedSpan sp;
   while (w->qt >= w->nq) {
     w->qt = 0;
     if (w->nq > 0 && ++w->h < a.pool.kv_heads) continue;
     w->h = 0;
     ++w->s;
-    w->nq = chunk_units<ChunkShape<D, Q8>::NQ>(a, w->s, &sp);
+    const int rows = ChunkShape<D, Q8>::NQ * chunk_rows(a);
+    w->nq = (spans[w->s].y + rows - 1) / rows;
   }
-  paged_span(a.spans, a.pool.page_shift, w->s, &sp);
+  const PagedSpan sp{spans[w->s].x, spans[w->s].y, spans[w->s].z};
   chunk_unit<D, Q8>(a, sp, w->qt, &p->u);
   p->h = w->h;
   p->cost = p->u.ue - p->u.ub;
@@ -188,6 +190,8 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
   // out of range, and 8-bit pages' 2^k, v and 2^-v
   __shared__ uint32_t absent[4];
   __shared__ float4 units[4];
+  __shared__ float q_down[Q8 ? NQ * 128 : 1];  // 8-bit pages: what a query row was scaled by, back
+  __shared__ int3 spans[kMaxPagedSequences];   // row0, rows (0: none of this kernel's), first position
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* sQ = smem;
@@ -241,7 +245,10 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
     for (int qt = lane; qt < units; qt += 32) sum += chunk_cost<D, Q8>(a, sp, qt);
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if (lane == 0) before[s] = sum;
+    if (lane == 0) {
+      before[s] = sum;
+      spans[s] = make_int3(sp.row0, units > 0 ? sp.n : 0, sp.first);
+    }
   }
   __syncthreads();
   {
@@ -274,8 +281,9 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
       if (before[mid] * kvh <= w.t) s0 = mid; else s1 = mid;
     }
     w.s = s0;
-    PagedSpan sp;
-    w.nq = chunk_units<NQ>(a, s0, &sp);
+    const PagedSpan sp{spans[s0].x, spans[s0].y, spans[s0].z};
+    const int unit_rows = NQ * chunk_rows(a);
+    w.nq = (sp.n + unit_rows - 1) / unit_rows;
     const int64_t per = before[s0 + 1] - before[s0];
     const int64_t rest = w.t - before[s0] * kvh;
     w.h = whole_times(rest, per);
@@ -314,7 +322,7 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
     auto next_piece = [&]() {
       __syncwarp();
       int more = 0;
-      if (lane == 0) more = chunk_next<D, Q8>(a, &walks[warp], &pieces[warp]);
+      if (lane == 0) more = chunk_next<D, Q8>(a, spans, &walks[warp], &pieces[warp]);
       return __shfl_sync(0xffffffffu, more, 0) != 0;
     };
     if (warp >= kMmaWarp) {
@@ -329,7 +337,7 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
         uint32_t pv[2][2] = {{0, 0}, {0, 0}};  // P.V products by block of a tile and query tile
         uint32_t sb = 0;                       // score products
         bool ok = true;
-        while (ok && chunk_next<D, Q8>(a, &walks[warp], &pieces[warp])) {
+        while (ok && chunk_next<D, Q8>(a, spans, &walks[warp], &pieces[warp])) {
           const int n_tiles = pc.end - pc.begin, n = n_tiles * S::kSubs;  // 64-key blocks
           const int at0 = pc.begin * S::kSubs;
           bool first[2] = {true, true};
@@ -677,64 +685,77 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
         const bool valid = pr < rows && r < pc.u.n;
         float scale = a.scale_log2;
         if (min(n, my_e) > max(0, my_b)) {
-          // the packed row's query, zeros for a row that is none; over 8-bit pages f16, scaled by
-          // a power of two, its elements in the converted keys' order
-          const int64_t at = int64_t(pc.u.row0 + r) * a.q_stride + int64_t(pc.h * a.group + ph) * D;
-          unsigned char* dst = sQ + i * S::kQBytes + p * 128;
-          auto load8 = [&](int c, float (&x)[8]) {
+          // The warp's 32 query rows, zeros for those that are none: a row on kCh lanes, eight loads
+          // of a lane in flight. Over 8-bit pages f16, a row scaled by a power of two to its
+          // range, its elements in the converted keys' order.
+          constexpr int kCh = D / 8, kRows = 32 / kCh, kBatch = 8;
+          const int ch = lane % kCh;
+#pragma unroll 1
+          for (int b = 0; b < kCh; b += kBatch) {
+            uint4 raw[kBatch][2];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-            if (!valid) return;
-            if (a.q_bf16) {
-              const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + at + c * 8;
-              if (a.q_vec) {
-                const uint4 w = *reinterpret_cast<const uint4*>(q);
-                x[0] = bf16_lo(w.x); x[1] = bf16_hi(w.x); x[2] = bf16_lo(w.y); x[3] = bf16_hi(w.y);
-                x[4] = bf16_lo(w.z); x[5] = bf16_hi(w.z); x[6] = bf16_lo(w.w); x[7] = bf16_hi(w.w);
+            for (int k = 0; k < kBatch; ++k) {
+              raw[k][0] = raw[k][1] = make_uint4(0, 0, 0, 0);
+              const int row = wq * 32 + (b + k) * kRows + lane / kCh;  // packed
+              const int rr = row / a.group, rh = row - rr * a.group;
+              if (rr >= rows || pc.u.q0 + i * rows + rr >= pc.u.n) continue;
+              const int64_t at = int64_t(pc.u.row0 + pc.u.q0 + i * rows + rr) * a.q_stride +
+                                 int64_t(pc.h * a.group + rh) * D + ch * 8;
+              if (a.q_bf16) {
+                const uint16_t* q = static_cast<const uint16_t*>(a.q) + at;
+                if (a.q_vec) raw[k][0] = *reinterpret_cast<const uint4*>(q);
+                else {
+                  raw[k][0].x = q[0] | uint32_t(q[1]) << 16; raw[k][0].y = q[2] | uint32_t(q[3]) << 16;
+                  raw[k][0].z = q[4] | uint32_t(q[5]) << 16; raw[k][0].w = q[6] | uint32_t(q[7]) << 16;
+                }
               } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = __bfloat162float(q[e]);
-              }
-            } else {
-              const float* q = static_cast<const float*>(a.q) + at + c * 8;
-              if (a.q_vec) {
-                const float4 u = reinterpret_cast<const float4*>(q)[0];
-                const float4 v = reinterpret_cast<const float4*>(q)[1];
-                x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-                x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
-              } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = q[e];
+                const uint32_t* q = static_cast<const uint32_t*>(a.q) + at;
+                if (a.q_vec) {
+                  raw[k][0] = reinterpret_cast<const uint4*>(q)[0];
+                  raw[k][1] = reinterpret_cast<const uint4*>(q)[1];
+                } else {
+                  raw[k][0] = make_uint4(q[0], q[1], q[2], q[3]);
+                  raw[k][1] = make_uint4(q[4], q[5], q[6], q[7]);
+                }
               }
             }
-          };
-          float up = 1.0f;
-          if constexpr (Q8) {
-            float top = 0.0f;
-#pragma unroll 4
-            for (int c = 0; c < D / 8; ++c) {
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+              const int row = wq * 32 + (b + k) * kRows + lane / kCh;
+              const uint4 u = raw[k][0], v = raw[k][1];
               float x[8];
-              load8(c, x);
+              if (a.q_bf16) {
+                x[0] = bf16_lo(u.x); x[1] = bf16_hi(u.x); x[2] = bf16_lo(u.y); x[3] = bf16_hi(u.y);
+                x[4] = bf16_lo(u.z); x[5] = bf16_hi(u.z); x[6] = bf16_lo(u.w); x[7] = bf16_hi(u.w);
+              } else {
+                x[0] = __uint_as_float(u.x); x[1] = __uint_as_float(u.y);
+                x[2] = __uint_as_float(u.z); x[3] = __uint_as_float(u.w);
+                x[4] = __uint_as_float(v.x); x[5] = __uint_as_float(v.y);
+                x[6] = __uint_as_float(v.z); x[7] = __uint_as_float(v.w);
+              }
+              uint4 w;
+              if constexpr (Q8) {
+                float top = 0.0f;
 #pragma unroll
-              for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+#pragma unroll
+                for (int off = kCh / 2; off >= 1; off >>= 1)
+                  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+                const int e = min(max(int(__float_as_uint(top) >> 23), 1), 253);
+                const float up = __uint_as_float(uint32_t(254 - e) << 23);
+                if (ch == 0) q_down[i * 128 + row] = __uint_as_float(uint32_t(e) << 23);
+                w = make_uint4(pack_f16(x[0] * up, x[2] * up), pack_f16(x[1] * up, x[3] * up),
+                               pack_f16(x[4] * up, x[6] * up), pack_f16(x[5] * up, x[7] * up));
+              } else {
+                w = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
+                               pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+              }
+              *reinterpret_cast<uint4*>(sQ + i * S::kQBytes + (ch / 8) * (BM * 128) + row * 128 +
+                                        (((ch % 8) ^ (row & 7)) * 16)) = w;
             }
-            const int e = min(max(int(__float_as_uint(top) >> 23), 1), 253);
-            up = __uint_as_float(uint32_t(254 - e) << 23);
-            scale *= __uint_as_float(uint32_t(e) << 23);
           }
-#pragma unroll 4
-          for (int c = 0; c < D / 8; ++c) {
-            float x[8];
-            load8(c, x);
-            uint4 w;
-            if constexpr (Q8)
-              w = make_uint4(pack_f16(x[0] * up, x[2] * up), pack_f16(x[1] * up, x[3] * up),
-                             pack_f16(x[4] * up, x[6] * up), pack_f16(x[5] * up, x[7] * up));
-            else
-              w = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
-                             pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
-            *reinterpret_cast<uint4*>(dst + (c / 8) * (BM * 128) + ((c % 8) ^ (p & 7)) * 16) = w;
-          }
+          __syncwarp();
+          if constexpr (Q8) scale *= q_down[i * 128 + p];
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           mbar_arrive(&q_full[i]);
         }
@@ -963,18 +984,29 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
 #pragma unroll
               for (int e = 0; e < 32; ++e) acc[e] = 0.0f;
 #pragma unroll 1
-              for (int x = c0; x <= c1; ++x) {
-                const float mx = __ldcg(a.part_ml + (slot_of(x) * 128 + p) * 2);
-                if (mx == -INFINITY) continue;  // no key of that piece is seen: its O is not there
-                const float f = exp2_approx(mx - mm);
-                const float* src = a.part_o + ((slot_of(x) * (D / 4) + cc * 8) * 128 + p) * 4;
+              for (int x = c0; x <= c1; x += 2) {  // two pieces' loads in flight
+                float4 v[2][8];
+                float f[2];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  const float4 v = __ldcg(reinterpret_cast<const float4*>(src + e * 512));
-                  acc[4 * e] = fmaf(f, v.x, acc[4 * e]);
-                  acc[4 * e + 1] = fmaf(f, v.y, acc[4 * e + 1]);
-                  acc[4 * e + 2] = fmaf(f, v.z, acc[4 * e + 2]);
-                  acc[4 * e + 3] = fmaf(f, v.w, acc[4 * e + 3]);
+                for (int y = 0; y < 2; ++y) {
+                  const int z = min(x + y, c1);
+                  const float mx = __ldcg(a.part_ml + (slot_of(z) * 128 + p) * 2);
+                  // (no key of that piece is seen: its O is not there)
+                  f[y] = mx == -INFINITY || x + y > c1 ? 0.0f : exp2_approx(mx - mm);
+                  const float* src = a.part_o + ((slot_of(z) * (D / 4) + cc * 8) * 128 + p) * 4;
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) v[y][e] = __ldcg(reinterpret_cast<const float4*>(src + e * 512));
+                }
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                  if (f[y] == 0.0f) continue;
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) {
+                    acc[4 * e] = fmaf(f[y], v[y][e].x, acc[4 * e]);
+                    acc[4 * e + 1] = fmaf(f[y], v[y][e].y, acc[4 * e + 1]);
+                    acc[4 * e + 2] = fmaf(f[y], v[y][e].z, acc[4 * e + 2]);
+                    acc[4 * e + 3] = fmaf(f[y], v[y][e].w, acc[4 * e + 3]);
+                  }
                 }
               }
               if (valid) write_out(cc, acc, inv);
