@@ -10,6 +10,7 @@
 
 #include "fa_attn.h"
 #include "fa_host.h"
+#include "fa_launch.cuh"
 #include "fa_paged.h"
 
 namespace {
@@ -152,7 +153,7 @@ bool vectors(const void* p, std::initializer_list<int64_t> strides, int elem, in
   return true;
 }
 
-// ---- the workspace: counters (zeroed by the caller), partials, then the rotated queries --------
+// ---- the workspace: counters (zeroed by the caller), partials, then a call's queries ------------
 
 struct Workspace {
   int64_t ml_at, o_at, q_at, bytes;
@@ -176,7 +177,7 @@ Workspace workspace_of(const fa_paged_cache* c, int rows, int max_rows, int sms)
   w.ml_at = FA_PAGED_COUNTER_BYTES;
   w.o_at = w.ml_at + up(ml * 4);
   w.q_at = w.o_at + up(o * 4);
-  w.bytes = w.q_at + up(int64_t(rows) * c->heads * c->head_dim * 2);
+  w.bytes = w.q_at + up(int64_t(rows) * c->heads * c->head_dim * 4);
   return w;
 }
 
@@ -272,11 +273,11 @@ int attend(const fa_paged_cache* c, int layer, const fa_paged_batch* b, const vo
   a.spans = spans_of(b);
   a.heads = c->heads;
   a.group = c->heads / c->kv_heads;
+  a.tile_rows = 128 / a.group;
   a.kind = b->mask;
   a.window = b->window;
   a.token_cols = fa::kPagedTokenCols;
   a.q_bf16 = dtype == FA_BF16;
-  a.q_vec = vectors(q, {q_stride}, a.q_bf16 ? 2 : 4, 16);
   a.out_bf16 = out_dtype == FA_BF16;
   a.out_vec = vectors(out, {out_stride}, a.out_bf16 ? 2 : 4, 16);
   a.q = q;
@@ -289,6 +290,16 @@ int attend(const fa_paged_cache* c, int layer, const fa_paged_batch* b, const vo
   a.part_o = reinterpret_cast<float*>(base + w.o_at);
   a.counters = reinterpret_cast<int*>(base);
   a.err = err;
+  if (!vectors(q, {q_stride}, a.q_bf16 ? 2 : 4, 16)) {
+    // rows that 16-byte loads do not fit are copied (in f32, exactly) to where they do
+    float* rows = reinterpret_cast<float*>(base + w.q_at);
+    const cudaError_t rc = fa::launch_prepare_queries(dtype == FA_BF16 ? fa::kKtBf16 : fa::kKtF32, q, q_stride,
+                                                      0, b->rows, c->heads, c->head_dim, 1.0f, rows, s);
+    if (rc != cudaSuccess) return cuda_fail(rc, "query copy launch");
+    a.q = rows;
+    a.q_stride = int64_t(c->heads) * c->head_dim;
+    a.q_bf16 = 0;
+  }
   // A batch may hold both kinds of sequences: each kernel leaves the other's alone. Where the
   // rows are as many as sequences of max_rows each make (a uniform batch, a single sequence) the
   // chunk kernel takes every sequence, and where no sequence has many rows the token kernel does:
@@ -504,12 +515,14 @@ int fa_attention_paged(const fa_paged_cache* cache, int32_t layer, const fa_page
   if (batch->sequences == 0 || batch->rows == 0) return FA_OK;
   OnDevice on(cache->device);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // the rotated queries are kept in bf16, as the tensor cores take them
+  // the rotated queries stay f32 over 8-bit pages, whose products round them to no less than f16;
+  // over bf16 pages they are kept in bf16, as the tensor cores take them
   void* q = static_cast<unsigned char*>(batch->workspace) + w.q_at;
   const int64_t width = int64_t(cache->heads) * cache->head_dim;
+  const int q_dtype = cache->dtype == FA_Q8 ? FA_F32 : FA_BF16;
   FA_TRY(write_input(cache, layer, batch, rope, angles, norm, qkv, qkv_stride, dtype, q, width,
-                     FA_BF16, err, s));
-  return attend(cache, layer, batch, q, width, FA_BF16, out, out_stride, out_dtype, w, sms, err, s);
+                     q_dtype, err, s));
+  return attend(cache, layer, batch, q, width, q_dtype, out, out_stride, out_dtype, w, sms, err, s);
 }
 
 }  // extern "C"

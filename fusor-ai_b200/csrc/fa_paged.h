@@ -131,8 +131,9 @@ struct PagedAttendArgs {
   int kind, window;      // mask: 0 causal, 1 window, 2 full
   int token_cols;        // packed rows up to which a sequence runs on the token kernel
   int merge_cols;        // token kernel: the most packed rows that a sequence of it can have
-  int q_bf16, q_vec, out_bf16, out_vec;
-  const void* q;         // row r, head h at q + r * q_stride + h * head_dim
+  int tile_rows;         // rows of a chunk's query tile: 128 / group
+  int q_bf16, out_bf16, out_vec;
+  const void* q;         // row r, head h at q + r * q_stride + h * head_dim; 16-byte aligned rows
   int64_t q_stride;
   void* out;
   int64_t out_stride;

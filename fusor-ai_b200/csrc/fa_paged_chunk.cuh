@@ -80,13 +80,15 @@ struct ChunkUnit {
 };
 
 struct ChunkWalk {
+  int64_t share;     // tiles of a CTA
   int64_t t, t_end;  // global tiles: the next piece's first, the share's end
   int64_t unit0;     // the unit's first global tile
   int s, h, qt, nq;  // sequence, KV head, unit of the sequence, units of the sequence
+  int cta;
 };
 
 // Rows of a query tile.
-__device__ __forceinline__ int chunk_rows(const PagedAttendArgs& a) { return 128 / a.group; }
+__device__ __forceinline__ int chunk_rows(const PagedAttendArgs& a) { return a.tile_rows; }
 
 // Units of sequence s (0 if it is empty, out of range or the token kernel's; -1 out of range).
 template <int NQ>
@@ -126,7 +128,7 @@ __device__ __forceinline__ void chunk_unit(const PagedAttendArgs& a, const Paged
 
 // Tiles of a whole unit.
 template <int D, bool Q8>
-__device__ __forceinline__ int chunk_cost(const PagedAttendArgs& a, const PagedSpan& sp, int qt) {
+__device__ __noinline__ int chunk_cost(const PagedAttendArgs& a, const PagedSpan& sp, int qt) {
   ChunkUnit u;
   chunk_unit<D, Q8>(a, sp, qt, &u);
   return u.ue - u.ub;
@@ -136,8 +138,7 @@ struct ChunkPiece {
   ChunkUnit u;
   int h;
   int begin, end;  // key tiles of this piece
-  int64_t unit0;
-  int cost;        // the whole unit's tiles
+  int c0, c1;      // the first and last CTA that the unit is shared among
 };
 
 // The next piece of the CTA's share, or false at its end. spans: every sequence's row0, rows (0 if
@@ -157,14 +158,109 @@ __device__ __forceinline__ bool chunk_next(const PagedAttendArgs& a, const int3*
   const PagedSpan sp{spans[w->s].x, spans[w->s].y, spans[w->s].z};
   chunk_unit<D, Q8>(a, sp, w->qt, &p->u);
   p->h = w->h;
-  p->cost = p->u.ue - p->u.ub;
-  p->unit0 = w->unit0;
+  const int cost = p->u.ue - p->u.ub;
+  share_owners(w->share, w->cta, w->unit0, cost, &p->c0, &p->c1);
   p->begin = p->u.ub + int(w->t - w->unit0);
   p->end = int(min(int64_t(p->u.ue), p->begin + (w->t_end - w->t)));
   w->t += p->end - p->begin;
-  w->unit0 += p->cost;
+  w->unit0 += cost;
   ++w->qt;
   return true;
+}
+
+// A warp's 32 query rows of query tile i (packed rows 32 wq ..) into the swizzled tile at dst, zeros
+// for those that are none: a row on D / 8 lanes, 8 or 16 loads of a lane in flight. Over 8-bit pages
+// f16, a row scaled by a power of two to its range (and back by down[row]), its elements in the
+// converted keys' order.
+template <int D, bool Q8, bool BF16>
+__device__ __forceinline__ void chunk_queries(const PagedAttendArgs& a, const ChunkPiece& pc, int i, int wq,
+                                           unsigned char* dst, float* down) {
+  constexpr int kCh = D / 8, kRows = 32 / kCh;
+  constexpr int kBatch = BF16 && !Q8 && kCh >= 16 ? 16 : 8, kVecs = BF16 ? 1 : 2;
+  const int lane = threadIdx.x & 31, ch = lane % kCh;
+  const int rows = chunk_rows(a), left = min(rows, pc.u.n - pc.u.q0 - i * rows);
+  const uint32_t magic = (65536 + a.group - 1) / a.group;  // row / group for rows below 128
+  const int64_t base = int64_t(pc.u.row0 + pc.u.q0 + i * rows) * a.q_stride +
+                       int64_t(pc.h * a.group) * D + ch * 8;
+  constexpr int kBytes = BF16 ? 2 : 4;
+#pragma unroll 1
+  for (int b = 0; b < kCh; b += kBatch) {
+    uint4 raw[kBatch][kVecs];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+#pragma unroll
+      for (int y = 0; y < kVecs; ++y) raw[k][y] = make_uint4(0, 0, 0, 0);
+      const int row = wq * 32 + (b + k) * kRows + lane / kCh;  // packed
+      const int rr = int(row * magic >> 16), rh = row - rr * a.group;
+      if (rr >= left) continue;
+      const unsigned char* q = static_cast<const unsigned char*>(a.q) + (base + rr * a.q_stride + rh * D) * kBytes;
+#pragma unroll
+      for (int y = 0; y < kVecs; ++y) raw[k][y] = *reinterpret_cast<const uint4*>(q + 16 * y);
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int row = wq * 32 + (b + k) * kRows + lane / kCh;
+      const uint4 u = raw[k][0], v = raw[k][kVecs - 1];
+      uint4 w = u;
+      if constexpr (Q8 || !BF16) {
+        float x[8];
+        if constexpr (BF16) {
+          x[0] = bf16_lo(u.x); x[1] = bf16_hi(u.x); x[2] = bf16_lo(u.y); x[3] = bf16_hi(u.y);
+          x[4] = bf16_lo(u.z); x[5] = bf16_hi(u.z); x[6] = bf16_lo(u.w); x[7] = bf16_hi(u.w);
+        } else {
+          x[0] = __uint_as_float(u.x); x[1] = __uint_as_float(u.y);
+          x[2] = __uint_as_float(u.z); x[3] = __uint_as_float(u.w);
+          x[4] = __uint_as_float(v.x); x[5] = __uint_as_float(v.y);
+          x[6] = __uint_as_float(v.z); x[7] = __uint_as_float(v.w);
+        }
+        if constexpr (Q8) {
+          float top = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+#pragma unroll
+          for (int off = kCh / 2; off >= 1; off >>= 1)
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          const int e = min(max(int(__float_as_uint(top) >> 23), 1), 253);
+          const float up = __uint_as_float(uint32_t(254 - e) << 23);
+          if (ch == 0) down[row] = __uint_as_float(uint32_t(e) << 23);
+          w = make_uint4(pack_f16(x[0] * up, x[2] * up), pack_f16(x[1] * up, x[3] * up),
+                         pack_f16(x[4] * up, x[6] * up), pack_f16(x[5] * up, x[7] * up));
+        } else {
+          w = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
+                         pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+        }
+      }
+      *reinterpret_cast<uint4*>(dst + (ch / 8) * (128 * 128) + row * 128 + (((ch % 8) ^ (row & 7)) * 16)) = w;
+    }
+  }
+}
+
+// 32 elements of a packed row's output, from element `at` of `out` on.
+__device__ __forceinline__ void chunk_write(void* out, int64_t at, int bf16, int vec, const float (&x)[32]) {
+  if (bf16) {
+    uint16_t* dst = static_cast<uint16_t*>(out) + at;
+    uint32_t w[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) w[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
+    if (vec) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        reinterpret_cast<uint4*>(dst)[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) dst[e] = uint16_t(w[e / 2] >> (16 * (e & 1)));
+    }
+  } else {
+    float* dst = static_cast<float*>(out) + at;
+    if (vec) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        reinterpret_cast<float4*>(dst)[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) dst[e] = x[e];
+    }
+  }
 }
 
 template <int D, bool Q8>
@@ -268,13 +364,15 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
   __syncthreads();
   const int64_t work = before[nseq] * kvh;
   // at least two tiles a CTA: a piece's partials cost about as much as a tile
-  const int ctas = int(min(int64_t(gridDim.x), (work + 1) / 2));
+  const int64_t share = share_size(work, int(min(int64_t(gridDim.x), (work + 1) / 2)) + (work == 0));
   const int cta = blockIdx.x;
-  const bool idle = cta >= ctas;
+  const bool idle = share * cta >= work;
   if (!idle && warp == 0) {
     ChunkWalk w;
-    w.t = share_begin(work, cta, ctas);
-    w.t_end = share_begin(work, cta + 1, ctas);
+    w.share = share;
+    w.cta = cta;
+    w.t = share * cta;
+    w.t_end = min(work, w.t + share);
     int s0 = 0, s1 = nseq;  // the last s with before[s] * kvh <= t
     while (s1 - s0 > 1) {
       const int mid = (s0 + s1) / 2;
@@ -502,7 +600,7 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
             const int st = stage_of();
             if (!vacant(st, phase_of())) { ok = false; break; }
             const uint32_t dst = smem_u32(tiles) + st * S::kTileBytes + (chunk / 8) * (BN * 128);
-#pragma unroll
+#pragma unroll 2
             for (int gr = 0; gr < kGroups; ++gr) {
               const int pg = __shfl_sync(0xffffffffu, page, gr), p0 = pos + gr * 16;
               const int64_t row0 = ((int64_t(max(pg, 0)) * kvh + pc.h) << shift) + (p0 & ((1 << shift) - 1));
@@ -685,75 +783,9 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
         const bool valid = pr < rows && r < pc.u.n;
         float scale = a.scale_log2;
         if (min(n, my_e) > max(0, my_b)) {
-          // The warp's 32 query rows, zeros for those that are none: a row on kCh lanes, eight loads
-          // of a lane in flight. Over 8-bit pages f16, a row scaled by a power of two to its
-          // range, its elements in the converted keys' order.
-          constexpr int kCh = D / 8, kRows = 32 / kCh, kBatch = 8;
-          const int ch = lane % kCh;
-#pragma unroll 1
-          for (int b = 0; b < kCh; b += kBatch) {
-            uint4 raw[kBatch][2];
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-              raw[k][0] = raw[k][1] = make_uint4(0, 0, 0, 0);
-              const int row = wq * 32 + (b + k) * kRows + lane / kCh;  // packed
-              const int rr = row / a.group, rh = row - rr * a.group;
-              if (rr >= rows || pc.u.q0 + i * rows + rr >= pc.u.n) continue;
-              const int64_t at = int64_t(pc.u.row0 + pc.u.q0 + i * rows + rr) * a.q_stride +
-                                 int64_t(pc.h * a.group + rh) * D + ch * 8;
-              if (a.q_bf16) {
-                const uint16_t* q = static_cast<const uint16_t*>(a.q) + at;
-                if (a.q_vec) raw[k][0] = *reinterpret_cast<const uint4*>(q);
-                else {
-                  raw[k][0].x = q[0] | uint32_t(q[1]) << 16; raw[k][0].y = q[2] | uint32_t(q[3]) << 16;
-                  raw[k][0].z = q[4] | uint32_t(q[5]) << 16; raw[k][0].w = q[6] | uint32_t(q[7]) << 16;
-                }
-              } else {
-                const uint32_t* q = static_cast<const uint32_t*>(a.q) + at;
-                if (a.q_vec) {
-                  raw[k][0] = reinterpret_cast<const uint4*>(q)[0];
-                  raw[k][1] = reinterpret_cast<const uint4*>(q)[1];
-                } else {
-                  raw[k][0] = make_uint4(q[0], q[1], q[2], q[3]);
-                  raw[k][1] = make_uint4(q[4], q[5], q[6], q[7]);
-                }
-              }
-            }
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-              const int row = wq * 32 + (b + k) * kRows + lane / kCh;
-              const uint4 u = raw[k][0], v = raw[k][1];
-              float x[8];
-              if (a.q_bf16) {
-                x[0] = bf16_lo(u.x); x[1] = bf16_hi(u.x); x[2] = bf16_lo(u.y); x[3] = bf16_hi(u.y);
-                x[4] = bf16_lo(u.z); x[5] = bf16_hi(u.z); x[6] = bf16_lo(u.w); x[7] = bf16_hi(u.w);
-              } else {
-                x[0] = __uint_as_float(u.x); x[1] = __uint_as_float(u.y);
-                x[2] = __uint_as_float(u.z); x[3] = __uint_as_float(u.w);
-                x[4] = __uint_as_float(v.x); x[5] = __uint_as_float(v.y);
-                x[6] = __uint_as_float(v.z); x[7] = __uint_as_float(v.w);
-              }
-              uint4 w;
-              if constexpr (Q8) {
-                float top = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
-#pragma unroll
-                for (int off = kCh / 2; off >= 1; off >>= 1)
-                  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-                const int e = min(max(int(__float_as_uint(top) >> 23), 1), 253);
-                const float up = __uint_as_float(uint32_t(254 - e) << 23);
-                if (ch == 0) q_down[i * 128 + row] = __uint_as_float(uint32_t(e) << 23);
-                w = make_uint4(pack_f16(x[0] * up, x[2] * up), pack_f16(x[1] * up, x[3] * up),
-                               pack_f16(x[4] * up, x[6] * up), pack_f16(x[5] * up, x[7] * up));
-              } else {
-                w = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
-                               pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
-              }
-              *reinterpret_cast<uint4*>(sQ + i * S::kQBytes + (ch / 8) * (BM * 128) + row * 128 +
-                                        (((ch % 8) ^ (row & 7)) * 16)) = w;
-            }
-          }
+          unsigned char* dst = sQ + i * S::kQBytes;
+          if (a.q_bf16) chunk_queries<D, Q8, true>(a, pc, i, wq, dst, q_down + (Q8 ? i * 128 : 0));
+          else chunk_queries<D, Q8, false>(a, pc, i, wq, dst, q_down + (Q8 ? i * 128 : 0));
           __syncwarp();
           if constexpr (Q8) scale *= q_down[i * 128 + p];
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -806,11 +838,16 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
           tc::tmem_ld64_wait(s_base, sreg);
           float* s = reinterpret_cast<float*>(sreg);
           const bool all_in = !valid || (kp >= runs.b0 && kp + 64 <= runs.b0 + runs.n0);
-          if (!all_in) mask_scores<64>(runs, kp, s);
-          if (gone != 0) {
+          if (!all_in || gone != 0) {
 #pragma unroll
-            for (int x = 0; x < 64; ++x)
-              if ((gone >> (h * 4 + (x >> 4))) & 1u) s[x] = -INFINITY;
+            for (int w = 0; w < 2; ++w) {
+              const uint32_t off = gone >> (h * 4 + w * 2);
+              const uint32_t bits = run_word(runs.b0, runs.n0, kp, w) &
+                                    ~((off & 1u ? 0xFFFFu : 0u) | (off & 2u ? 0xFFFF0000u : 0u));
+#pragma unroll
+              for (int x = 0; x < 32; ++x)
+                if (!((bits >> x) & 1u)) s[32 * w + x] = -INFINITY;
+            }
           }
           float mx0 = s[0], mx1 = s[1], mx2 = s[2], mx3 = s[3];
 #pragma unroll
@@ -884,76 +921,67 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
           tc::fence_after_sync();
         }
         if (poisoned) l_sum = __int_as_float(0x7fffffff);
-        const int c0 = share_owner(work, pc.unit0, ctas);
-        const int c1 = share_owner(work, pc.unit0 + pc.cost - 1, ctas);
+        const int c0 = pc.c0, c1 = pc.c1;
         const int64_t orow = int64_t(pc.u.row0 + r) * a.out_stride + int64_t(pc.h * a.group + ph) * D;
-        // 32 columns of O in the elements' order
-        auto order = [&](uint32_t (&o)[32]) {
-          if constexpr (Q8) {
-#pragma unroll
-            for (int x = 0; x < 32; x += 4) {
-              const uint32_t y = o[x + 1];
-              o[x + 1] = o[x + 2];
-              o[x + 2] = y;
-            }
-          }
-        };
-        auto write_out = [&](int cc, const float (&x)[32], float inv) {
-          if (a.out_bf16) {
-            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + orow + cc * 32;
-            if (a.out_vec) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                reinterpret_cast<uint4*>(dst)[e] =
-                    make_uint4(pack_bf16x2(x[8 * e] * inv, x[8 * e + 1] * inv),
-                               pack_bf16x2(x[8 * e + 2] * inv, x[8 * e + 3] * inv),
-                               pack_bf16x2(x[8 * e + 4] * inv, x[8 * e + 5] * inv),
-                               pack_bf16x2(x[8 * e + 6] * inv, x[8 * e + 7] * inv));
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) dst[e] = __float2bfloat16_rn(x[e] * inv);
-            }
-          } else {
-            float* dst = static_cast<float*>(a.out) + orow + cc * 32;
-            if (a.out_vec) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                reinterpret_cast<float4*>(dst)[e] = make_float4(
-                    x[4 * e] * inv, x[4 * e + 1] * inv, x[4 * e + 2] * inv, x[4 * e + 3] * inv);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) dst[e] = x[e] * inv;
-            }
-          }
-        };
-        if (c0 == c1) {
+        // O to the output, or (a piece of a unit) to the partials; then, by the last piece to
+        // arrive, the partials merged to the output: one loop over O's columns for all three.
+        // Partials lie by float4s of 128 packed rows (a warp's stores are contiguous).
+        auto slot_of = [&](int x) { return int64_t(2 * x + (x == c0 ? 1 : 0)) * NQ + i; };
+        const int64_t slot = slot_of(cta);
+        int mode = c0 == c1 ? 0 : 1;  // 2: merge
+        float mm = -INFINITY;
+        for (;;) {
           const float inv = l_sum == 0.0f ? 0.0f : 1.0f / l_sum;
 #pragma unroll 1
           for (int cc = 0; cc < D / 32; ++cc) {
             uint32_t o[32];
-            if (have) tc::tmem_ld32_wait(o_base + cc * 32, o);
-            else {
+            float* x = reinterpret_cast<float*>(o);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = 0;
-            }
-            order(o);
-            if (valid) write_out(cc, *reinterpret_cast<const float(*)[32]>(&o), inv);
-          }
-        } else {
-          // a piece: partials by float4s of 128 packed rows (a warp's stores are contiguous)
-          const int64_t slot = (int64_t(2 * cta + (cta == c0 ? 1 : 0)) * NQ + i);
-          if (have) {
-#pragma unroll 1
-            for (int cc = 0; cc < D / 32; ++cc) {
-              uint32_t o[32];
+            for (int e = 0; e < 32; ++e) o[e] = 0;
+            if (mode < 2) {
+              if (!have) break;
               tc::tmem_ld32_wait(o_base + cc * 32, o);
-              order(o);
+              if constexpr (Q8) {
+                // the elements' order
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                  const uint32_t y = o[e + 1];
+                  o[e + 1] = o[e + 2];
+                  o[e + 2] = y;
+                }
+              }
+            } else {
+#pragma unroll 1
+              for (int z = c0; z <= c1; ++z) {
+                const float mx = __ldcg(a.part_ml + (slot_of(z) * 128 + p) * 2);
+                const float* src = a.part_o + ((slot_of(z) * (D / 4) + cc * 8) * 128 + p) * 4;
+                float4 v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = __ldcg(reinterpret_cast<const float4*>(src + e * 512));
+                // (no key of that piece is seen: its O is not there)
+                if (mx == -INFINITY) continue;
+                const float f = exp2_approx(mx - mm);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  x[4 * e] = fmaf(f, v[e].x, x[4 * e]);
+                  x[4 * e + 1] = fmaf(f, v[e].y, x[4 * e + 1]);
+                  x[4 * e + 2] = fmaf(f, v[e].z, x[4 * e + 2]);
+                  x[4 * e + 3] = fmaf(f, v[e].w, x[4 * e + 3]);
+                }
+              }
+            }
+            if (mode == 1) {
 #pragma unroll
               for (int e = 0; e < 8; ++e)
                 *reinterpret_cast<uint4*>(a.part_o + ((slot * (D / 4) + cc * 8 + e) * 128 + p) * 4) =
                     make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            } else if (valid) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[e] *= inv;
+              chunk_write(a.out, orow + cc * 32, a.out_bf16, a.out_vec, *reinterpret_cast<const float(*)[32]>(x));
             }
           }
+          if (mode != 1) break;
           *reinterpret_cast<float2*>(a.part_ml + (slot * 128 + p) * 2) =
               make_float2(have ? m_used : -INFINITY, l_sum);
           // each warp's rows count their pieces on their own counter: no barrier among the warps
@@ -965,53 +993,17 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
             last = atomicAdd(counter, 1) == c1 - c0;
             if (last) *counter = 0;
           }
-          if (__shfl_sync(0xffffffffu, last, 0) != 0) {
-            __threadfence();
-            auto slot_of = [&](int x) { return int64_t(2 * x + (x == c0 ? 1 : 0)) * NQ + i; };
-            float mm = -INFINITY, ll = 0.0f;
+          if (__shfl_sync(0xffffffffu, last, 0) == 0) break;
+          __threadfence();
+          l_sum = 0.0f;
 #pragma unroll 4
-            for (int x = c0; x <= c1; ++x)
-              mm = fmaxf(mm, __ldcg(a.part_ml + (slot_of(x) * 128 + p) * 2));
+          for (int z = c0; z <= c1; ++z) mm = fmaxf(mm, __ldcg(a.part_ml + (slot_of(z) * 128 + p) * 2));
 #pragma unroll 4
-            for (int x = c0; x <= c1; ++x) {
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml + (slot_of(x) * 128 + p) * 2));
-              ll += ml.x == -INFINITY ? ml.y : ml.y * exp2_approx(ml.x - mm);
-            }
-            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-#pragma unroll 1
-            for (int cc = 0; cc < D / 32; ++cc) {
-              float acc[32];
-#pragma unroll
-              for (int e = 0; e < 32; ++e) acc[e] = 0.0f;
-#pragma unroll 1
-              for (int x = c0; x <= c1; x += 2) {  // two pieces' loads in flight
-                float4 v[2][8];
-                float f[2];
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                  const int z = min(x + y, c1);
-                  const float mx = __ldcg(a.part_ml + (slot_of(z) * 128 + p) * 2);
-                  // (no key of that piece is seen: its O is not there)
-                  f[y] = mx == -INFINITY || x + y > c1 ? 0.0f : exp2_approx(mx - mm);
-                  const float* src = a.part_o + ((slot_of(z) * (D / 4) + cc * 8) * 128 + p) * 4;
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) v[y][e] = __ldcg(reinterpret_cast<const float4*>(src + e * 512));
-                }
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                  if (f[y] == 0.0f) continue;
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) {
-                    acc[4 * e] = fmaf(f[y], v[y][e].x, acc[4 * e]);
-                    acc[4 * e + 1] = fmaf(f[y], v[y][e].y, acc[4 * e + 1]);
-                    acc[4 * e + 2] = fmaf(f[y], v[y][e].z, acc[4 * e + 2]);
-                    acc[4 * e + 3] = fmaf(f[y], v[y][e].w, acc[4 * e + 3]);
-                  }
-                }
-              }
-              if (valid) write_out(cc, acc, inv);
-            }
+          for (int z = c0; z <= c1; ++z) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml + (slot_of(z) * 128 + p) * 2));
+            l_sum += ml.x == -INFINITY ? ml.y : ml.y * exp2_approx(ml.x - mm);
           }
+          mode = 2;
         }
         tc::fence_before_sync();
       }

@@ -340,13 +340,13 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
   const TokPlan plan{before, spans, kvh};
   const int64_t work = before[nseq] * kvh;
   if (work == 0) return;
-  const int ctas = int(min(int64_t(gridDim.x), work));  // a tile each at least
+  const int64_t share = share_size(work, int(min(int64_t(gridDim.x), work)));  // a tile at least
   const int cta = blockIdx.x;
-  if (cta >= ctas) return;
+  if (share * cta >= work) return;
 
   TokWalk lw, cw;  // the loads' walk and the products' walk
-  lw.t = cw.t = share_begin(work, cta, ctas);
-  lw.t_end = cw.t_end = share_begin(work, cta + 1, ctas);
+  lw.t = cw.t = share * cta;
+  lw.t_end = cw.t_end = min(work, share * (cta + 1));
   {
     int s0 = 0, s1 = nseq;  // the last s with before[s] * kvh <= t
     while (s1 - s0 > 1) {
@@ -450,23 +450,11 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
           y[0] = y[1] = y[2] = y[3] = 0.0f;
           if (!valid) continue;
           if (a.q_bf16) {
-            const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q) + e0 + 4 * j;
-            if (a.q_vec) {
-              const uint2 w = *reinterpret_cast<const uint2*>(p);
-              y[0] = bf16_lo(w.x); y[1] = bf16_hi(w.x); y[2] = bf16_lo(w.y); y[3] = bf16_hi(w.y);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) y[e] = __bfloat162float(p[e]);
-            }
+            const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.q) + e0 + 4 * j);
+            y[0] = bf16_lo(w.x); y[1] = bf16_hi(w.x); y[2] = bf16_lo(w.y); y[3] = bf16_hi(w.y);
           } else {
-            const float* p = static_cast<const float*>(a.q) + e0 + 4 * j;
-            if (a.q_vec) {
-              const float4 w = *reinterpret_cast<const float4*>(p);
-              y[0] = w.x; y[1] = w.y; y[2] = w.z; y[3] = w.w;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) y[e] = p[e];
-            }
+            const float4 w = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + e0 + 4 * j);
+            y[0] = w.x; y[1] = w.y; y[2] = w.z; y[3] = w.w;
           }
         }
       }
@@ -838,8 +826,8 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
       }
     __syncthreads();
     const int64_t unit0 = plan.before[cw.s] * kvh + int64_t(cw.h) * cw.tiles;  // its first tile
-    const int c0 = share_owner(work, unit0, ctas);
-    const int c1 = share_owner(work, unit0 + cw.tiles - 1, ctas);
+    int c0, c1;
+    share_owners(share, cta, unit0, cw.tiles, &c0, &c1);
     const int pieces = c1 - c0 + 1;
     const int cols = cw.n * a.group;
     constexpr int kVecs = D / 4;  // float4s of a column

@@ -2,13 +2,13 @@
 // numbers as they are in memory (so a captured call follows them when it is replayed).
 //
 // A unit is a (sequence, KV head) or a (sequence, KV head, query tile); its cost is the key tiles
-// that it sees. All units' key tiles stand in one row, and CTA c of n takes tiles [cW/n, (c+1)W/n)
-// of the W: every CTA the same number, whatever the lengths. A unit that crosses from one CTA to
-// the next is cut there: each piece leaves (max, sum, unnormalised output) partials, and the last
-// piece to arrive merges them in the order of the CTAs. A CTA has at most two cut units, the one
-// that it enters in the middle (slot 2c) and the one that it leaves (slot 2c + 1), so the
-// partials' memory depends on the grid alone. A unit's arrivals are counted at the CTA that
-// starts it (counters[c]; the last piece sets it back to zero).
+// that it sees. All units' key tiles stand in one row, and CTA c takes tiles [cQ, (c + 1)Q) of it, Q
+// = ceil(all / CTAs): every CTA the same number (the last may have fewer), whatever the lengths. A
+// unit that crosses from one CTA to the next is cut there: each piece leaves (max, sum,
+// unnormalised output) partials, and the last piece to arrive merges them in the order of the CTAs.
+// A CTA has at most two cut units, the one that it enters in the middle (slot 2c) and the one that
+// it leaves (slot 2c + 1), so the partials' memory depends on the grid alone. A unit's arrivals are
+// counted at the CTA that starts it (counters[c]; the last piece sets it back to zero).
 #pragma once
 
 #include "fa_paged.h"
@@ -16,17 +16,21 @@
 
 namespace fa {
 
-// CTA c's first tile of W shared among n. (A 64-bit division takes some hundred instructions, which
-// short calls wait for: 32 bits where they do, n being at most 4096.)
-__device__ __forceinline__ int64_t share_begin(int64_t w, int c, int n) {
-  if (w < (1 << 20)) return int64_t(uint32_t(w) * uint32_t(c) / uint32_t(n));
-  return int64_t((unsigned long long)(w) * (unsigned long long)(c) / (unsigned long long)(n));
+// Tiles of a CTA's share: ceil(w / n). (A 64-bit division takes some hundred instructions, which
+// short calls wait for: 32 bits where they do.)
+__device__ __forceinline__ int64_t share_size(int64_t w, int n) {
+  return w < (1 << 30) ? int64_t((uint32_t(w) + n - 1) / uint32_t(n)) : (w + n - 1) / n;
 }
 
-// The CTA whose share holds tile t.
-__device__ __forceinline__ int share_owner(int64_t w, int64_t t, int n) {
-  if (w < (1 << 20)) return int(((uint32_t(t) + 1) * uint32_t(n) - 1) / uint32_t(w));
-  return int((((unsigned long long)(t) + 1) * (unsigned long long)(n)-1) / (unsigned long long)(w));
+// The first and the last CTA that a unit of `cost` tiles from global tile unit0 on is shared among,
+// asked by a CTA (of shares of q) that has tiles of it.
+__device__ __forceinline__ void share_owners(int64_t q, int cta, int64_t unit0, int cost, int* c0,
+                                             int* c1) {
+  const int64_t begin = q * cta;
+  const uint32_t q32 = uint32_t(min(q, int64_t(0x7fffffff)));  // (distances within a unit fit 31 bits)
+  const uint32_t before = unit0 < begin ? uint32_t(begin - unit0) : 0u;
+  *c0 = cta - int((before + q32 - 1) / q32);
+  *c1 = cta + int(uint32_t(unit0 + cost - 1 - begin) / q32);
 }
 
 // How many times `per` goes into t.
