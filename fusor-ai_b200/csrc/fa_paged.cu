@@ -69,6 +69,7 @@ int check_spans(const fa_paged_batch* b) {
   if (b->sequences < 0 || b->rows < 0 || b->max_rows < 0 || b->table_width < 0)
     return fail(FA_ERR_ARG, "a negative count: %d sequences, %d rows, max_rows %d, table_width %d",
                 b->sequences, b->rows, b->max_rows, b->table_width);
+  if (b->rows > (1 << 28)) return fail(FA_ERR_ARG, "%d rows; at most %d", b->rows, 1 << 28);
   if (b->sequences > fa::kMaxPagedSequences)
     return fail(FA_ERR_ARG, "%d sequences; at most %d", b->sequences, fa::kMaxPagedSequences);
   if (b->table_stride < b->table_width)
@@ -332,7 +333,7 @@ extern "C" {
 int fa_paged_workspace_bytes(const fa_paged_cache* cache, int32_t rows, int32_t max_rows,
                              uint64_t* bytes) {
   FA_TRY(check_shape(cache));
-  if (rows < 0 || max_rows < 0 || bytes == nullptr) return fail(FA_ERR_ARG, "bad rows or null bytes");
+  if (rows < 0 || rows > (1 << 28) || max_rows < 0 || bytes == nullptr) return fail(FA_ERR_ARG, "bad rows or null bytes");
   int sms = 0;
   unsigned* err = nullptr;
   FA_TRY(fa::host::device_info(cache->device, &sms, &err));

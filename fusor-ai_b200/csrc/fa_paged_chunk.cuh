@@ -317,7 +317,7 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
       mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], S::kLoad);
       mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1);
+      mbar_init(&s_full[i], 2);
       mbar_init(&p_full[2 * i], 128);
       mbar_init(&p_full[2 * i + 1], 128);
       mbar_init(&o_done[i], 1);
@@ -455,6 +455,8 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
                                 kd + uint64_t((db * BN * 128 + koff) >> 4), kIdescQK, k > 0 ? 1u : 0u);
             }
             tc::commit(&s_full[b]);
+            // (and this thread's own arrival, which passes on what the loaders wrote for the softmax)
+            mbar_arrive(&s_full[b]);
             ++sb;
           };
           // block h of tile L: its probabilities are in columns 32 h of the scores' 128, or at the

@@ -218,6 +218,15 @@ def _stream(stream=None):
     return C.c_void_p(stream.cuda_stream)
 
 
+def _stream_of(device, stream=None):
+    """`stream`, or torch's current stream of `device` (which need not be the current device)."""
+    import torch
+    if stream is not None:
+        return C.c_void_p(stream.cuda_stream)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return C.c_void_p(raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream)
+
+
 def _dptr(t):
     return None if t is None else C.c_void_p(t.data_ptr())
 
@@ -586,9 +595,14 @@ def normalize_and_rotate(heads: int, head_dim: int, qkv, out, norm: int = NORM_R
                                          out.stride(0), dt, _stream(stream)))
 
 
+_ROWS_DTYPES = {}
+
+
 def _rows_dtype(t, what):
-    import torch
-    dt = {torch.float32: F32, torch.bfloat16: BF16}.get(t.dtype)
+    if not _ROWS_DTYPES:
+        import torch
+        _ROWS_DTYPES.update({torch.float32: F32, torch.bfloat16: BF16})
+    dt = _ROWS_DTYPES.get(t.dtype)
     if dt is None:
         raise ValueError(f"{what} of {t.dtype}: float32 or bfloat16")
     if t.dim() == 0 or (t.stride(-1) != 1 and t.shape[-1] > 1):
@@ -598,7 +612,9 @@ def _rows_dtype(t, what):
 
 def _stride0(t):
     """Elements between rows (of a single row: its width, as torch leaves its stride open)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t[0].numel() if t.shape[0] else 1)
+    if t.shape[0] > 1:
+        return t.stride(0)
+    return max(t.stride(0), t.numel(), t.shape[-1])
 
 
 class PagedCache:
@@ -638,6 +654,7 @@ class PagedCache:
                               page_size, dtype, self.device, keys.data_ptr(), values.data_ptr(),
                               key_scales.data_ptr() if dtype == Q8 else None,
                               value_scales.data_ptr() if dtype == Q8 else None)
+        self._ref = C.byref(self._c)
 
     def attention_input(self, layer: int, batch: "PagedBatch", qkv, angles=None,
                         rope: int = ROPE_HALF, norm=None, q_out=None, stream=None):
@@ -647,9 +664,9 @@ class PagedCache:
         if q_out is not None and (_rows_dtype(q_out, "q_out") != dt):
             raise ValueError("q_out has qkv's dtype")
         _check(lib().fa_attention_input_paged(
-            C.byref(self._c), layer, C.byref(batch._c), rope if angles is not None else ROPE_NONE,
+            self._ref, layer, batch._ref, rope if angles is not None else ROPE_NONE,
             _dptr(angles), _norm(norm), _dptr(qkv), _stride0(qkv), dt, _dptr(q_out),
-            0 if q_out is None else _stride0(q_out), _stream(stream)))
+            0 if q_out is None else _stride0(q_out), _stream_of(self.device, stream)))
 
     def _rows(self, batch, keys, values):
         batch.covers(keys, values)
@@ -664,31 +681,31 @@ class PagedCache:
     def write(self, layer: int, batch: "PagedBatch", keys, values, stream=None):
         """Key and value rows (rows, kv_heads, head_dim) into the batch's pages as they are."""
         r = self._rows(batch, keys, values)
-        _check(lib().fa_paged_write(C.byref(self._c), layer, C.byref(batch._c), C.byref(r),
-                                    _stream(stream)))
+        _check(lib().fa_paged_write(self._ref, layer, batch._ref, C.byref(r),
+                                    _stream_of(self.device, stream)))
 
     def read(self, layer: int, batch: "PagedBatch", keys, values, stream=None):
         """The batch's rows read back into keys and values (rows, kv_heads, head_dim)."""
         r = self._rows(batch, keys, values)
-        _check(lib().fa_paged_read(C.byref(self._c), layer, C.byref(batch._c), C.byref(r),
-                                   _stream(stream)))
+        _check(lib().fa_paged_read(self._ref, layer, batch._ref, C.byref(r),
+                                   _stream_of(self.device, stream)))
 
     def attend(self, layer: int, batch: "PagedBatch", q, out, stream=None):
         """KvCache::attend (transformer.rs:182-219) of rotated queries over the pages."""
         batch.covers(q, out)
         _check(lib().fa_attend_paged(
-            C.byref(self._c), layer, C.byref(batch._c), _dptr(q), _stride0(q),
+            self._ref, layer, batch._ref, _dptr(q), _stride0(q),
             _rows_dtype(q, "q"), _dptr(out), _stride0(out), _rows_dtype(out, "out"),
-            _stream(stream)))
+            _stream_of(self.device, stream)))
 
     def attention(self, layer: int, batch: "PagedBatch", qkv, out, angles=None,
                   rope: int = ROPE_HALF, norm=None, stream=None):
         """The attention phase of one layer: the batch's rows kept, then attended."""
         batch.covers(qkv, out, angles)
         _check(lib().fa_attention_paged(
-            C.byref(self._c), layer, C.byref(batch._c), rope if angles is not None else ROPE_NONE,
+            self._ref, layer, batch._ref, rope if angles is not None else ROPE_NONE,
             _dptr(angles), _norm(norm), _dptr(qkv), _stride0(qkv), _rows_dtype(qkv, "qkv"),
-            _dptr(out), _stride0(out), _rows_dtype(out, "out"), _stream(stream)))
+            _dptr(out), _stride0(out), _rows_dtype(out, "out"), _stream_of(self.device, stream)))
 
 
 class PagedBatch:
@@ -718,6 +735,7 @@ class PagedBatch:
         self._c = _PagedBatch(n, rows, max_rows, tables.shape[1], stride, row_starts.data_ptr(),
                               firsts.data_ptr(), tables.data_ptr(), mask.kind, mask.window,
                               self.workspace.data_ptr(), nbytes.value)
+        self._ref = C.byref(self._c)
 
     def covers(self, *tensors):
         for t in tensors:

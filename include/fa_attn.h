@@ -447,10 +447,10 @@ typedef struct {
   float* value_scales;
 } fa_paged_cache;
 
-/* The spans of a call over a paged cache: the rows of `sequences` sequences (at most 1024) one
- * after the other, sequence s's rows row_starts[s] .. row_starts[s + 1] of the call's arrays at
- * the positions from firsts[s] on; its position p lies in slot p % page_size of the page
- * tables[s * table_stride + p / page_size]. The numbers are DEVICE memory, read by the kernels,
+/* The spans of a call over a paged cache: the rows of `sequences` sequences (at most 1024, of 2^28
+ * rows in all) one after the other, sequence s's rows row_starts[s] .. row_starts[s + 1] of the
+ * call's arrays at the positions from firsts[s] on; its position p lies in slot p % page_size of
+ * the page tables[s * table_stride + p / page_size]. The numbers are DEVICE memory, read by the kernels,
  * so a captured call follows them when it is replayed (the host's part of a call depends on
  * rows, max_rows and the mask alone). A sequence may have no rows; rows of the arrays past
  * row_starts[sequences] are padding and left as they are. The mask is FA_MASK_CAUSAL,

@@ -97,6 +97,7 @@ def test_numbers_refused(host, code, say):
 @pytest.mark.parametrize("over,code", [
     (dict(sequences=-1), fa.ERR_ARG), (dict(rows=-1), fa.ERR_ARG), (dict(max_rows=-1), fa.ERR_ARG),
     (dict(sequences=1025), fa.ERR_ARG), (dict(table_stride=1), fa.ERR_ARG),
+    (dict(rows=2**28 + 1), fa.ERR_ARG),
     (dict(null="row_starts"), fa.ERR_ARG), (dict(null="firsts"), fa.ERR_ARG),
     (dict(null="tables"), fa.ERR_ARG)])
 def test_batches_refused(over, code):
