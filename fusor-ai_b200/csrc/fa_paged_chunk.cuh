@@ -682,14 +682,18 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
             }
           }
         };
-        // the exponent that takes the largest finite scale to [2^8, 2^9): 127 of it stay in f16
-        auto exponent = [&](const float (&x)[kKeys]) {
+        // the exponent that takes the largest finite scale to [2^8, 2^9) (127 of it stay in f16), or
+        // 2^least for smaller ones. A row's sum is kept in the unit of its largest values, so the
+        // tiles' units must not lie further apart than f32 reaches: from the values' least, 2^-40,
+        // they do not for scales up to 2^70 (and a value is off by at most 2^-58 more).
+        constexpr int kLeastKeys = -118, kLeastValues = -40;
+        auto exponent = [&](const float (&x)[kKeys], int least) {
           float top = 0.0f;
 #pragma unroll
           for (int i = 0; i < kKeys; ++i)
             top = fmaxf(top, fabsf(x[i]) <= 3.402823466e38f ? fabsf(x[i]) : 0.0f);
           const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-          return bits == 0 ? 0 : min(max(int(bits >> 23) - 127, -110), 120) - 8;
+          return bits == 0 ? 0 : min(max(int(bits >> 23) - 135, least), 112);
         };
         auto power = [](int e) { return __uint_as_float(uint32_t(127 + e) << 23); };
         int at = pc.begin, end = pc.end;
@@ -703,7 +707,7 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
           const int st = stage_of();
           const bool was_edge = edge;
           const uint32_t was_gone = gone;
-          const int ev = exponent(vs), ek = is_v ? 0 : exponent(ks);
+          const int ev = exponent(vs, kLeastValues), ek = is_v ? 0 : exponent(ks, kLeastKeys);
           // this tile's scales as f16 pairs
           const float down = power(is_v ? -ev : -ek);
           __half2 hs[kKeys];
@@ -831,7 +835,8 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
           float scale_t = scale, up_t = 0.0f, down_t = 1.0f;
           if constexpr (Q8) {
             const float4 un = units[(tile + L) & 3];
-            scale_t = scale * un.x;
+            // (not 0, for a masked score times it would be a NaN)
+            scale_t = fmaxf(scale * un.x, 1.175494351e-38f);
             up_t = un.y;
             down_t = un.z;
           }

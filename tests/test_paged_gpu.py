@@ -492,6 +492,66 @@ def test_scores_of_any_size():
     fa.device_status()
 
 
+@pytest.mark.parametrize("size", [1e30, 1e-30])
+@pytest.mark.parametrize("dims", [(14, 2, 64), (32, 8, 128), (8, 2, 256)], ids=str)
+def test_chunk_scores_of_any_size(dims, size):
+    """The same over chunks, at every head_dim."""
+    torch = torch_()
+    shape = fa.Shape(1, *dims)
+    spans = Spans([(70, 130)], 16)
+    cache = make_cache(shape, spans, fa.Q8)
+    cache.key_scales.copy_(torch.rand_like(cache.key_scales) / (40 * size))
+    q = torch.randn((spans.rows, shape.width), device="cuda") * size
+    out = torch.empty((spans.rows, shape.width), device="cuda")
+    cache.attend(0, spans.batch(cache), q, out)
+    fa.device_status()
+    check_close(out, *reference(cache, 0, spans, q.double(), CAUSAL), False)
+
+
+@pytest.mark.parametrize("sp", BOTH, ids=["tokens", "chunks"])
+@pytest.mark.parametrize("dims", [(14, 2, 64), (32, 8, 128), (8, 2, 256)], ids=str)
+@pytest.mark.parametrize("mask", [CAUSAL, fa.Mask.window_of(40)], ids=str)
+@pytest.mark.parametrize("small", [2.0 ** -14, 2.0 ** -60], ids=["2^-14", "2^-60"])
+def test_queries_of_zeros_over_small_keys(dims, sp, mask, small):
+    """A row whose query is zero (a padded one) weighs its keys alike, however small they are."""
+    torch = torch_()
+    shape = fa.Shape(1, *dims)
+    spans = Spans(sp, 16)
+    cache = make_cache(shape, spans, fa.Q8)
+    cache.key_scales *= small
+    q = torch.randn((spans.rows, shape.width), device="cuda").bfloat16()
+    q[::2] = 0
+    q[1::4] *= 2.0 ** -100
+    out = torch.empty((spans.rows, shape.width), device="cuda")
+    cache.attend(0, spans.batch(cache, mask), q, out)
+    fa.device_status()
+    check_close(out, *reference(cache, 0, spans, q.double(), mask), False)
+
+
+@pytest.mark.parametrize("sp", BOTH, ids=["tokens", "chunks"])
+@pytest.mark.parametrize("dims", [(14, 2, 64), (32, 8, 128), (8, 2, 256)], ids=str)
+@pytest.mark.parametrize("sizes", [(60, -80), (-80, 60), (-40, -40), (-20, 20)], ids=str)
+def test_values_of_any_size(dims, sp, sizes):
+    """Blocks of positions whose values differ by many powers of two: the weights of the small
+    ones count in the sum all the same."""
+    torch = torch_()
+    shape = fa.Shape(1, *dims)
+    spans = Spans(sp, 16)
+    cache = make_cache(shape, spans, fa.Q8)
+    for i, (rows, first) in enumerate(spans.spans):
+        for lo in range(0, first + rows, 128):
+            page, slot = spans.places(i, lo, min(lo + 128, first + rows))
+            cache.value_scales[0, page, :, slot] *= 2.0 ** sizes[lo // 128 % 2]
+    q = torch.randn((spans.rows, shape.width), device="cuda").bfloat16()
+    out = torch.empty((spans.rows, shape.width), device="cuda")
+    cache.attend(0, spans.batch(cache), q, out)
+    fa.device_status()
+    want, tol = reference(cache, 0, spans, q.double(), CAUSAL)
+    up = 2.0 ** -max(sizes)
+    # (values are off by at most 2^-58 besides)
+    check_close(out.double() * up, want * up, tol * up + 2.0 ** -58 * up, False)
+
+
 @pytest.mark.parametrize("rows", [2, 60])
 @pytest.mark.parametrize("dims", [(14, 2, 64), (32, 8, 128), (8, 2, 256)], ids=str)
 def test_huge_heads_leave_the_others_their_precision(dims, rows):
