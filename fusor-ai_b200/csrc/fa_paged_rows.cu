@@ -58,24 +58,15 @@ __device__ __forceinline__ bool place_of(const PagedSpans& b, const PagedPool& p
   return true;
 }
 
-// E consecutive elements as f32: one vector load where the row is aligned for it.
-template <typename T, int E>
-__device__ __forceinline__ void load_elems(const T* p, bool vec, float (&x)[E]) {
+// Four consecutive elements: one load where the row is aligned for it.
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, bool vec, T* x) {
   if (vec) {
-    constexpr int B = E * int(sizeof(T));
-    alignas(16) T raw[E];
-    if constexpr (B == 4) *reinterpret_cast<uint32_t*>(raw) = __ldcs(reinterpret_cast<const unsigned int*>(p));
-    else if constexpr (B == 8) *reinterpret_cast<uint2*>(raw) = __ldcs(reinterpret_cast<const uint2*>(p));
-    else {
-#pragma unroll
-      for (int i = 0; i < B / 16; ++i)
-        reinterpret_cast<uint4*>(raw)[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = float(raw[e]);
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(x) = __ldcs(reinterpret_cast<const uint4*>(p));
+    else *reinterpret_cast<uint2*>(x) = __ldcs(reinterpret_cast<const uint2*>(p));
   } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = float(p[e]);
+    for (int e = 0; e < 4; ++e) x[e] = p[e];
   }
 }
 
@@ -117,127 +108,135 @@ __device__ __forceinline__ uint32_t pack_bytes(int a, int b, int c, int d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// One CTA per row. A head's elements lie eight to a lane on D / 8 lanes, so that a warp takes 32 / (D
-// / 8) heads of one kind (queries, keys, values) at a time (a step); it takes every kRowWarps-th
-// step, the first one's loads issued before the row's place is looked up. RoPE by halves finds the partner of an element half a head's lanes away,
-// interleaved RoPE within the lane; the row's cosines and sines are loaded once for all of a warp's
-// heads. Arithmetic of the rotation: each product rounded, then the difference or sum
-// (ops.rs:77-95; x - y is x + (-y), so that a lane's sign goes into its sine once).
-// Bound by the latency of a row's loads, hidden by many warps: 10 thousand rows of 32/8 heads of 128
-// (bf16 rows, 8-bit pages, 231 MB) take 57 us with 48 warps an SM (40 registers), 76 us with two
-// or three steps' loads in flight and 28 warps.
+// One CTA per row. A head's elements lie eight to a lane on D / 8 lanes, four of each half (the
+// partners of RoPE by halves are in one lane, and those of interleaved RoPE too), so that a warp
+// takes 32 / (D / 8) heads of one kind (queries, keys, values) at a time (a step); it takes every
+// kRowWarps-th step, the first one's loads issued before the row's place is looked up and each next
+// one's before the last is worked on. The row's cosines and sines are loaded once for all of a
+// warp's heads. Arithmetic of the rotation: each product rounded, then the difference or sum
+// (ops.rs:77-95).
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowWarps * 32, 12)
     paged_write_kernel(const __grid_constant__ PagedWriteArgs a) {
-  constexpr int E = 8, LH = D / E, HW = 32 / LH;  // lanes of a head, heads of a step
+  constexpr int LH = D / 8, HW = 32 / LH;  // lanes of a head, heads of a step
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = lane % LH, which = lane / LH;
+  const int lo = sub * 4;  // this lane's elements lo .. lo + 3 and D / 2 + lo ..
   const int r = blockIdx.x;
   const int kvh = a.pool.kv_heads;
   const int q_steps = a.q_out == nullptr ? 0 : (a.heads + HW - 1) / HW, kv_steps = (kvh + HW - 1) / HW;
   const int steps = q_steps + 2 * kv_steps;
-  const T* const q = static_cast<const T*>(a.q) + int64_t(r) * a.q_stride + sub * E;
-  const T* const k = static_cast<const T*>(a.k) + int64_t(r) * a.k_stride + sub * E;
-  const T* const v = static_cast<const T*>(a.v) + int64_t(r) * a.v_stride + sub * E;
   // a step's kind (0 queries, 1 keys, 2 values) and this lane's head of it
   auto kind_of = [&](int t) { return t < q_steps ? 0 : t < q_steps + kv_steps ? 1 : 2; };
   auto head_of = [&](int t, int kind) {
     return (kind == 0 ? t : kind == 1 ? t - q_steps : t - q_steps - kv_steps) * HW + which;
   };
-  float x[E];
+  alignas(16) T raw[8];
   auto load = [&](int t) {
     const int kind = kind_of(t), h = head_of(t, kind);
-    const T* p = kind == 0 ? q + h * D : kind == 1 ? k + h * a.k_head_stride : v + h * a.v_head_stride;
-    if (h < (kind == 0 ? a.heads : kvh)) {
-      load_elems<T, E>(p, a.vec != 0, x);
+    const void* base = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+    const int64_t row = kind == 0 ? a.q_stride : kind == 1 ? a.k_stride : a.v_stride;
+    const int64_t head = kind == 0 ? D : kind == 1 ? a.k_head_stride : a.v_head_stride;
+    if (h >= (kind == 0 ? a.heads : kvh)) return;  // (the lane keeps what it had)
+    const T* p = static_cast<const T*>(base) + r * row + h * head + lo;
+    load4(p, a.vec != 0, raw);
+    load4(p + D / 2, a.vec != 0, raw + 4);
+  };
+#pragma unroll
+  for (int e = 0; e < 8; ++e) raw[e] = T(0.0f);
+  if (warp < steps) load(warp);
+  alignas(16) float c[4], s[4];
+  if (a.rope != 0) {
+    // by halves: the elements' own; interleaved: of pairs lo / 2, lo / 2 + 1, and those of D / 2 + lo
+    const float* cs = a.angles + int64_t(r) * D;
+    if (a.rope == 1) {
+      load4(cs + lo, a.angles_vec != 0, c);
+      load4(cs + D / 2 + lo, a.angles_vec != 0, s);
     } else {
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = 0.0f;
+      for (int e = 0; e < 4; ++e) {
+        const int pair = (e & 1) + lo / 2 + (e >> 1) * (D / 4);
+        c[e] = cs[pair];
+        s[e] = cs[D / 2 + pair];
+      }
     }
-  };
-  if (warp < steps) load(warp);
-  float c[E], s[E];
-  if (a.rope == 1) {
-    const float* cs = a.angles + int64_t(r) * D + (sub % (LH / 2)) * E;
-    load_elems<float, E>(cs, a.angles_vec != 0, c);
-    load_elems<float, E>(cs + D / 2, a.angles_vec != 0, s);
-#pragma unroll
-    for (int e = 0; e < E; ++e) s[e] = sub < LH / 2 ? -s[e] : s[e];
-  } else if (a.rope == 2) {
-    const float* cs = a.angles + int64_t(r) * D + sub * (E / 2);
-#pragma unroll
-    for (int e = 0; e < E / 2; ++e) { c[e] = cs[e]; s[e] = cs[D / 2 + e]; }
   }
   int page, slot;
   if (!place_of(a.spans, a.pool, r, lane, &page, &slot, a.err)) return;  // the warp's, as one
   for (int t = warp; t < steps; t += kRowWarps) {
-    if (t != warp) load(t);
     const int kind = kind_of(t), h = head_of(t, kind);  // the kind is the warp's
     const bool live = h < (kind == 0 ? a.heads : kvh);
+    float x[8];  // elements lo .. lo + 3, D / 2 + lo ..
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = float(raw[e]);
+    if (t + kRowWarps < steps) load(t + kRowWarps);
     if (kind < 2) {
       const float* weight = kind == 0 ? a.q_norm : a.k_norm;
       if (weight != nullptr) {
         float ss = 0.0f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) ss = fmaf(x[e], x[e], ss);
+        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
         for (int off = LH / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
         const float inverse = 1.0f / sqrtf(ss / float(D) + a.eps);
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = __fmul_rn(__fmul_rn(x[e], inverse), weight[sub * E + e]);
+        for (int e = 0; e < 8; ++e)
+          x[e] = __fmul_rn(__fmul_rn(x[e], inverse), weight[(e >> 2) * (D / 2) + lo + (e & 3)]);
       }
+      auto turn = [&](float& x0, float& x1, int i) {
+        const float y0 = x0, y1 = x1;
+        x0 = __fsub_rn(__fmul_rn(y0, c[i]), __fmul_rn(y1, s[i]));
+        x1 = __fadd_rn(__fmul_rn(y1, c[i]), __fmul_rn(y0, s[i]));
+      };
       if (a.rope == 1) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float o = __shfl_xor_sync(0xffffffffu, x[e], LH / 2);
-          x[e] = __fadd_rn(__fmul_rn(x[e], c[e]), __fmul_rn(o, s[e]));
-        }
+        for (int e = 0; e < 4; ++e) turn(x[e], x[4 + e], e);
       } else if (a.rope == 2) {
 #pragma unroll
-        for (int e = 0; e < E / 2; ++e) {
-          const float y0 = x[2 * e], y1 = x[2 * e + 1];
-          x[2 * e] = __fsub_rn(__fmul_rn(y0, c[e]), __fmul_rn(y1, s[e]));
-          x[2 * e + 1] = __fadd_rn(__fmul_rn(y1, c[e]), __fmul_rn(y0, s[e]));
-        }
+        for (int e = 0; e < 4; ++e) turn(x[2 * e], x[2 * e + 1], e);
       }
     }
+    const float(&x0)[4] = *reinterpret_cast<const float(*)[4]>(&x[0]);
+    const float(&x1)[4] = *reinterpret_cast<const float(*)[4]>(&x[4]);
     if (kind == 0) {
-      if (live)
-        store_elems<E>(a.q_out, int64_t(r) * a.q_out_stride + h * D + sub * E, a.q_out_bf16 != 0,
-                       a.q_out_vec != 0, x);
+      if (live) {
+        const int64_t at = int64_t(r) * a.q_out_stride + h * D + lo;
+        store_elems<4>(a.q_out, at, a.q_out_bf16 != 0, a.q_out_vec != 0, x0);
+        store_elems<4>(a.q_out, at + D / 2, a.q_out_bf16 != 0, a.q_out_vec != 0, x1);
+      }
       continue;
     }
     const int64_t row = ((int64_t(page) * kvh + h) << a.pool.page_shift) + slot;
     unsigned char* base = kind == 1 ? a.pool.keys : a.pool.values;
     if (!a.pool.q8) {
-      if (live) store_elems<E>(base, row * D + sub * E, true, true, x);
+      if (live) {
+        store_elems<4>(base, row * D + lo, true, true, x0);
+        store_elems<4>(base, row * D + D / 2 + lo, true, true, x1);
+      }
       continue;
     }
-    float top = 0.0f, total = 0.0f;  // (total: NaN if an element is not finite)
+    // the largest |x|, as integers (they rise with the floats; an infinity or a NaN is above all)
+    uint32_t bits = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      top = fmaxf(top, fabsf(x[e]));
-      total = fmaf(x[e], 0.0f, total);
-    }
+    for (int e = 0; e < 8; ++e) bits = max(bits, __float_as_uint(x[e]) & 0x7fffffffu);
 #pragma unroll
-    for (int off = LH / 2; off >= 1; off >>= 1) {
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-      total += __shfl_xor_sync(0xffffffffu, total, off);
-    }
-    const bool finite = total == 0.0f;
+    for (int off = LH / 2; off >= 1; off >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, off));
+    const float top = __uint_as_float(bits);
+    const bool finite = bits < 0x7f800000u;
     const bool some = finite && top >= 7.888609052e-31f;  // 2^-100
     const float inverse = some ? __fdiv_rn(127.0f, top) : 0.0f;
     const float scale = !finite ? __int_as_float(0x7fffffff) : some ? __fdiv_rn(top, 127.0f) : 0.0f;
     // x (127 / top) is within +-127 but for two roundings, and so rounds to -127 .. 127; what is
     // not finite times 0 converts to 0
-    int n[E];
+    int n[8];
 #pragma unroll
-    for (int e = 0; e < E; ++e) n[e] = __float2int_rn(__fmul_rn(x[e], inverse));
+    for (int e = 0; e < 8; ++e) n[e] = __float2int_rn(__fmul_rn(x[e], inverse));
     if (!live) continue;
-    *reinterpret_cast<uint2*>(base + row * D + sub * E) =
-        make_uint2(pack_bytes(n[0], n[1], n[2], n[3]), pack_bytes(n[4], n[5], n[6], n[7]));
+    unsigned char* to = base + row * D + lo;
+    *reinterpret_cast<uint32_t*>(to) = pack_bytes(n[0], n[1], n[2], n[3]);
+    *reinterpret_cast<uint32_t*>(to + D / 2) = pack_bytes(n[4], n[5], n[6], n[7]);
     if (sub == 0) (kind == 1 ? a.pool.key_scales : a.pool.value_scales)[row] = scale;
   }
 }

@@ -450,8 +450,8 @@ typedef struct {
 /* The spans of a call over a paged cache: the rows of `sequences` sequences (at most 1024, of 2^28
  * rows in all) one after the other, sequence s's rows row_starts[s] .. row_starts[s + 1] of the
  * call's arrays at the positions from firsts[s] on; its position p lies in slot p % page_size of
- * the page tables[s * table_stride + p / page_size]. The numbers are DEVICE memory, read by the kernels,
- * so a captured call follows them when it is replayed (the host's part of a call depends on
+ * the page tables[s * table_stride + p / page_size]. The numbers are DEVICE memory, read by the
+ * kernels, so a captured call follows them when it is replayed (the host's part of a call depends on
  * rows, max_rows and the mask alone). A sequence may have no rows; rows of the arrays past
  * row_starts[sequences] are padding and left as they are. The mask is FA_MASK_CAUSAL,
  * FA_MASK_WINDOW or FA_MASK_FULL (every position up to the sequence's last new row).
@@ -529,7 +529,9 @@ int fa_paged_read(const fa_paged_cache* cache, int32_t layer, const fa_paged_bat
  * sequences' pages under the mask, into out (rows out_stride apart, of out_dtype), scores scaled
  * by 1/sqrt(head_dim). Any number of rows to a sequence: single tokens, chunks, and both in one
  * call. Queries and probabilities are rounded to 16 bits for the tensor cores, scores, sums and
- * outputs accumulated in f32. A row that sees no position (its pages out of range) is zero. */
+ * outputs accumulated in f32. A row that sees no position (its pages out of range) is zero. A value
+ * that is not finite reaches the rows that see its position, whose elements may all become NaN,
+ * and no others. Value scales are to be below 2^70 (larger ones may lose smaller values' weights). */
 int fa_attend_paged(const fa_paged_cache* cache, int32_t layer, const fa_paged_batch* batch,
                     const void* q, int64_t q_stride, int32_t dtype, void* out,
                     int64_t out_stride, int32_t out_dtype, void* stream);
