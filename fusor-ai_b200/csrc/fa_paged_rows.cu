@@ -7,6 +7,8 @@
 // a NaN scale (it reads back as NaN throughout, and attends as NaN where it is seen).
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "fa_paged.h"
 #include "fa_ptx.cuh"
 
@@ -115,7 +117,11 @@ __device__ __forceinline__ uint32_t pack_bytes(int a, int b, int c, int d) {
 // one's before the last is worked on. The row's cosines and sines are loaded once for all of a
 // warp's heads. Arithmetic of the rotation: each product rounded, then the difference or sum
 // (ops.rs:77-95).
-template <typename T, int D>
+// Bound by issued instructions (80 % of the cycles of a long call) with memory close behind, so each
+// kind has a loop of its own, and calls whose arrays are all 16-byte aligned have a kernel without
+// the element-wise accesses (Vec): 8500 rows of 32/8 heads of 128 (bf16 rows, 8-bit pages, 196 MB)
+// take 44 us (4.4 TB/s), 51 us in one loop of all kinds that tests the alignment.
+template <typename T, int D, bool Vec>
 __global__ void __launch_bounds__(kRowWarps * 32, 12)
     paged_write_kernel(const __grid_constant__ PagedWriteArgs a) {
   constexpr int LH = D / 8, HW = 32 / LH;  // lanes of a head, heads of a step
@@ -128,32 +134,29 @@ __global__ void __launch_bounds__(kRowWarps * 32, 12)
   const int kvh = a.pool.kv_heads;
   const int q_steps = a.q_out == nullptr ? 0 : (a.heads + HW - 1) / HW, kv_steps = (kvh + HW - 1) / HW;
   const int steps = q_steps + 2 * kv_steps;
-  // a step's kind (0 queries, 1 keys, 2 values) and this lane's head of it
-  auto kind_of = [&](int t) { return t < q_steps ? 0 : t < q_steps + kv_steps ? 1 : 2; };
-  auto head_of = [&](int t, int kind) {
-    return (kind == 0 ? t : kind == 1 ? t - q_steps : t - q_steps - kv_steps) * HW + which;
-  };
   alignas(16) T raw[8];
-  auto load = [&](int t) {
-    const int kind = kind_of(t), h = head_of(t, kind);
-    const void* base = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-    const int64_t row = kind == 0 ? a.q_stride : kind == 1 ? a.k_stride : a.v_stride;
-    const int64_t head = kind == 0 ? D : kind == 1 ? a.k_head_stride : a.v_head_stride;
-    if (h >= (kind == 0 ? a.heads : kvh)) return;  // (the lane keeps what it had)
+  auto load = [&](const void* base, int64_t row, int64_t head, int heads, int t) {
+    const int h = t * HW + which;
+    if (h >= heads) return;  // (the lane keeps what it had)
     const T* p = static_cast<const T*>(base) + r * row + h * head + lo;
-    load4(p, a.vec != 0, raw);
-    load4(p + D / 2, a.vec != 0, raw + 4);
+    load4(p, Vec, raw);
+    load4(p + D / 2, Vec, raw + 4);
+  };
+  auto load_any = [&](int t) {
+    if (t < q_steps) load(a.q, a.q_stride, D, a.heads, t);
+    else if (t < q_steps + kv_steps) load(a.k, a.k_stride, a.k_head_stride, kvh, t - q_steps);
+    else if (t < steps) load(a.v, a.v_stride, a.v_head_stride, kvh, t - q_steps - kv_steps);
   };
 #pragma unroll
   for (int e = 0; e < 8; ++e) raw[e] = T(0.0f);
-  if (warp < steps) load(warp);
+  load_any(warp);
   alignas(16) float c[4], s[4];
   if (a.rope != 0) {
     // by halves: the elements' own; interleaved: of pairs lo / 2, lo / 2 + 1, and those of D / 2 + lo
     const float* cs = a.angles + int64_t(r) * D;
     if (a.rope == 1) {
-      load4(cs + lo, a.angles_vec != 0, c);
-      load4(cs + D / 2 + lo, a.angles_vec != 0, s);
+      load4(cs + lo, Vec, c);
+      load4(cs + D / 2 + lo, Vec, s);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -165,84 +168,98 @@ __global__ void __launch_bounds__(kRowWarps * 32, 12)
   }
   int page, slot;
   if (!place_of(a.spans, a.pool, r, lane, &page, &slot, a.err)) return;  // the warp's, as one
-  for (int t = warp; t < steps; t += kRowWarps) {
-    const int kind = kind_of(t), h = head_of(t, kind);  // the kind is the warp's
-    const bool live = h < (kind == 0 ? a.heads : kvh);
-    float x[8];  // elements lo .. lo + 3, D / 2 + lo ..
+  const int64_t row0 = ((int64_t(page) * kvh) << a.pool.page_shift) + slot;  // KV head 0's
+  // The steps of one kind: 0 queries, 1 keys, 2 values; `begin` of them all to `end`.
+  int t = warp;
+  auto section = [&](auto kind_c, int begin, int end) {
+    constexpr int kind = decltype(kind_c)::value;
+    const int heads = kind == 0 ? a.heads : kvh;
+    for (; t < end; t += kRowWarps) {
+      const int h = (t - begin) * HW + which;
+      const bool live = h < heads;
+      float x[8];  // elements lo .. lo + 3, D / 2 + lo ..
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = float(raw[e]);
-    if (t + kRowWarps < steps) load(t + kRowWarps);
-    if (kind < 2) {
-      const float* weight = kind == 0 ? a.q_norm : a.k_norm;
-      if (weight != nullptr) {
-        float ss = 0.0f;
+      for (int e = 0; e < 8; ++e) x[e] = float(raw[e]);
+      if (kind == 0 && t + kRowWarps < end) load(a.q, a.q_stride, D, heads, t + kRowWarps);
+      else load_any(t + kRowWarps);
+      if constexpr (kind < 2) {
+        const float* weight = kind == 0 ? a.q_norm : a.k_norm;
+        if (weight != nullptr) {
+          float ss = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+          for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
-        for (int off = LH / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-        const float inverse = 1.0f / sqrtf(ss / float(D) + a.eps);
+          for (int off = LH / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+          const float inverse = 1.0f / sqrtf(ss / float(D) + a.eps);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          x[e] = __fmul_rn(__fmul_rn(x[e], inverse), weight[(e >> 2) * (D / 2) + lo + (e & 3)]);
+          for (int e = 0; e < 8; ++e)
+            x[e] = __fmul_rn(__fmul_rn(x[e], inverse), weight[(e >> 2) * (D / 2) + lo + (e & 3)]);
+        }
+        auto turn = [&](float& x0, float& x1, int i) {
+          const float y0 = x0, y1 = x1;
+          x0 = __fsub_rn(__fmul_rn(y0, c[i]), __fmul_rn(y1, s[i]));
+          x1 = __fadd_rn(__fmul_rn(y1, c[i]), __fmul_rn(y0, s[i]));
+        };
+        if (a.rope == 1) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) turn(x[e], x[4 + e], e);
+        } else if (a.rope == 2) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) turn(x[2 * e], x[2 * e + 1], e);
+        }
       }
-      auto turn = [&](float& x0, float& x1, int i) {
-        const float y0 = x0, y1 = x1;
-        x0 = __fsub_rn(__fmul_rn(y0, c[i]), __fmul_rn(y1, s[i]));
-        x1 = __fadd_rn(__fmul_rn(y1, c[i]), __fmul_rn(y0, s[i]));
-      };
-      if (a.rope == 1) {
+      const float(&x0)[4] = *reinterpret_cast<const float(*)[4]>(&x[0]);
+      const float(&x1)[4] = *reinterpret_cast<const float(*)[4]>(&x[4]);
+      if constexpr (kind == 0) {
+        if (live) {
+          const int64_t at = r * a.q_out_stride + h * D + lo;
+          store_elems<4>(a.q_out, at, a.q_out_bf16 != 0, Vec, x0);
+          store_elems<4>(a.q_out, at + D / 2, a.q_out_bf16 != 0, Vec, x1);
+        }
+      } else {
+        const int64_t row = row0 + (int64_t(h) << a.pool.page_shift);
+        unsigned char* base = kind == 1 ? a.pool.keys : a.pool.values;
+        if (!a.pool.q8) {
+          if (live) {
+            store_elems<4>(base, row * D + lo, true, true, x0);
+            store_elems<4>(base, row * D + D / 2 + lo, true, true, x1);
+          }
+          continue;
+        }
+        // the largest |x|, as integers (they rise with the floats; an infinity or a NaN is above all)
+        uint32_t bits = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) turn(x[e], x[4 + e], e);
-      } else if (a.rope == 2) {
+        for (int e = 0; e < 8; ++e) bits = max(bits, __float_as_uint(x[e]) & 0x7fffffffu);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) turn(x[2 * e], x[2 * e + 1], e);
+        for (int off = LH / 2; off >= 1; off >>= 1)
+          bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, off));
+        const float top = __uint_as_float(bits);
+        const bool finite = bits < 0x7f800000u;
+        const bool some = finite && top >= 7.888609052e-31f;  // 2^-100
+        const float inverse = some ? __fdiv_rn(127.0f, top) : 0.0f;
+        // x (127 / top) is within +-127 but for two roundings, and so rounds to -127 .. 127; what is
+        // not finite times 0 converts to 0
+        int n[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) n[e] = __float2int_rn(__fmul_rn(x[e], inverse));
+        if (!live) continue;
+        unsigned char* to = base + row * D + lo;
+        *reinterpret_cast<uint32_t*>(to) = pack_bytes(n[0], n[1], n[2], n[3]);
+        *reinterpret_cast<uint32_t*>(to + D / 2) = pack_bytes(n[4], n[5], n[6], n[7]);
+        if (sub == 0)
+          (kind == 1 ? a.pool.key_scales : a.pool.value_scales)[row] =
+              !finite ? __int_as_float(0x7fffffff) : some ? __fdiv_rn(top, 127.0f) : 0.0f;
       }
     }
-    const float(&x0)[4] = *reinterpret_cast<const float(*)[4]>(&x[0]);
-    const float(&x1)[4] = *reinterpret_cast<const float(*)[4]>(&x[4]);
-    if (kind == 0) {
-      if (live) {
-        const int64_t at = int64_t(r) * a.q_out_stride + h * D + lo;
-        store_elems<4>(a.q_out, at, a.q_out_bf16 != 0, a.q_out_vec != 0, x0);
-        store_elems<4>(a.q_out, at + D / 2, a.q_out_bf16 != 0, a.q_out_vec != 0, x1);
-      }
-      continue;
-    }
-    const int64_t row = ((int64_t(page) * kvh + h) << a.pool.page_shift) + slot;
-    unsigned char* base = kind == 1 ? a.pool.keys : a.pool.values;
-    if (!a.pool.q8) {
-      if (live) {
-        store_elems<4>(base, row * D + lo, true, true, x0);
-        store_elems<4>(base, row * D + D / 2 + lo, true, true, x1);
-      }
-      continue;
-    }
-    // the largest |x|, as integers (they rise with the floats; an infinity or a NaN is above all)
-    uint32_t bits = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) bits = max(bits, __float_as_uint(x[e]) & 0x7fffffffu);
-#pragma unroll
-    for (int off = LH / 2; off >= 1; off >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, off));
-    const float top = __uint_as_float(bits);
-    const bool finite = bits < 0x7f800000u;
-    const bool some = finite && top >= 7.888609052e-31f;  // 2^-100
-    const float inverse = some ? __fdiv_rn(127.0f, top) : 0.0f;
-    const float scale = !finite ? __int_as_float(0x7fffffff) : some ? __fdiv_rn(top, 127.0f) : 0.0f;
-    // x (127 / top) is within +-127 but for two roundings, and so rounds to -127 .. 127; what is
-    // not finite times 0 converts to 0
-    int n[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) n[e] = __float2int_rn(__fmul_rn(x[e], inverse));
-    if (!live) continue;
-    unsigned char* to = base + row * D + lo;
-    *reinterpret_cast<uint32_t*>(to) = pack_bytes(n[0], n[1], n[2], n[3]);
-    *reinterpret_cast<uint32_t*>(to + D / 2) = pack_bytes(n[4], n[5], n[6], n[7]);
-    if (sub == 0) (kind == 1 ? a.pool.key_scales : a.pool.value_scales)[row] = scale;
-  }
+  };
+  section(std::integral_constant<int, 0>{}, 0, q_steps);
+  section(std::integral_constant<int, 1>{}, q_steps, q_steps + kv_steps);
+  section(std::integral_constant<int, 2>{}, q_steps + kv_steps, steps);
 }
 
 // A warp takes two rows: their places, then 16 bytes of them a lane at a time, eight such loads in
-// flight (two vectors of keys and of values of each row). Bound by memory.
+// flight (two vectors of keys and of values of each row). Bound by memory: 125 thousand positions of
+// 8 KV heads of 128 out of 8-bit pages to bf16 rows (780 MB) take 162 us, 4.8 TB/s.
 constexpr int kReadWarps = 8, kReadRows = 2 * kReadWarps;
 
 template <bool Q8, int D>
@@ -337,19 +354,21 @@ cudaError_t launch(void (*kernel)(Args), int grid, int block, const Args& args,
 cudaError_t launch_paged_write(const PagedWriteArgs& a, cudaStream_t stream) {
   if (a.spans.rows == 0) return cudaSuccess;
   const int d = a.pool.head_dim;
-  auto go = [&](void (*k)(PagedWriteArgs)) {
-    return launch(k, a.spans.rows, kRowWarps * 32, a, stream);
+  // (of every array that is there, each 16-byte aligned; else element by element)
+  const bool vec = a.vec != 0 && (a.rope != 1 || a.angles_vec != 0) && (a.q_out == nullptr || a.q_out_vec != 0);
+  auto go = [&](auto t, auto dim) {
+    using T = decltype(t);
+    constexpr int D = decltype(dim)::value;
+    return launch(vec ? paged_write_kernel<T, D, true> : paged_write_kernel<T, D, false>, a.spans.rows,
+                  kRowWarps * 32, a, stream);
   };
-  if (a.in_bf16) {
-    if (d == 64) return go(paged_write_kernel<__nv_bfloat16, 64>);
-    if (d == 128) return go(paged_write_kernel<__nv_bfloat16, 128>);
-    if (d == 256) return go(paged_write_kernel<__nv_bfloat16, 256>);
-  } else {
-    if (d == 64) return go(paged_write_kernel<float, 64>);
-    if (d == 128) return go(paged_write_kernel<float, 128>);
-    if (d == 256) return go(paged_write_kernel<float, 256>);
-  }
-  return cudaErrorInvalidValue;
+  auto dims = [&](auto t) {
+    if (d == 64) return go(t, std::integral_constant<int, 64>{});
+    if (d == 128) return go(t, std::integral_constant<int, 128>{});
+    if (d == 256) return go(t, std::integral_constant<int, 256>{});
+    return cudaErrorInvalidValue;
+  };
+  return a.in_bf16 ? dims(__nv_bfloat16(0.0f)) : dims(0.0f);
 }
 
 cudaError_t launch_paged_read(const PagedReadArgs& a, cudaStream_t stream) {
