@@ -598,7 +598,7 @@ def normalize_and_rotate(heads: int, head_dim: int, qkv, out, norm: int = NORM_R
 _ROWS_DTYPES = {}
 
 
-def _rows_dtype(t, what):
+def _rows_dtype(t, what, width=0):
     if not _ROWS_DTYPES:
         import torch
         _ROWS_DTYPES.update({torch.float32: F32, torch.bfloat16: BF16})
@@ -607,7 +607,19 @@ def _rows_dtype(t, what):
         raise ValueError(f"{what} of {t.dtype}: float32 or bfloat16")
     if t.dim() == 0 or (t.stride(-1) != 1 and t.shape[-1] > 1):
         raise ValueError(f"{what} with unit stride along a row")
+    if width and (t.dim() != 2 or t.shape[1] < width):
+        raise ValueError(f"{what} of {tuple(t.shape)}: rows of {width} elements")
     return dt
+
+
+def _angles(t, head_dim):
+    """Rows of cosines and sines (rows, head_dim), or None."""
+    if t is None:
+        return None
+    import torch
+    if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != head_dim or not t.is_contiguous():
+        raise ValueError(f"angles: contiguous float32 rows of {head_dim}")
+    return C.c_void_p(t.data_ptr())
 
 
 def _stride0(t):
@@ -655,17 +667,18 @@ class PagedCache:
                               key_scales.data_ptr() if dtype == Q8 else None,
                               value_scales.data_ptr() if dtype == Q8 else None)
         self._ref = C.byref(self._c)
+        self._qkv_width = (shape.heads + 2 * shape.kv_heads) * shape.head_dim
 
     def attention_input(self, layer: int, batch: "PagedBatch", qkv, angles=None,
                         rope: int = ROPE_HALF, norm=None, q_out=None, stream=None):
         """RoPE (+ head norm) and keep of the batch's rows into their pages (layer.rs:175-234)."""
         batch.covers(qkv, q_out, angles)
-        dt = _rows_dtype(qkv, "qkv")
-        if q_out is not None and (_rows_dtype(q_out, "q_out") != dt):
+        dt = _rows_dtype(qkv, "qkv", self._qkv_width)
+        if q_out is not None and _rows_dtype(q_out, "q_out", self.shape.width) != dt:
             raise ValueError("q_out has qkv's dtype")
         _check(lib().fa_attention_input_paged(
             self._ref, layer, batch._ref, rope if angles is not None else ROPE_NONE,
-            _dptr(angles), _norm(norm), _dptr(qkv), _stride0(qkv), dt, _dptr(q_out),
+            _angles(angles, self.shape.head_dim), _norm(norm), _dptr(qkv), _stride0(qkv), dt, _dptr(q_out),
             0 if q_out is None else _stride0(q_out), _stream_of(self.device, stream)))
 
     def _rows(self, batch, keys, values):
@@ -695,7 +708,7 @@ class PagedCache:
         batch.covers(q, out)
         _check(lib().fa_attend_paged(
             self._ref, layer, batch._ref, _dptr(q), _stride0(q),
-            _rows_dtype(q, "q"), _dptr(out), _stride0(out), _rows_dtype(out, "out"),
+            _rows_dtype(q, "q", self.shape.width), _dptr(out), _stride0(out), _rows_dtype(out, "out", self.shape.width),
             _stream_of(self.device, stream)))
 
     def attention(self, layer: int, batch: "PagedBatch", qkv, out, angles=None,
@@ -704,8 +717,8 @@ class PagedCache:
         batch.covers(qkv, out, angles)
         _check(lib().fa_attention_paged(
             self._ref, layer, batch._ref, rope if angles is not None else ROPE_NONE,
-            _dptr(angles), _norm(norm), _dptr(qkv), _stride0(qkv), _rows_dtype(qkv, "qkv"),
-            _dptr(out), _stride0(out), _rows_dtype(out, "out"), _stream_of(self.device, stream)))
+            _angles(angles, self.shape.head_dim), _norm(norm), _dptr(qkv), _stride0(qkv), _rows_dtype(qkv, "qkv", self._qkv_width),
+            _dptr(out), _stride0(out), _rows_dtype(out, "out", self.shape.width), _stream_of(self.device, stream)))
 
 
 class PagedBatch:

@@ -168,3 +168,39 @@ def test_pool_tensors_are_checked():
         fa.PagedCache(shape, 3, 16, fa.F32, keys=good, values=good)
     flags, _ = fa.capabilities()
     assert flags & 16
+
+
+def test_row_arrays_are_checked():
+    """Rows narrower than the heads need (though their stride may be wide enough), angles of another
+    type or width: refused before the library is called."""
+    import torch
+    shape = fa.Shape(1, 4, 2, 64)
+    pages = torch.zeros((1, 3, 2, 16, 64), dtype=torch.bfloat16)
+    cache = fa.PagedCache(shape, 3, 16, fa.BF16, keys=pages, values=pages.clone())
+
+    class Batch:
+        _ref = None
+
+        def covers(self, *tensors):
+            pass
+
+    batch = Batch()
+    qkv, q = torch.zeros((2, 512)), torch.zeros((2, 256))
+    narrow_qkv, narrow = torch.zeros((2, 600))[:, :511], torch.zeros((2, 600))[:, :255]
+    angles = torch.zeros((2, 64))
+    bad = [
+        lambda: cache.attend(0, batch, narrow, q),
+        lambda: cache.attend(0, batch, q, narrow),
+        lambda: cache.attend(0, batch, q.view(2, 4, 64), q),
+        lambda: cache.attention(0, batch, narrow_qkv, q, angles),
+        lambda: cache.attention(0, batch, qkv, narrow, angles),
+        lambda: cache.attention(0, batch, qkv, q, angles.bfloat16()),
+        lambda: cache.attention(0, batch, qkv, q, angles[:, :32]),
+        lambda: cache.attention(0, batch, qkv, q, torch.zeros((2, 128))[:, :64]),
+        lambda: cache.attention_input(0, batch, narrow_qkv, angles),
+        lambda: cache.attention_input(0, batch, qkv, angles, q_out=narrow),
+        lambda: cache.attention_input(0, batch, qkv, angles.double()),
+    ]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
