@@ -17,12 +17,12 @@
 //     to their places; 8-bit pages through registers, a tile's bytes loaded while the one before
 //     it is converted to f16;
 //   one warp: TMEM and the MMA issue (one thread).
-// 8-bit pages are dequantised to f16 (2^-12 of the value, an eighth of bf16's rounding) with each
+// 8-bit pages are dequantised to f16 (2^-11 of the value, an eighth of bf16's rounding) with each
 // tile's scales divided by a power of two, 2^k for the keys and 2^v for the values, that takes the
 // largest to [2^8, 2^9): none overflows, and one keeps f16's precision down to 2^-22 of its tile's
-// largest. 2^k multiplies the tile's scores (with the softmax's scale), v is
-// added to their base-2 exponents, so that the probabilities carry 2^v and the outputs of all
-// tiles stay in one unit; the row's sum takes 2^-v back out. A per-key multiplication of the
+// largest (values below 2^-47 keep less, see `exponent`). 2^k multiplies the tile's scores (with the
+// softmax's scale), v is added to their base-2 exponents, so that the probabilities carry 2^v and
+// the outputs of all tiles stay in one unit; the row's sum takes 2^-v back out. A per-key multiplication of the
 // scores and of the probabilities instead (exact integers in the products) costs every softmax
 // thread 64 16-byte shared loads a tile. Probabilities are f16 too, up to 2^15 (the maximum is
 // lazy by 2^8, and 2^7 are added for f16's small end). A word's bytes come out as 0, 2, 1, 3
@@ -39,6 +39,12 @@
 // tiles, where some rows see a key and others do not, a value that is not finite would reach all
 // of them (0 x inf): the loaders take it out and mark its key, and the rows that see the key get
 // a NaN sum. Every wait is bounded (mbar_wait).
+//
+// Measured: 2048 rows after 14336 positions, 32/8 heads of 128 (515 GFLOP): 0.563 ms over bf16 pages
+// (916 TFLOP/s, the softmax and the handshakes between the roles), 0.758 ms over 8-bit pages (680
+// TFLOP/s: the conversion next to it; 56 % of the shared memory's bandwidth, tensor pipe 31 %). Five
+// chunks of 100 to 999 rows under a window of 1024, 8/2 heads of 256: 98 us, shares of about 12
+// tiles a CTA whose fixed costs (plan 6-9 thousand cycles, queries 4-16, merge 20) weigh as much.
 #pragma once
 
 #include "fa_decode.cuh"
