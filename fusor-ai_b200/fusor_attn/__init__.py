@@ -598,7 +598,7 @@ def normalize_and_rotate(heads: int, head_dim: int, qkv, out, norm: int = NORM_R
 _ROWS_DTYPES = {}
 
 
-def _rows_dtype(t, what, width=0):
+def _rows_dtype(t, what):
     if not _ROWS_DTYPES:
         import torch
         _ROWS_DTYPES.update({torch.float32: F32, torch.bfloat16: BF16})
@@ -607,9 +607,21 @@ def _rows_dtype(t, what, width=0):
         raise ValueError(f"{what} of {t.dtype}: float32 or bfloat16")
     if t.dim() == 0 or (t.stride(-1) != 1 and t.shape[-1] > 1):
         raise ValueError(f"{what} with unit stride along a row")
-    if width and (t.dim() != 2 or t.shape[1] < width):
-        raise ValueError(f"{what} of {tuple(t.shape)}: rows of {width} elements")
     return dt
+
+
+def _row_array(t, what, width):
+    """Rows of `width` elements at least: their address, the elements between them, their dtype."""
+    dt = _ROWS_DTYPES.get(t.dtype)
+    if dt is None:
+        dt = _rows_dtype(t, what)
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[1] < width:
+        raise ValueError(f"{what} of {tuple(shape)}: rows of {width} elements")
+    if stride[1] != 1 and shape[1] > 1:
+        raise ValueError(f"{what} with unit stride along a row")
+    # (torch leaves the stride of a single row open)
+    return t.data_ptr(), stride[0] if shape[0] > 1 else max(stride[0], shape[1]), dt
 
 
 def _angles(t, head_dim):
@@ -619,14 +631,7 @@ def _angles(t, head_dim):
     import torch
     if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != head_dim or not t.is_contiguous():
         raise ValueError(f"angles: contiguous float32 rows of {head_dim}")
-    return C.c_void_p(t.data_ptr())
-
-
-def _stride0(t):
-    """Elements between rows (of a single row: its width, as torch leaves its stride open)."""
-    if t.shape[0] > 1:
-        return t.stride(0)
-    return max(t.stride(0), t.numel(), t.shape[-1])
+    return t.data_ptr()
 
 
 class PagedCache:
@@ -667,29 +672,33 @@ class PagedCache:
                               key_scales.data_ptr() if dtype == Q8 else None,
                               value_scales.data_ptr() if dtype == Q8 else None)
         self._ref = C.byref(self._c)
+        self._width, self._kv = shape.width, (shape.kv_heads, shape.head_dim)
         self._qkv_width = (shape.heads + 2 * shape.kv_heads) * shape.head_dim
 
     def attention_input(self, layer: int, batch: "PagedBatch", qkv, angles=None,
                         rope: int = ROPE_HALF, norm=None, q_out=None, stream=None):
         """RoPE (+ head norm) and keep of the batch's rows into their pages (layer.rs:175-234)."""
         batch.covers(qkv, q_out, angles)
-        dt = _rows_dtype(qkv, "qkv", self._qkv_width)
-        if q_out is not None and _rows_dtype(q_out, "q_out", self.shape.width) != dt:
+        src, stride, dt = _row_array(qkv, "qkv", self._qkv_width)
+        dst, q_stride, q_dt = (None, 0, dt) if q_out is None else _row_array(
+            q_out, "q_out", self._width)
+        if q_dt != dt:
             raise ValueError("q_out has qkv's dtype")
         _check(lib().fa_attention_input_paged(
             self._ref, layer, batch._ref, rope if angles is not None else ROPE_NONE,
-            _angles(angles, self.shape.head_dim), _norm(norm), _dptr(qkv), _stride0(qkv), dt, _dptr(q_out),
-            0 if q_out is None else _stride0(q_out), _stream_of(self.device, stream)))
+            _angles(angles, self.shape.head_dim), _norm(norm), src, stride, dt, dst, q_stride,
+            _stream_of(self.device, stream)))
 
     def _rows(self, batch, keys, values):
         batch.covers(keys, values)
         dt = _rows_dtype(keys, "keys")
-        want = (self.shape.kv_heads, self.shape.head_dim)
-        if keys.shape != values.shape or keys.dtype != values.dtype or tuple(keys.shape[1:]) != want:
-            raise ValueError(f"keys and values of one shape (rows, {want[0]}, {want[1]}) and dtype")
-        if keys.stride() != values.stride():
+        shape, stride = keys.shape, keys.stride()
+        if shape != values.shape or keys.dtype != values.dtype or tuple(shape[1:]) != self._kv:
+            raise ValueError(f"keys and values of one shape (rows, {self._kv[0]}, {self._kv[1]}) "
+                             "and dtype")
+        if stride != values.stride():
             raise ValueError("keys and values with the same strides")
-        return _PagedRows(keys.data_ptr(), values.data_ptr(), keys.stride(0), keys.stride(1), dt)
+        return _PagedRows(keys.data_ptr(), values.data_ptr(), stride[0], stride[1], dt)
 
     def write(self, layer: int, batch: "PagedBatch", keys, values, stream=None):
         """Key and value rows (rows, kv_heads, head_dim) into the batch's pages as they are."""
@@ -707,9 +716,8 @@ class PagedCache:
         """KvCache::attend (transformer.rs:182-219) of rotated queries over the pages."""
         batch.covers(q, out)
         _check(lib().fa_attend_paged(
-            self._ref, layer, batch._ref, _dptr(q), _stride0(q),
-            _rows_dtype(q, "q", self.shape.width), _dptr(out), _stride0(out), _rows_dtype(out, "out", self.shape.width),
-            _stream_of(self.device, stream)))
+            self._ref, layer, batch._ref, *_row_array(q, "q", self._width),
+            *_row_array(out, "out", self._width), _stream_of(self.device, stream)))
 
     def attention(self, layer: int, batch: "PagedBatch", qkv, out, angles=None,
                   rope: int = ROPE_HALF, norm=None, stream=None):
@@ -717,8 +725,9 @@ class PagedCache:
         batch.covers(qkv, out, angles)
         _check(lib().fa_attention_paged(
             self._ref, layer, batch._ref, rope if angles is not None else ROPE_NONE,
-            _angles(angles, self.shape.head_dim), _norm(norm), _dptr(qkv), _stride0(qkv), _rows_dtype(qkv, "qkv", self._qkv_width),
-            _dptr(out), _stride0(out), _rows_dtype(out, "out", self.shape.width), _stream_of(self.device, stream)))
+            _angles(angles, self.shape.head_dim), _norm(norm),
+            *_row_array(qkv, "qkv", self._qkv_width), *_row_array(out, "out", self._width),
+            _stream_of(self.device, stream)))
 
 
 class PagedBatch:
