@@ -19,7 +19,7 @@ namespace {
 constexpr int kRowWarps = 4;
 
 // Row r's place: its page and slot, or false (with the error word set) if the batch's numbers are
-// out of range. Rows past the last sequence's are left alone. One warp; two trips to memory (three
+// out of range. Rows before the first sequence's and past the last's are left alone. One warp; two trips to memory (three
 // for more than 32 sequences): the row's sequence s is the number of sequences that end at or
 // before it (row_starts rises, or the span check refuses what is found), and each lane has its
 // sequence's span at hand when s is known.
@@ -47,7 +47,8 @@ __device__ __forceinline__ bool place_of(const PagedSpans& b, const PagedPool& p
   PagedSpan span;
   const bool ok = in < 32 && paged_span_of(b, pool.page_shift, r0, r1, first, &span);
   if (!ok || r < span.row0 || r >= span.row0 + span.n) {
-    if (lane == 0) atomicOr(err, kErrPagedSpan);
+    // (rows before the first sequence's are padding too)
+    if (lane == 0 && !(ok && s == 0 && r < span.row0)) atomicOr(err, kErrPagedSpan);
     return false;
   }
   const int pos = span.first + (r - span.row0);

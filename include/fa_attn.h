@@ -451,10 +451,10 @@ typedef struct {
  * rows in all) one after the other, sequence s's rows row_starts[s] .. row_starts[s + 1] of the
  * call's arrays at the positions from firsts[s] on; its position p lies in slot p % page_size of
  * the page tables[s * table_stride + p / page_size]. The numbers are DEVICE memory, read by the
- * kernels, so a captured call follows them when it is replayed (the host's part of a call depends on
- * rows, max_rows and the mask alone). A sequence may have no rows; rows of the arrays past
- * row_starts[sequences] are padding and left as they are. The mask is FA_MASK_CAUSAL,
- * FA_MASK_WINDOW or FA_MASK_FULL (every position up to the sequence's last new row).
+ * kernels, so a captured call follows them when it is replayed (the host's part of a call depends
+ * on rows, max_rows and the mask alone). A sequence may have no rows; rows of the arrays before
+ * row_starts[0] and past row_starts[sequences] are padding and left as they are. The mask is
+ * FA_MASK_CAUSAL, FA_MASK_WINDOW or FA_MASK_FULL (every position up to the sequence's last new row).
  * Numbers out of range (rows outside the call's, more of them than max_rows, positions past
  * table_width pages, page ids outside the pool) fault nothing: such a sequence is left out of the
  * call, a position on such a page is not written and not seen, and fa_device_status returns

@@ -749,6 +749,35 @@ def test_more_rows_than_max_rows_are_left_out():
         assert (out[1:] == 5.0).all() and (out[0] != 5.0).all()
 
 
+@pytest.mark.parametrize("sp", BOTH, ids=["tokens", "chunks"])
+@pytest.mark.parametrize("dtype", [fa.Q8, fa.BF16], ids=["q8", "bf16"])
+def test_rows_before_the_first_sequence_are_padding(sp, dtype):
+    torch = torch_()
+    shape = fa.Shape(1, 8, 2, 128)
+    spans = Spans(sp, 16)
+    lead = 3
+    n, kv = spans.rows, (2, 128)
+    qkv = torch.randn((lead + n, 12 * 128), device="cuda").bfloat16()
+    outs, rows = [], []
+    for at in (0, lead):
+        cache = make_cache(shape, spans, dtype)
+        batch = fa.PagedBatch(cache, spans.row_starts + at, spans.firsts, spans.tables, at + n,
+                              spans.max_rows)
+        batch.check()
+        x = qkv[lead - at:]
+        out = torch.full((at + n, shape.width), 5.0, device="cuda", dtype=torch.bfloat16)
+        k = torch.full((at + n, *kv), 6.0, device="cuda")
+        v = torch.full((at + n, *kv), 7.0, device="cuda")
+        cache.attention(0, batch, x, out)
+        cache.read(0, batch, k, v)
+        fa.device_status()
+        assert (out[:at] == 5.0).all() and (k[:at] == 6.0).all() and (v[:at] == 7.0).all()
+        outs.append(out[at:])
+        rows.append((k[at:], v[at:]))
+    assert torch.equal(*outs)
+    assert all(torch.equal(a, b) for a, b in zip(*rows))
+
+
 def test_empty_batches():
     torch = torch_()
     shape = fa.Shape(1, 4, 2, 64)
