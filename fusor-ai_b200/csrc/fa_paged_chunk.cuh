@@ -422,11 +422,14 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
   if (!idle) {
     const ChunkWalk& walk = walks[warp];
     const ChunkPiece& pc = pieces[warp];
-    // the warp's next piece (the whole warp, except the MMA issuer's one thread)
+    // The warp's next piece (the whole warp, except the MMA issuer's one thread). A shuffle orders no
+    // memory: the barriers keep lane 0's writes after the others' reads of the piece before, and
+    // before their reads of this one.
     auto next_piece = [&]() {
       __syncwarp();
       int more = 0;
       if (lane == 0) more = chunk_next<D, Q8>(a, spans, &walks[warp], &pieces[warp]);
+      __syncwarp();
       return __shfl_sync(0xffffffffu, more, 0) != 0;
     };
     if (warp >= kMmaWarp) {
@@ -1007,7 +1010,9 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
             if (last) *counter = 0;
           }
           if (__shfl_sync(0xffffffffu, last, 0) == 0) break;
+          // (lane 0 saw the other pieces' arrivals; the whole warp reads what they left)
           __threadfence();
+          __syncwarp();
           l_sum = 0.0f;
 #pragma unroll 4
           for (int z = c0; z <= c1; ++z) mm = fmaxf(mm, __ldcg(a.part_ml + (slot_of(z) * 128 + p) * 2));

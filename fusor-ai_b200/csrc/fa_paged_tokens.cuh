@@ -870,10 +870,10 @@ __global__ void __launch_bounds__(kTokThreads, (TokShape<D, Q8, NT>::kCtas))
         const int before_me = atomicAdd(&a.counters[c0], 1);
         arrived = before_me == pieces - 1;
         if (arrived) a.counters[c0] = 0;
+        __threadfence();  // (the other pieces' arrivals, before the whole CTA reads what they left)
       }
       __syncthreads();
       if (arrived) {
-        __threadfence();
         token_merge<D>(a, cw.row0, cw.h, cols, c0, pieces);
       }
     }
