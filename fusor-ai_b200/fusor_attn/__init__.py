@@ -218,13 +218,48 @@ def _stream(stream=None):
     return C.c_void_p(stream.cuda_stream)
 
 
-def _stream_of(device, stream=None):
-    """`stream`, or torch's current stream of `device` (which need not be the current device)."""
+def _raw_stream(device, stream=None):
+    """The handle of `stream`, or of torch's current stream of `device` (which need not be the
+    current device)."""
     import torch
     if stream is not None:
-        return C.c_void_p(stream.cuda_stream)
+        return stream.cuda_stream
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return C.c_void_p(raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream)
+    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
+
+
+class _Owned:
+    """Tensors that a handle allocates (and fills) on torch's current stream of `device`, for calls on
+    any stream: one that has not used them yet waits for what was queued when they were made, and
+    the allocator keeps their memory until its calls are done. (A capturing stream cannot wait for
+    work outside its capture; torch.cuda.graph waits for the whole device before it begins.)"""
+
+    def __init__(self, device, *tensors):
+        import torch
+        self.tensors = tensors
+        home = torch.cuda.current_stream(device)
+        self.streams = {home.cuda_stream}
+        self.made = None
+        with torch.cuda.stream(home):
+            if not torch.cuda.is_current_stream_capturing():
+                self.made = home.record_event()
+
+    def on(self, device, raw, stream):
+        if raw in self.streams:
+            return
+        import torch
+        if stream is None:
+            stream = torch.cuda.current_stream(device)
+        elif not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(raw, device)
+        with torch.cuda.stream(stream):
+            if torch.cuda.is_current_stream_capturing():
+                return
+        if self.made is not None:
+            stream.wait_event(self.made)
+        for t in self.tensors:
+            t.record_stream(stream)
+        self.streams.add(raw)
 
 
 def _dptr(t):
@@ -646,6 +681,7 @@ class PagedCache:
         if dtype not in (BF16, Q8):
             raise FaError(ERR_UNSUPPORTED, f"pages of dtype {dtype}: BF16 or Q8")
         self.shape, self.pages, self.page_size, self.dtype = shape, pages, page_size, dtype
+        self._own = None
         dims = (shape.layers, pages, shape.kv_heads, page_size, shape.head_dim)
         elem = torch.int8 if dtype == Q8 else torch.bfloat16
         if keys is None:
@@ -654,9 +690,12 @@ class PagedCache:
             where = torch.device("cuda", device)
             keys = torch.zeros(dims, dtype=elem, device=where)
             values = torch.zeros(dims, dtype=elem, device=where)
+            mine = [keys, values]
             if dtype == Q8:
                 key_scales = torch.zeros(dims[:-1], device=where)
                 value_scales = torch.zeros(dims[:-1], device=where)
+                mine += [key_scales, value_scales]
+            self._own = _Owned(device, *mine)
         given = [(keys, dims, elem), (values, dims, elem)]
         if dtype == Q8:
             given += [(key_scales, dims[:-1], torch.float32), (value_scales, dims[:-1], torch.float32)]
@@ -675,6 +714,15 @@ class PagedCache:
         self._width, self._kv = shape.width, (shape.kv_heads, shape.head_dim)
         self._qkv_width = (shape.heads + 2 * shape.kv_heads) * shape.head_dim
 
+    def _on(self, stream, *owned):
+        """The handle of a call's stream, what the call's handles allocated ready for it."""
+        raw = _raw_stream(self.device, stream)
+        if self._own is not None:
+            self._own.on(self.device, raw, stream)
+        for own in owned:
+            own.on(self.device, raw, stream)
+        return C.c_void_p(raw)
+
     def attention_input(self, layer: int, batch: "PagedBatch", qkv, angles=None,
                         rope: int = ROPE_HALF, norm=None, q_out=None, stream=None):
         """RoPE (+ head norm) and keep of the batch's rows into their pages (layer.rs:175-234)."""
@@ -687,7 +735,7 @@ class PagedCache:
         _check(lib().fa_attention_input_paged(
             self._ref, layer, batch._ref, rope if angles is not None else ROPE_NONE,
             _angles(angles, self.shape.head_dim), _norm(norm), src, stride, dt, dst, q_stride,
-            _stream_of(self.device, stream)))
+            self._on(stream)))
 
     def _rows(self, batch, keys, values):
         batch.covers(keys, values)
@@ -704,20 +752,20 @@ class PagedCache:
         """Key and value rows (rows, kv_heads, head_dim) into the batch's pages as they are."""
         r = self._rows(batch, keys, values)
         _check(lib().fa_paged_write(self._ref, layer, batch._ref, C.byref(r),
-                                    _stream_of(self.device, stream)))
+                                    self._on(stream)))
 
     def read(self, layer: int, batch: "PagedBatch", keys, values, stream=None):
         """The batch's rows read back into keys and values (rows, kv_heads, head_dim)."""
         r = self._rows(batch, keys, values)
         _check(lib().fa_paged_read(self._ref, layer, batch._ref, C.byref(r),
-                                   _stream_of(self.device, stream)))
+                                   self._on(stream)))
 
     def attend(self, layer: int, batch: "PagedBatch", q, out, stream=None):
         """KvCache::attend (transformer.rs:182-219) of rotated queries over the pages."""
         batch.covers(q, out)
         _check(lib().fa_attend_paged(
             self._ref, layer, batch._ref, *_row_array(q, "q", self._width),
-            *_row_array(out, "out", self._width), _stream_of(self.device, stream)))
+            *_row_array(out, "out", self._width), self._on(stream, batch._own)))
 
     def attention(self, layer: int, batch: "PagedBatch", qkv, out, angles=None,
                   rope: int = ROPE_HALF, norm=None, stream=None):
@@ -727,14 +775,15 @@ class PagedCache:
             self._ref, layer, batch._ref, rope if angles is not None else ROPE_NONE,
             _angles(angles, self.shape.head_dim), _norm(norm),
             *_row_array(qkv, "qkv", self._qkv_width), *_row_array(out, "out", self._width),
-            _stream_of(self.device, stream)))
+            self._on(stream, batch._own)))
 
 
 class PagedBatch:
     """The spans of calls over a paged cache (fa_paged_batch): row_starts (sequences + 1), firsts
     (sequences) and tables (sequences x table pages) as int32 device tensors, which the kernels
     read when they run; `rows` rows in the call's arrays, at most `max_rows` of them a sequence's.
-    It owns the attention's workspace: batches that may run at the same time are separate ones."""
+    It owns the attention's workspace: batches that may run at the same time are separate ones, and
+    a captured call's batch is kept as long as its graph."""
 
     def __init__(self, cache: PagedCache, row_starts, firsts, tables, rows: int, max_rows: int,
                  mask: Mask = Mask(MASK_CAUSAL)):
@@ -753,6 +802,7 @@ class PagedBatch:
         where = torch.device("cuda", cache.device)
         self.workspace = torch.empty(nbytes.value, dtype=torch.uint8, device=where)
         self.workspace[:PAGED_COUNTER_BYTES].zero_()
+        self._own = _Owned(cache.device, self.workspace)
         stride = tables.stride(0) if n > 1 else tables.shape[1]
         self._c = _PagedBatch(n, rows, max_rows, tables.shape[1], stride, row_starts.data_ptr(),
                               firsts.data_ptr(), tables.data_ptr(), mask.kind, mask.window,
