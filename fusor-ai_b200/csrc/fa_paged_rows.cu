@@ -18,13 +18,16 @@ namespace {
 
 constexpr int kRowWarps = 4;
 
-// Row r's place: its page and slot, or false (with the error word set) if the batch's numbers are
-// out of range. Rows before the first sequence's and past the last's are left alone. One warp; two trips to memory (three
+// Row r's place: its page and slot. kNoRow if no sequence holds the row (rows before the first
+// sequence's and past the last's are padding) or its span is out of range, kNoPage if its page is;
+// what is out of range is set in the error word. One warp; two trips to memory (three
 // for more than 32 sequences): the row's sequence s is the number of sequences that end at or
 // before it (row_starts rises, or the span check refuses what is found), and each lane has its
 // sequence's span at hand when s is known.
-__device__ __forceinline__ bool place_of(const PagedSpans& b, const PagedPool& pool, int r,
-                                         int lane, int* page, int* slot, unsigned* err) {
+constexpr int kNoRow = 0, kNoPage = 1, kPlaced = 2;
+
+__device__ __forceinline__ int place_of(const PagedSpans& b, const PagedPool& pool, int r,
+                                        int lane, int* page, int* slot, unsigned* err) {
   int base = 0;
   if (b.sequences > 32) {
     const int at = (lane + 1) * 32;  // the end of block `lane` of 32 sequences
@@ -40,25 +43,24 @@ __device__ __forceinline__ bool place_of(const PagedSpans& b, const PagedPool& p
   }
   const int in = __popc(__ballot_sync(0xffffffffu, mine < b.sequences && r1 <= r));
   const int s = base + in;
-  if (s >= b.sequences) return false;
+  if (s >= b.sequences) return kNoRow;
   r0 = __shfl_sync(0xffffffffu, r0, in & 31);
   r1 = __shfl_sync(0xffffffffu, r1, in & 31);
   first = __shfl_sync(0xffffffffu, first, in & 31);
   PagedSpan span;
   const bool ok = in < 32 && paged_span_of(b, pool.page_shift, r0, r1, first, &span);
   if (!ok || r < span.row0 || r >= span.row0 + span.n) {
-    // (rows before the first sequence's are padding too)
     if (lane == 0 && !(ok && s == 0 && r < span.row0)) atomicOr(err, kErrPagedSpan);
-    return false;
+    return kNoRow;
   }
   const int pos = span.first + (r - span.row0);
   *page = b.tables[int64_t(s) * b.table_stride + (pos >> pool.page_shift)];
   *slot = pos & ((1 << pool.page_shift) - 1);
   if (!paged_page_ok(*page, pool.pages)) {
     if (lane == 0) atomicOr(err, kErrPagedPage);
-    return false;
+    return kNoPage;
   }
-  return true;
+  return kPlaced;
 }
 
 // Four consecutive elements: one load where the row is aligned for it.
@@ -168,7 +170,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 12)
     }
   }
   int page, slot;
-  if (!place_of(a.spans, a.pool, r, lane, &page, &slot, a.err)) return;  // the warp's, as one
+  const int place = place_of(a.spans, a.pool, r, lane, &page, &slot, a.err);  // the warp's, as one
+  if (place == kNoRow) return;
   const int64_t row0 = ((int64_t(page) * kvh) << a.pool.page_shift) + slot;  // KV head 0's
   // The steps of one kind: 0 queries, 1 keys, 2 values; `begin` of them all to `end`.
   int t = warp;
@@ -254,6 +257,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 12)
     }
   };
   section(std::integral_constant<int, 0>{}, 0, q_steps);
+  if (place == kNoPage) return;  // (the row's query is rotated all the same: it attends)
   section(std::integral_constant<int, 1>{}, q_steps, q_steps + kv_steps);
   section(std::integral_constant<int, 2>{}, q_steps + kv_steps, steps);
 }
@@ -277,7 +281,8 @@ __global__ void __launch_bounds__(kReadWarps * 32)
   for (int i = 0; i < 2; ++i) {
     const int r = r0 + i * kReadWarps;
     int page = 0, slot = 0;
-    const bool ok = r < a.spans.rows && place_of(a.spans, a.pool, r, lane, &page, &slot, a.err);
+    const bool ok = r < a.spans.rows &&
+                    place_of(a.spans, a.pool, r, lane, &page, &slot, a.err) == kPlaced;
     place[i] = ok ? ((int64_t(page) * a.pool.kv_heads) << a.pool.page_shift) + slot : -1;
   }
   const int vectors = a.pool.kv_heads * kPerHead;

@@ -457,7 +457,8 @@ typedef struct {
  * FA_MASK_CAUSAL, FA_MASK_WINDOW or FA_MASK_FULL (every position up to the sequence's last new row).
  * Numbers out of range (rows outside the call's, more of them than max_rows, positions past
  * table_width pages, page ids outside the pool) fault nothing: such a sequence is left out of the
- * call, a position on such a page is not written and not seen, and fa_device_status returns
+ * call, a position on such a page is not written and not seen (a new row there still has its query
+ * rotated and attends to the positions that are left), and fa_device_status returns
  * FA_ERR_CAPACITY (spans) or FA_ERR_ARG (page ids). fa_paged_check finds them on the host.
  * Pages that a call writes belong to one sequence each. */
 typedef struct {

@@ -1,10 +1,10 @@
 """Calls over the paged cache at the edges of what its interface allows, on the GPU: many pieces to
-a warp, handles made on one stream and used on another, against the formulas in 64 bits. The bounds are those of test_paged_gpu.py.
+a warp, handles made on one stream and used on another, numbers out of range, against the formulas in 64 bits. The bounds are those of test_paged_gpu.py.
 """
 import pytest
 
 import fusor_attn as fa
-from test_paged_gpu import CAUSAL, Spans, make_cache, run_attend, torch_
+from test_paged_gpu import CAUSAL, Spans, angles_of, make_cache, run_attend, torch_
 
 pytestmark = pytest.mark.gpu
 
@@ -123,3 +123,48 @@ def test_a_cache_made_on_a_busy_stream_is_used_on_another(dtype):
     assert torch.equal(back[1], back[0])
     assert all((t == 5).all() for t in other)
     fa.device_status()
+
+
+# ---- numbers out of range ----------------------------------------------------------------------
+
+@pytest.mark.parametrize("sp", [[(1, 300), (2, 79), (1, 20)], [(100, 201), (1, 64), (40, 0)]],
+                         ids=["tokens", "chunks"])
+@pytest.mark.parametrize("dims", DIMS, ids=str)
+@pytest.mark.parametrize("dtype", [fa.Q8, fa.BF16], ids=["q8", "bf16"])
+def test_a_new_rows_own_page_out_of_range(dims, sp, dtype):
+    """attention() where pages of new rows are outside the pool: those rows' own queries attend to
+    the positions that are left, whatever the workspace held before, and nothing of them is kept."""
+    torch = torch_()
+    shape = fa.Shape(1, *dims)
+    spans = Spans(sp, 16)
+    cache = make_cache(shape, spans, dtype)
+    # (the call's own queries are kept in f32 over 8-bit pages, in bf16 over bf16 pages)
+    kind = torch.float32 if dtype == fa.Q8 else torch.bfloat16
+    qkv = torch.randn((spans.rows, shape.qkv), device="cuda").to(kind)
+    angles = angles_of(spans, dims[2])
+    q = torch.empty((spans.rows, shape.width), device="cuda", dtype=kind)
+    cache.attention_input(0, spans.batch(cache), qkv, angles, q_out=q)
+    fa.device_status()
+    good = spans.tables.clone()
+    for seq, page, bad in ((0, sp[0][1] // 16 + (sp[0][0] > 1), -1), (1, sp[1][1] // 16, spans.pages)):
+        spans.tables.copy_(good)
+        spans.tables[seq, page] = bad
+        batch = spans.batch(cache)
+        batch.workspace[fa.PAGED_COUNTER_BYTES:] = 0xFF  # NaN, in f32 and in bf16
+        held = [t.clone() for t in (cache.keys, cache.values)]
+        got_q = torch.full_like(q, 7.0)
+        cache.attention_input(0, batch, qkv, angles, q_out=got_q)
+        with pytest.raises(fa.FaError) as e:
+            fa.device_status()
+        assert e.value.code == fa.ERR_ARG
+        assert torch.equal(got_q, q)
+        out = torch.full((spans.rows, shape.width), 5.0, device="cuda")
+        want = torch.full_like(out, 6.0)
+        cache.attention(0, batch, qkv, out, angles)
+        cache.attend(0, batch, q, want)
+        with pytest.raises(fa.FaError):
+            fa.device_status()
+        assert torch.isfinite(out).all() and torch.equal(out, want)
+        page_id = int(good[seq, page])  # the page that the table named before: not written
+        for t, old in zip((cache.keys, cache.values), held):
+            assert torch.equal(t[0, page_id], old[0, page_id])
