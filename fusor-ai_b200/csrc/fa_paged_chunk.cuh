@@ -19,13 +19,14 @@
 //   one warp: TMEM and the MMA issue (one thread).
 // 8-bit pages are dequantised to f16 (2^-11 of the value, an eighth of bf16's rounding) with each
 // tile's scales divided by a power of two, 2^k for the keys and 2^v for the values, that takes the
-// largest to [2^8, 2^9): none overflows, and one keeps f16's precision down to 2^-22 of its tile's
-// largest (values below 2^-47 keep less, see `exponent`). 2^k multiplies the tile's scores (with the
-// softmax's scale), v is added to their base-2 exponents, so that the probabilities carry 2^v and
-// the outputs of all tiles stay in one unit; the row's sum takes 2^-v back out. A per-key multiplication of the
-// scores and of the probabilities instead (exact integers in the products) costs every softmax
-// thread 64 16-byte shared loads a tile. Probabilities are f16 too, up to 2^15 (the maximum is
-// lazy by 2^8, and 2^7 are added for f16's small end). A word's bytes come out as 0, 2, 1, 3
+// largest to [2^8, 2^9): none overflows. 2^k multiplies the tile's scores (with the softmax's scale),
+// v is added to their base-2 exponents, so that the probabilities carry 2^v and the outputs of all
+// tiles stay in one unit; the row's sum takes 2^-v back out. Where a tile's scales lie more than 2^8
+// apart, each of its keys has a k, or a v, of its own: in the unit of a far larger one f16 would lose
+// it (all of it from 2^-33 on), for rows too that do not see the large one or give it no weight.
+// (Per-key multiplications of scores and probabilities in every tile would cost every softmax thread
+// 64 16-byte shared loads a tile.) Probabilities are f16 too, up to 2^15 (the maximum is lazy by 2^8,
+// and 2^7 are added for f16's small end). A word's bytes come out as 0, 2, 1, 3
 // (two pairs without a byte permutation): Q's rows and the output's columns follow that order.
 //
 // A tile's scores are one product of 128 keys (of 64, the tensor core takes as long for each MMA:
@@ -289,9 +290,11 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
   __shared__ uint32_t poison[2][BN / 32];  // by V stage: keys with a value that is not finite
   // by tile % 4 (a tile's keys may arrive while a softmax group is still at the tile two before
   // it, never three: its scores wait for that group's products): a bit per 16 keys whose page is
-  // out of range, and 8-bit pages' 2^k, v and 2^-v
+  // out of range, and 8-bit pages' 2^k, v and 2^-v (2^k or 2^-v negative: each key has its own k or v)
   __shared__ uint32_t absent[4];
-  __shared__ float4 units[4];
+  __shared__ float k_units[4];
+  __shared__ float2 v_units[4];
+  __shared__ signed char own_k[4][Q8 ? BN : 1], own_v[4][Q8 ? BN : 1];
   __shared__ float q_down[Q8 ? NQ * 128 : 1];  // 8-bit pages: what a query row was scaled by, back
   __shared__ int3 spans[kMaxPagedSequences];   // row0, rows (0: none of this kernel's), first position
   unsigned char* smem = reinterpret_cast<unsigned char*>(
@@ -310,7 +313,8 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
                                                // score buffer
   uint64_t* o_done = p_full + 4;               // [2]: each P.V
   uint64_t* o_final = o_done + 2;              // [2]: a piece's last P.V
-  uint64_t* drained = o_final + 2;
+  uint64_t* v_told = o_final + 2;              // [4]: by tile % 4, 8-bit pages' v_units, own_v
+  uint64_t* drained = v_told + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -329,6 +333,7 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
       mbar_init(&o_done[i], 1);
       mbar_init(&o_final[i], 1);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(&v_told[i], 1);
     mbar_init(drained, 1);
     mbar_fence_init();
   }
@@ -464,7 +469,9 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
                                 kd + uint64_t((db * BN * 128 + koff) >> 4), kIdescQK, k > 0 ? 1u : 0u);
             }
             tc::commit(&s_full[b]);
-            // (and this thread's own arrival, which passes on what the loaders wrote for the softmax)
+            // (and this thread's own arrival, which passes on what the loaders wrote for the softmax;
+            // the tile's values may still be on their way, their units come before them)
+            if constexpr (Q8) ok = ok && mbar_wait(&v_told[(tile + L) & 3], ((tile + L) >> 2) & 1, a.err);
             mbar_arrive(&s_full[b]);
             ++sb;
           };
@@ -662,7 +669,7 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
         constexpr int kKeys = BN / 32;
         const int w4 = warp & 3, r8 = lane & 7, c4 = lane >> 3;
         uint4 raw[kItems];
-        float ks[kKeys], vs[kKeys];  // scales of keys lane, lane + 32, ... (ks: key loaders)
+        float sc[kKeys];  // scales of keys lane, lane + 32, ...
         // item k of the warp: rows 8 rg .. 8 rg + 7, chunks 4 cg .. 4 cg + 3
         auto rg_of = [&](int k) { return kWide == 1 ? 4 * k + w4 : kWide == 2 ? 2 * k + (w4 >> 1) : k; };
         const int cg = kWide == 1 ? 0 : kWide == 2 ? w4 & 1 : w4;
@@ -676,6 +683,7 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
           raw[k] = __ldg(reinterpret_cast<const uint4*>(
               pool + (row_of(rg_of(k) >> 1) + (rg_of(k) & 1) * 8 + r8) * kRB + (cg * 4 + c4) * 16));
         };
+        const float* scales = is_v ? a.pool.value_scales : a.pool.key_scales;
         auto load_scales = [&]() {
 #pragma unroll
           for (int x = 0; x < kKeys; ++x) {
@@ -683,27 +691,23 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
             const int pg = __shfl_sync(0xffffffffu, page, row >> 4);
             const bool there = pg >= 0 && p >= lo && p < hi;
             const int64_t at = ((int64_t(max(pg, 0)) * kvh + pc.h) << shift) + (p & ((1 << shift) - 1));
-            const float v = __ldg(a.pool.value_scales + at);
-            vs[x] = there ? v : 0.0f;
-            if (!is_v) {
-              const float k = __ldg(a.pool.key_scales + at);
-              ks[x] = there ? k : 0.0f;
-            }
+            const float v = __ldg(scales + at);
+            sc[x] = there ? v : 0.0f;
           }
         };
-        // the exponent that takes the largest finite scale to [2^8, 2^9) (127 of it stay in f16), or
-        // 2^least for smaller ones. A row's sum is kept in the unit of its largest values, so the
-        // tiles' units must not lie further apart than f32 reaches: from the values' least, 2^-40,
-        // they do not for scales up to 2^70 (and a value is off by at most 2^-58 more).
-        constexpr int kLeastKeys = -118, kLeastValues = -40;
-        auto exponent = [&](const float (&x)[kKeys], int least) {
-          float top = 0.0f;
-#pragma unroll
-          for (int i = 0; i < kKeys; ++i)
-            top = fmaxf(top, fabsf(x[i]) <= 3.402823466e38f ? fabsf(x[i]) : 0.0f);
-          const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-          return bits == 0 ? 0 : min(max(int(bits >> 23) - 135, least), 112);
+        // The exponent that takes a scale to [2^8, 2^9) (127 of it stay in f16), or 2^least for
+        // smaller ones. A row's sum is kept in the unit of its largest values, so units must not lie
+        // further apart than f32 reaches: from the values' least, 2^-40, they do not for scales up to
+        // 2^70 (and a value is off by at most 2^-58 more).
+        const int least = is_v ? -40 : -118;
+        auto exponent = [&](uint32_t bits) { return min(max(int(bits >> 23) - 135, least), 112); };
+        auto finite_bits = [](float x) {
+          return fabsf(x) <= 3.402823466e38f ? __float_as_uint(fabsf(x)) : 0u;
         };
+        // Whether a scale in the unit of its tile, that is not zero, lies more than 2^8 below the
+        // largest. f16 would then lose what rows are made of that do not see the largest, or give it
+        // no weight: every key gets its own unit.
+        auto far_below = [](float y) { return fabsf(y) < 1.0f && y != 0.0f; };
         auto power = [](int e) { return __uint_as_float(uint32_t(127 + e) << 23); };
         int at = pc.begin, end = pc.end;
         if (more) {
@@ -716,17 +720,38 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
           const int st = stage_of();
           const bool was_edge = edge;
           const uint32_t was_gone = gone;
-          const int ev = exponent(vs, kLeastValues), ek = is_v ? 0 : exponent(ks, kLeastKeys);
+          uint32_t top = 0;
+#pragma unroll
+          for (int x = 0; x < kKeys; ++x) top = max(top, finite_bits(sc[x]));
+          const int e = exponent(__reduce_max_sync(0xffffffffu, top));
           // this tile's scales as f16 pairs
-          const float down = power(is_v ? -ev : -ek);
+          const float down = power(-e);
           __half2 hs[kKeys];
           uint32_t bad = 0;  // keys lane + 32 x whose value scale is not finite
+          bool own = false;
 #pragma unroll
           for (int x = 0; x < kKeys; ++x) {
-            const float sc = is_v ? vs[x] : ks[x];
-            const bool drop = is_v && was_edge && !(fabsf(sc) <= 3.402823466e38f);
+            const bool drop = is_v && was_edge && !(fabsf(sc[x]) <= 3.402823466e38f);
             bad |= uint32_t(drop) << x;
-            hs[x] = __float2half2_rn(drop ? 0.0f : sc * down);
+            const float y = drop ? 0.0f : sc[x] * down;
+            own = own || far_below(y);
+            hs[x] = __float2half2_rn(y);
+          }
+          own = __any_sync(0xffffffffu, own);
+          // (the tile four before this one, whose place the units take, is done with: its products
+          // came before those that made room for the last tile)
+          if (own) {
+#pragma unroll
+            for (int x = 0; x < kKeys; ++x) {
+              const int mine = exponent(finite_bits(sc[x]));
+              if ((warp & 3) == 0) (is_v ? own_v : own_k)[tile & 3][lane + 32 * x] = (signed char)(mine);
+              if (!((bad >> x) & 1u)) hs[x] = __float2half2_rn(sc[x] * power(-mine));
+            }
+          }
+          if (is_v && warp == 4) {
+            if (lane == 0) v_units[tile & 3] = make_float2(float(e), own ? -power(-e) : power(-e));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&v_told[tile & 3]);
           }
           // the tile after this one, of this piece or the next
           if (++at == end) {
@@ -767,7 +792,7 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
           }
           if (!is_v && tid == 0) {
             absent[tile & 3] = was_gone;
-            units[tile & 3] = make_float4(power(ek), float(ev), power(-ev), 0.0f);
+            k_units[tile & 3] = own ? -power(e) : power(e);
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           mbar_arrive(&full[st]);
@@ -832,6 +857,41 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
           const uint32_t buf = (tile + L) & 1;  // one query tile: the score buffer
           const uint32_t s_base = lane_base + (NQ == 2 ? uint32_t(h) * 64 : buf * 64);
           const uint32_t p_base = lane_base + (NQ == 2 ? uint32_t(h) * 32 : buf * 64);
+          // A block's end: the keys that the loaders marked, O to the maximum's new unit, and word to
+          // the issuer. (Once in each of the two paths below: where they join, the common one takes
+          // 30 us longer of 790 for 2048 rows after 14336 positions.)
+          auto finish = [&](float alpha) __attribute__((always_inline)) {
+            if (kp0 + L * BN < lo_all || kp0 + (L + 1) * BN > hi_all) {
+              // an edge tile (of the unit, as the loaders see it): keys that they marked
+              const uint32_t vt = tile + L;
+              const bool v_there = mbar_wait(&v_full[vt % S::kVStages], (vt / S::kVStages) & 1, a.err);
+              if (!__all_sync(0xffffffffu, v_there)) return ok = false;
+              const volatile uint32_t* marks = poison[vt % S::kVStages];
+#pragma unroll
+              for (int w = 0; w < 2; ++w)
+                if (marks[h * 2 + w] & run_word(runs.b0, runs.n0, kp, w)) poisoned = true;
+            }
+            if (__any_sync(0xffffffffu, alpha != 1.0f) && c > 0) {
+              // O holds the products of this piece's earlier tiles, the last of which may still run
+              if (!__all_sync(0xffffffffu, mbar_wait(&o_done[i], (sc - 1) & 1, a.err))) return ok = false;
+              tc::fence_after_sync();
+#pragma unroll 1
+              for (int cc = 0; cc < D / 32; ++cc) {
+                uint32_t o[32];
+                tc::tmem_ld32_wait(o_base + cc * 32, o);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                tc::tmem_st32(o_base + cc * 32, o);
+                tc::tmem_wait_st();
+              }
+            }
+            tc::tmem_wait_st();
+            tc::fence_before_sync();
+            mbar_arrive(&p_full[NQ == 2 ? uint32_t(2 * i + h) : buf]);
+            ++c;
+            ++sc;
+            return true;
+          };
           if (h == 0 || c == 0) {
             // every decision before a whole-warp tcgen05 instruction is made warp-uniform
             const bool there = NQ == 2 ? mbar_wait(&s_full[i], st & 1, a.err)
@@ -840,18 +900,65 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
             ++st;
             tc::fence_after_sync();
           }
+          const uint32_t gone = *const_cast<const volatile uint32_t*>(&absent[(tile + L) & 3]);
+          float alpha = 1.0f;
+          float k_unit = 1.0f;
+          float2 v_unit = make_float2(0.0f, 1.0f);
+          if constexpr (Q8) {
+            k_unit = k_units[(tile + L) & 3];
+            v_unit = v_units[(tile + L) & 3];
+          }
+          uint32_t sreg[64];
+          tc::tmem_ld64_wait(s_base, sreg);
+          if (Q8 && (k_unit < 0.0f || v_unit.y < 0.0f)) {  // (the same for all)
+            // Keys with units of their own: what follows below, 32 keys at a time and twice over (the
+            // maximum first), the scores as base-2 exponents with each key's v in them.
+            const signed char* ks = &own_k[(tile + L) & 3][h * 64];
+            const signed char* vs = &own_v[(tile + L) & 3][h * 64];
+            float top = -INFINITY, sum = 0.0f, less = 0.0f;
+#pragma unroll 1
+            for (int step = 0; step < 4; ++step) {
+              const int k0 = (step & 1) * 32;
+              uint32_t r[32];
+              tc::tmem_ld32_wait(s_base + k0, r);
+              const uint32_t off = gone >> (h * 4 + k0 / 16);
+              const uint32_t in = run_word(runs.b0, runs.n0, kp + k0, 0) &
+                                  ~((off & 1u ? 0xFFFFu : 0u) | (off & 2u ? 0xFFFF0000u : 0u));
+              if (step == 2) {
+                if (top > m_used + 8.0f || (m_used == -INFINITY && top > -INFINITY)) {
+                  if (m_used > -INFINITY) alpha = exp2_approx(m_used - top);
+                  m_used = top;
+                }
+                less = 7.0f - (m_used == -INFINITY ? 0.0f : m_used);
+              }
+#pragma unroll
+              for (int x = 0; x < 32; ++x) {
+                const float unit = k_unit < 0.0f ? __uint_as_float(uint32_t(127 + ks[k0 + x]) << 23) : k_unit;
+                const float v = v_unit.y < 0.0f ? float(vs[k0 + x]) : v_unit.x;
+                float y = fmaf(__uint_as_float(r[x]), fmaxf(scale * unit, 1.175494351e-38f), v);
+                if (!((in >> x) & 1u)) y = -INFINITY;
+                if (step < 2) top = fmaxf(top, y);
+                else sum += exp2_approx(y + (less - v));  // (each key's 2^-v taken back out)
+                r[x] = __float_as_uint(exp2_approx(y + less));
+              }
+              if (step < 2) continue;
+              uint32_t w[16];
+#pragma unroll
+              for (int x = 0; x < 16; ++x) w[x] = pack_f16(__uint_as_float(r[2 * x]), __uint_as_float(r[2 * x + 1]));
+              tc::tmem_st16(p_base + k0 / 2, w);
+            }
+            l_sum = l_sum * alpha + sum;
+            if (!finish(alpha)) break;
+            continue;
+          }
           // the tile's units: its scores' scale, what its exponents and its sum take besides
           float scale_t = scale, up_t = 0.0f, down_t = 1.0f;
           if constexpr (Q8) {
-            const float4 un = units[(tile + L) & 3];
             // (not 0, for a masked score times it would be a NaN)
-            scale_t = fmaxf(scale * un.x, 1.175494351e-38f);
-            up_t = un.y;
-            down_t = un.z;
+            scale_t = fmaxf(scale * k_unit, 1.175494351e-38f);
+            up_t = v_unit.x;
+            down_t = v_unit.y;
           }
-          const uint32_t gone = *const_cast<const volatile uint32_t*>(&absent[(tile + L) & 3]);
-          uint32_t sreg[64];
-          tc::tmem_ld64_wait(s_base, sreg);
           float* s = reinterpret_cast<float*>(sreg);
           const bool all_in = !valid || (kp >= runs.b0 && kp + 64 <= runs.b0 + runs.n0);
           if (!all_in || gone != 0) {
@@ -876,7 +983,6 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
           mx0 = fmax3(mx0, s[60], s[61]);
           mx1 = fmax3(mx1, s[62], s[63]);
           const float m_tile = fmaf(fmax3(mx0, mx1, fmaxf(mx2, mx3)), scale_t, up_t);
-          float alpha = 1.0f;
           if (m_tile > m_used + 8.0f || (m_used == -INFINITY && m_tile > -INFINITY)) {
             if (m_used > -INFINITY) alpha = exp2_approx(m_used - m_tile);
             m_used = m_tile;
@@ -898,35 +1004,7 @@ __global__ void __launch_bounds__((ChunkShape<D, Q8>::kThreads), 1)
           }
           tc::tmem_st32(p_base, *reinterpret_cast<const uint32_t(*)[32]>(&sreg[0]));
           l_sum = l_sum * alpha + ((sum2a.x + sum2a.y) + (sum2b.x + sum2b.y)) * down_t;
-          if (kp0 + L * BN < lo_all || kp0 + (L + 1) * BN > hi_all) {
-            // an edge tile (of the unit, as the loaders see it): keys that they marked
-            const uint32_t vt = tile + L;
-            const bool v_there = mbar_wait(&v_full[vt % S::kVStages], (vt / S::kVStages) & 1, a.err);
-            if (!__all_sync(0xffffffffu, v_there)) { ok = false; break; }
-            const volatile uint32_t* marks = poison[vt % S::kVStages];
-#pragma unroll
-            for (int w = 0; w < 2; ++w)
-              if (marks[h * 2 + w] & run_word(runs.b0, runs.n0, kp, w)) poisoned = true;
-          }
-          if (__any_sync(0xffffffffu, alpha != 1.0f) && c > 0) {
-            // O holds the products of this piece's earlier tiles, the last of which may still run
-            if (!__all_sync(0xffffffffu, mbar_wait(&o_done[i], (sc - 1) & 1, a.err))) { ok = false; break; }
-            tc::fence_after_sync();
-#pragma unroll 1
-            for (int cc = 0; cc < D / 32; ++cc) {
-              uint32_t o[32];
-              tc::tmem_ld32_wait(o_base + cc * 32, o);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              tc::tmem_st32(o_base + cc * 32, o);
-              tc::tmem_wait_st();
-            }
-          }
-          tc::tmem_wait_st();
-          tc::fence_before_sync();
-          mbar_arrive(&p_full[NQ == 2 ? uint32_t(2 * i + h) : buf]);
-          ++c;
-          ++sc;
+          if (!finish(alpha)) break;
         }
         if (!ok) break;
         tile += uint32_t(n_tiles);

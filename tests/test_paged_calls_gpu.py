@@ -1,10 +1,14 @@
 """Calls over the paged cache at the edges of what its interface allows, on the GPU: many pieces to
-a warp, handles made on one stream and used on another, numbers out of range, against the formulas in 64 bits. The bounds are those of test_paged_gpu.py.
+a warp, handles made on one stream and used on another, numbers out of range, 8-bit
+scales far apart, against the formulas in 64 bits. The bounds are those of test_paged_gpu.py.
 """
+import math
+
 import pytest
 
 import fusor_attn as fa
-from test_paged_gpu import CAUSAL, Spans, angles_of, make_cache, run_attend, torch_
+from test_paged_gpu import (CAUSAL, Spans, angles_of, check_close, held, make_cache, reference,
+                            run_attend, torch_, visible)
 
 pytestmark = pytest.mark.gpu
 
@@ -168,3 +172,127 @@ def test_a_new_rows_own_page_out_of_range(dims, sp, dtype):
         page_id = int(good[seq, page])  # the page that the table named before: not written
         for t, old in zip((cache.keys, cache.values), held):
             assert torch.equal(t[0, page_id], old[0, page_id])
+
+
+# ---- 8-bit scales far apart --------------------------------------------------------------------
+
+def eight_bit_reference(cache, spans, q, weighty):
+    """Outputs of one sequence's causal rows in f64 and their bounds: test_paged_gpu.py's, with the
+    scores' errors taken over the keys that a row sees, or (weighty) over those that have a weight
+    in f64, and one more. The weights go into the products in f16, where those below 2^-14 are off by
+    at most 2^-25. The token kernel's weights carry their value's scale s_j and the largest is at
+    least 2^6: each is off by at most 2^-31 of the largest p_j s_j. The chunk kernel's go with values
+    whose scales are put into [2^8, 2^9), the largest of a tile (which here lie within 2^2 of each
+    other, or have units of their own) or each its own: the largest weight is at least 2^7 and its
+    scale at least 2^6, and 2^-25 with a scale of at most 2^9 is 2^-29 of the largest p_j s_j. An
+    element of at most 127 steps is so off by at most 127 x 2^-29 of it for every position."""
+    torch = torch_()
+    (rows, first), = spans.spans
+    end = first + rows
+    heads, kvh, d = cache.shape.heads, cache.shape.kv_heads, cache.shape.head_dim
+    k, v = held(cache, 0, *spans.places(0, 0, end))
+    page, slot = spans.places(0, 0, end)
+    scales = cache.value_scales[0][page, :, slot].double()
+    see = visible(CAUSAL, torch.arange(first, end, device="cuda"), end)
+    want = torch.zeros((rows, heads * d), dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(want)
+    for h in range(heads):
+        cols, kv = slice(h * d, (h + 1) * d), h * kvh // heads
+        qh, kh, vh = q[:, cols].double(), k[:, kv], v[:, kv]
+        p = torch.softmax(torch.where(see, qh @ kh.T / math.sqrt(d), -math.inf), 1)
+        off = (3 * 2.0 ** -11 + 1e-5) * (qh.abs() @ kh.abs().T) + 2.0 ** -14.9 * (
+            qh.abs().amax(1, keepdim=True) @ kh.abs().sum(1)[None])
+        off = torch.where(p > 0 if weighty else see, off / math.sqrt(d), 0.0).amax(1, keepdim=True)
+        want[:, cols] = p @ vh
+        tol[:, cols] = (3 * 2.0 ** -11 + 2 * off + 1e-4) * (p @ vh.abs())
+        tol[:, cols] += end * 127 * 2.0 ** -29 * (p * scales[:, kv]).amax(1, keepdim=True)
+    return want, tol
+
+
+@pytest.mark.parametrize("rows", [2, 60], ids=["token", "chunk"])
+@pytest.mark.parametrize("dims", DIMS, ids=str)
+@pytest.mark.parametrize("what", ["keys", "values", "both"])
+@pytest.mark.parametrize("power", [26, 35])
+def test_a_scale_far_above_its_neighbours(dims, rows, what, power):
+    """One new position's keys or values 2^26 or 2^35 times its neighbours': the rows before it are
+    as precise as without it, whatever tile it shares with their keys."""
+    torch = torch_()
+    shape = fa.Shape(1, *dims)
+    spans = Spans([(rows, 90)], 16)
+    cache = make_cache(shape, spans, fa.Q8)
+    page, slot = spans.places(0, 90 + rows // 2, 91 + rows // 2)
+    if what != "values":
+        cache.key_scales[0, page, :, slot] *= 2.0 ** power
+    if what != "keys":
+        cache.value_scales[0, page, :, slot] *= 2.0 ** power
+    q = torch.randn((rows, shape.width), device="cuda").bfloat16()
+    out = torch.empty((rows, shape.width), device="cuda")
+    cache.attend(0, spans.batch(cache), q, out)
+    fa.device_status()
+    check_close(out, *eight_bit_reference(cache, spans, q, False), False)
+
+
+@pytest.mark.parametrize("rows", [2, 60], ids=["token", "chunk"])
+@pytest.mark.parametrize("dims", DIMS, ids=str)
+@pytest.mark.parametrize("at", [0, 37, 91], ids=str)
+@pytest.mark.parametrize("power", [9, 26, 35, 60])
+def test_a_huge_position_that_no_row_gives_weight(dims, rows, at, power):
+    """A position whose keys and values are far above the others' and whose scores lie far below
+    them (in 64 bits its weights are exactly zero): every row is what the others make it."""
+    torch = torch_()
+    shape = fa.Shape(1, *dims)
+    spans = Spans([(rows, 90)], 16)
+    cache = make_cache(shape, spans, fa.Q8)
+    page, slot = spans.places(0, at, at + 1)
+    cache.keys[0, page, :, slot] = -127  # (queries are positive)
+    cache.key_scales[0, page, :, slot] = 2.0 ** power
+    cache.value_scales[0, page, :, slot] = 2.0 ** power
+    q = torch.rand((rows, shape.width), device="cuda") + 0.5
+    out = torch.empty((rows, shape.width), device="cuda")
+    cache.attend(0, spans.batch(cache), q, out)
+    fa.device_status()
+    check_close(out, *eight_bit_reference(cache, spans, q, True), False)
+
+
+@pytest.mark.parametrize("rows,first", [(2, 3000), (170, 3000), (700, 0)])
+@pytest.mark.parametrize("dims", DIMS, ids=str)
+def test_scales_of_any_size_side_by_side(dims, rows, first):
+    """Every position's scales a power of two of their own, over many tiles and shared among CTAs."""
+    torch = torch_()
+    shape = fa.Shape(1, *dims)
+    spans = Spans([(rows, first)], 64)
+    cache = make_cache(shape, spans, fa.Q8)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for t, lo, hi in ((cache.key_scales, -25, 1), (cache.value_scales, -25, 25)):
+        t *= 2.0 ** torch.randint(lo, hi, t.shape, generator=g, device="cuda")
+    q = torch.randn((rows, shape.width), generator=g, device="cuda").bfloat16()
+    out = torch.empty((rows, shape.width), device="cuda")
+    batch = spans.batch(cache)
+    cache.attend(0, batch, q, out)
+    check_close(out, *eight_bit_reference(cache, spans, q, False), False)
+    again = torch.empty_like(out)
+    cache.attend(0, batch, q, again)
+    fa.device_status()
+    assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("rows", [1, 60], ids=["token", "chunk"])
+@pytest.mark.parametrize("dims", DIMS, ids=str)
+def test_heads_of_zeros_beside_tiny_values(dims, rows):
+    """Blocks of positions whose values are all zero weigh in the sums of rows whose other values are
+    tiny, and take nothing from them."""
+    torch = torch_()
+    shape = fa.Shape(1, *dims)
+    spans = Spans([(rows, 500)], 16)
+    cache = make_cache(shape, spans, fa.Q8)
+    cache.value_scales *= 2.0 ** -30
+    page, slot = spans.places(0, 128, 256)
+    cache.values[0, page, :, slot] = 0
+    cache.value_scales[0, page, :, slot] = 0
+    q = torch.randn((rows, shape.width), device="cuda").bfloat16()
+    out = torch.empty((rows, shape.width), device="cuda")
+    cache.attend(0, spans.batch(cache), q, out)
+    fa.device_status()
+    want, tol = reference(cache, 0, spans, q.double(), CAUSAL)
+    up = 2.0 ** 30  # (values are off by at most 2^-58 besides)
+    check_close(out.double() * up, want * up, tol * up + 2.0 ** -58 * up, False)
