@@ -268,7 +268,8 @@ int write_input(const fa_paged_cache* c, int layer, const fa_paged_batch* b, int
 int attend(const fa_paged_cache* c, int layer, const fa_paged_batch* b, const void* q,
            int64_t q_stride, int dtype, void* out, int64_t out_stride, int out_dtype,
            const Workspace& w, int sms, unsigned* err, cudaStream_t s) {
-  if (b->sequences == 0 || b->rows == 0 || b->max_rows == 0) return FA_OK;
+  // (max_rows 0 is a call like any other: the token kernel reports the sequences that have rows)
+  if (b->sequences == 0 || b->rows == 0) return FA_OK;
   fa::PagedAttendArgs a{};
   a.pool = pool_of(c, layer);
   a.spans = spans_of(b);

@@ -460,6 +460,7 @@ typedef struct {
  * call, a position on such a page is not written and not seen (a new row there still has its query
  * rotated and attends to the positions that are left), and fa_device_status returns
  * FA_ERR_CAPACITY (spans) or FA_ERR_ARG (page ids). fa_paged_check finds them on the host.
+ * (A call of no rows or no sequences launches nothing, and so finds nothing.)
  * Pages that a call writes belong to one sequence each. */
 typedef struct {
   int32_t sequences;

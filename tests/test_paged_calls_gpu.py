@@ -174,6 +174,31 @@ def test_a_new_rows_own_page_out_of_range(dims, sp, dtype):
             assert torch.equal(t[0, page_id], old[0, page_id])
 
 
+@pytest.mark.parametrize("dtype", [fa.Q8, fa.BF16], ids=["q8", "bf16"])
+def test_no_rows_allowed_to_a_sequence(dtype):
+    """max_rows 0: a sequence that has rows all the same is left out and reported, as with any other
+    number; sequences without rows are in order."""
+    torch = torch_()
+    shape = fa.Shape(1, 8, 2, 128)
+    spans = Spans([(1, 10), (30, 5)], 16)
+    cache = make_cache(shape, spans, dtype)
+    qkv = torch.randn((31, shape.qkv), device="cuda")
+    pools = [t.clone() for t in (cache.keys, cache.values)]
+    for call in ("attend", "attention"):
+        out = torch.full((31, shape.width), 5.0, device="cuda")
+        batch = spans.batch(cache, max_rows=0)
+        getattr(cache, call)(0, batch, qkv, out)
+        with pytest.raises(fa.CapacityError):
+            fa.device_status()
+        assert (out == 5.0).all()
+    assert torch.equal(cache.keys, pools[0]) and torch.equal(cache.values, pools[1])
+    empty = Spans([(0, 10), (0, 5)], 16, pad_rows=4)
+    out = torch.full((4, shape.width), 5.0, device="cuda")
+    cache.attend(0, empty.batch(cache, max_rows=0), qkv, out)
+    fa.device_status()
+    assert (out == 5.0).all()
+
+
 # ---- 8-bit scales far apart --------------------------------------------------------------------
 
 def eight_bit_reference(cache, spans, q, weighty):
