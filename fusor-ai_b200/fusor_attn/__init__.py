@@ -127,6 +127,8 @@ class _PagedRows(C.Structure):
 
 PAGED_COUNTER_BYTES = 8192
 
+_timeouts = 0  # seen by device_status: paged batches zero their counters again
+
 _lib = None
 
 # name -> (restype, argtypes) for every entry point of include/fa_attn.h
@@ -228,6 +230,14 @@ def _raw_stream(device, stream=None):
     return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
 
 
+def _stream_object(device, raw, stream):
+    """The torch stream of _raw_stream's handle."""
+    import torch
+    if stream is None:
+        return torch.cuda.current_stream(device)
+    return stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(raw, device)
+
+
 class _Owned:
     """Tensors that a handle allocates (and fills) on torch's current stream of `device`, for calls on
     any stream: one that has not used them yet waits for what was queued when they were made, and
@@ -248,10 +258,7 @@ class _Owned:
         if raw in self.streams:
             return
         import torch
-        if stream is None:
-            stream = torch.cuda.current_stream(device)
-        elif not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(raw, device)
+        stream = _stream_object(device, raw, stream)
         with torch.cuda.stream(stream):
             if torch.cuda.is_current_stream_capturing():
                 return
@@ -714,13 +721,16 @@ class PagedCache:
         self._width, self._kv = shape.width, (shape.kv_heads, shape.head_dim)
         self._qkv_width = (shape.heads + 2 * shape.kv_heads) * shape.head_dim
 
-    def _on(self, stream, *owned):
-        """The handle of a call's stream, what the call's handles allocated ready for it."""
+    def _on(self, stream, batch=None):
+        """The handle of a call's stream, what the call's handles allocated ready for it (an
+        attention call's batch with its workspace)."""
         raw = _raw_stream(self.device, stream)
         if self._own is not None:
             self._own.on(self.device, raw, stream)
-        for own in owned:
-            own.on(self.device, raw, stream)
+        if batch is not None:
+            batch._own.on(self.device, raw, stream)
+            if batch._timeouts != _timeouts:
+                batch.reset(stream)
         return C.c_void_p(raw)
 
     def attention_input(self, layer: int, batch: "PagedBatch", qkv, angles=None,
@@ -765,7 +775,7 @@ class PagedCache:
         batch.covers(q, out)
         _check(lib().fa_attend_paged(
             self._ref, layer, batch._ref, *_row_array(q, "q", self._width),
-            *_row_array(out, "out", self._width), self._on(stream, batch._own)))
+            *_row_array(out, "out", self._width), self._on(stream, batch)))
 
     def attention(self, layer: int, batch: "PagedBatch", qkv, out, angles=None,
                   rope: int = ROPE_HALF, norm=None, stream=None):
@@ -775,7 +785,7 @@ class PagedCache:
             self._ref, layer, batch._ref, rope if angles is not None else ROPE_NONE,
             _angles(angles, self.shape.head_dim), _norm(norm),
             *_row_array(qkv, "qkv", self._qkv_width), *_row_array(out, "out", self._width),
-            self._on(stream, batch._own)))
+            self._on(stream, batch)))
 
 
 class PagedBatch:
@@ -803,11 +813,24 @@ class PagedBatch:
         self.workspace = torch.empty(nbytes.value, dtype=torch.uint8, device=where)
         self.workspace[:PAGED_COUNTER_BYTES].zero_()
         self._own = _Owned(cache.device, self.workspace)
+        self._timeouts = _timeouts
         stride = tables.stride(0) if n > 1 else tables.shape[1]
         self._c = _PagedBatch(n, rows, max_rows, tables.shape[1], stride, row_starts.data_ptr(),
                               firsts.data_ptr(), tables.data_ptr(), mask.kind, mask.window,
                               self.workspace.data_ptr(), nbytes.value)
         self._ref = C.byref(self._c)
+
+    def reset(self, stream=None):
+        """Zeroes the arrival counters on `stream`. After device_status has raised ERR_TIMEOUT (a call
+        that gave up leaves them as they were) a batch's next call does this by itself; the replays
+        of a captured call need it from their caller."""
+        import torch
+        raw = _raw_stream(self.cache.device, stream)
+        self._own.on(self.cache.device, raw, stream)
+        with torch.cuda.stream(_stream_object(self.cache.device, raw, stream)):
+            self.workspace[:PAGED_COUNTER_BYTES].zero_()
+            if not torch.cuda.is_current_stream_capturing():
+                self._timeouts = _timeouts
 
     def covers(self, *tensors):
         for t in tensors:
@@ -905,7 +928,11 @@ class PeerExchange:
 def device_status(stream=None):
     """Raises FaError(ERR_TIMEOUT) if a kernel gave up a device-side wait, CapacityError or
     FaError(ERR_ARG) if a paged call met spans or page ids out of range."""
-    _check(lib().fa_device_status(_stream(stream)))
+    global _timeouts
+    rc = lib().fa_device_status(_stream(stream))
+    if rc == ERR_TIMEOUT:
+        _timeouts += 1
+    _check(rc)
 
 
 def rng_normal(seed: int, n: int) -> np.ndarray:

@@ -129,6 +129,45 @@ def test_a_cache_made_on_a_busy_stream_is_used_on_another(dtype):
     fa.device_status()
 
 
+@pytest.mark.parametrize("dtype", [fa.Q8, fa.BF16], ids=["q8", "bf16"])
+def test_a_batch_after_a_call_that_gave_up(dtype, monkeypatch):
+    """Counters left as they were when a wait gave up (put there by hand, and the status with them):
+    once the status has been seen, a batch's next call starts from zeros, on any stream; replays of
+    a captured call do after a reset."""
+    torch = torch_()
+    spans, cache, batch, q, out = split_run(dtype)
+    got = torch.zeros_like(out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.attend(0, batch, q, got)
+
+    def give_up():
+        torch.cuda.synchronize()
+        batch.workspace[:fa.PAGED_COUNTER_BYTES] = 1
+        got.zero_()
+        with monkeypatch.context() as m:
+            m.setattr(fa.lib(), "fa_device_status", lambda stream: fa.ERR_TIMEOUT)
+            with pytest.raises(fa.FaError) as e:
+                fa.device_status()
+        assert e.value.code == fa.ERR_TIMEOUT
+        torch.cuda.synchronize()
+
+    for stream in (None, torch.cuda.Stream()):
+        give_up()
+        cache.attend(0, batch, q, got, stream=stream)
+        torch.cuda.synchronize()
+        assert torch.equal(got, out)
+    give_up()
+    batch.reset()
+    for _ in range(2):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, out)
+    assert (batch.workspace[:fa.PAGED_COUNTER_BYTES] == 0).all()
+    fa.device_status()
+
+
 # ---- numbers out of range ----------------------------------------------------------------------
 
 @pytest.mark.parametrize("sp", [[(1, 300), (2, 79), (1, 20)], [(100, 201), (1, 64), (40, 0)]],
