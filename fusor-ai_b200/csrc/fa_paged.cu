@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <cstdlib>
 #include <new>
 #include <vector>
 
@@ -403,7 +404,43 @@ int fa_attention_input_paged(const fa_paged_cache* cache, int32_t layer,
 
 namespace {
 
-int check_rows(const fa_paged_cache* c, const fa_paged_batch* b, const fa_paged_rows* r) {
+// Whether a head row of `d` elements at row * row_stride + head * head_stride shares elements with
+// another of the set, or with one of the same set `delta` elements on: whether delta + i row_stride +
+// j head_stride, |i| < rows, |j| < heads, comes within d of 0 (with delta 0, but for i = j = 0).
+bool head_rows_overlap(int64_t delta, int rows, int heads, int64_t row_stride, int64_t head_stride, int d) {
+  if (rows == 1) row_stride = 0;
+  if (delta == 0 && ((heads == 1 || head_stride >= d) &&
+                     (rows == 1 || row_stride >= (heads - 1) * head_stride + d)))
+    return false;  // (heads within rows: no need to look)
+  for (int64_t j = 1 - heads; j < heads; ++j) {
+    const int64_t x = delta + j * head_stride;
+    const int64_t near = row_stride == 0 ? 0 : -x / row_stride;  // (to within one)
+    for (int64_t n = near - 1; n <= near + 1; ++n) {
+      const int64_t i = std::min<int64_t>(std::max<int64_t>(n, 1 - rows), rows - 1);
+      if ((delta != 0 || i != 0 || j != 0) && std::abs(x + i * row_stride) < d) return true;
+    }
+  }
+  return false;
+}
+
+// The rows that a read writes: no element from two of them. (keys and values may be one array, which
+// then holds the values: a thread stores its values after its keys.)
+int check_rows_out(const fa_paged_cache* c, const fa_paged_batch* b, const fa_paged_rows* r) {
+  if (b->rows == 0) return FA_OK;
+  const int64_t most = int64_t(1) << 34;  // (keeps what follows within 64 bits)
+  const int64_t rs = b->rows > 1 ? r->row_stride : 0, hs = c->kv_heads > 1 ? r->head_stride : 0;
+  if (rs > most || hs > most) return fail(FA_ERR_ARG, "strides of %lld and %lld elements", (long long)rs, (long long)hs);
+  const int d = c->head_dim, e = r->dtype == FA_BF16 ? 2 : 4;
+  if (head_rows_overlap(0, b->rows, c->kv_heads, rs, hs, d))
+    return fail(FA_ERR_ARG, "rows %lld apart with heads %lld apart overlap", (long long)rs, (long long)hs);
+  const int64_t apart = (reinterpret_cast<intptr_t>(r->values) - reinterpret_cast<intptr_t>(r->keys)) / e;
+  if (apart != 0 && std::abs(apart) < (b->rows - 1) * rs + (c->kv_heads - 1) * hs + d &&
+      head_rows_overlap(apart, b->rows, c->kv_heads, rs, hs, d))
+    return fail(FA_ERR_ARG, "keys and values overlap");
+  return FA_OK;
+}
+
+int check_rows(const fa_paged_cache* c, const fa_paged_batch* b, const fa_paged_rows* r, bool written) {
   if (r == nullptr) return fail(FA_ERR_ARG, "null rows");
   FA_TRY(check_rows_dtype(r->dtype, "rows"));
   if (b->rows > 0 && (r->keys == nullptr || r->values == nullptr))
@@ -412,6 +449,7 @@ int check_rows(const fa_paged_cache* c, const fa_paged_batch* b, const fa_paged_
     return fail(FA_ERR_ARG, "negative strides");
   const uintptr_t e = r->dtype == FA_BF16 ? 2 : 4;
   if (!aligned(r->keys, e) || !aligned(r->values, e)) return fail(FA_ERR_ARG, "misaligned rows");
+  if (written) FA_TRY(check_rows_out(c, b, r));
   FA_TRY(fa::host::pointer_on(r->keys, c->device, "keys of the rows"));
   FA_TRY(fa::host::pointer_on(r->values, c->device, "values of the rows"));
   return FA_OK;
@@ -422,7 +460,7 @@ int check_rows(const fa_paged_cache* c, const fa_paged_batch* b, const fa_paged_
 int fa_paged_write(const fa_paged_cache* cache, int32_t layer, const fa_paged_batch* batch,
                    const fa_paged_rows* rows, void* stream) {
   FA_TRY(check_call(cache, layer, batch));
-  FA_TRY(check_rows(cache, batch, rows));
+  FA_TRY(check_rows(cache, batch, rows, false));
   FA_TRY(check_pointers(cache, batch));
   int sms = 0;
   unsigned* err = nullptr;
@@ -449,7 +487,7 @@ int fa_paged_write(const fa_paged_cache* cache, int32_t layer, const fa_paged_ba
 int fa_paged_read(const fa_paged_cache* cache, int32_t layer, const fa_paged_batch* batch,
                   const fa_paged_rows* rows, void* stream) {
   FA_TRY(check_call(cache, layer, batch));
-  FA_TRY(check_rows(cache, batch, rows));
+  FA_TRY(check_rows(cache, batch, rows, true));
   FA_TRY(check_pointers(cache, batch));
   int sms = 0;
   unsigned* err = nullptr;

@@ -522,7 +522,9 @@ int fa_paged_write(const fa_paged_cache* cache, int32_t layer, const fa_paged_ba
 
 /* The batch's rows read back out of a layer's pages (KvCache::copy_rows over pages,
  * transformer.rs:221-239): the values that the pages stand for, in f32 or rounded to bf16. A batch
- * with firsts 0 and every position as a row reads whole sequences. */
+ * with firsts 0 and every position as a row reads whole sequences. The rows share no elements (strides
+ * by which they do, or keys and values that overlap in part, are FA_ERR_ARG); keys and values may be
+ * one array, which then holds the values. */
 int fa_paged_read(const fa_paged_cache* cache, int32_t layer, const fa_paged_batch* batch,
                   const fa_paged_rows* rows, void* stream);
 

@@ -360,3 +360,31 @@ def test_heads_of_zeros_beside_tiny_values(dims, rows):
     want, tol = reference(cache, 0, spans, q.double(), CAUSAL)
     up = 2.0 ** 30  # (values are off by at most 2^-58 besides)
     check_close(out.double() * up, want * up, tol * up + 2.0 ** -58 * up, False)
+
+
+# ---- layouts of rows ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [fa.Q8, fa.BF16], ids=["q8", "bf16"])
+def test_rows_read_into_one_array_of_keys_and_values(dtype):
+    """Keys and values side by side in each row of one array; one array for both holds the values;
+    rows that share elements are refused."""
+    torch = torch_()
+    spans = Spans([(30, 5), (1, 40)], 16)
+    cache = make_cache(fa.Shape(1, 8, 4, 128), spans, dtype)
+    batch = spans.batch(cache)
+    apart = torch.empty((2, spans.rows, 4, 128), device="cuda")
+    cache.read(0, batch, apart[0], apart[1])
+    both = torch.empty((spans.rows, 2, 4, 128), device="cuda")
+    cache.read(0, batch, both[:, 0], both[:, 1])
+    one = torch.empty((spans.rows, 4, 128), device="cuda")
+    cache.read(0, batch, one, one)
+    fa.device_status()
+    assert torch.equal(both.transpose(0, 1), apart) and torch.equal(one, apart[1])
+    for k, v in ((one[:, :1].expand(-1, 4, -1), apart[1][:, :1].expand(-1, 4, -1)),
+                 (one[:1].expand(spans.rows, -1, -1), apart[1][:1].expand(spans.rows, -1, -1)),
+                 (both[:-1].flatten(0, 1)[:spans.rows], both.flatten(0, 1)[1:1 + spans.rows])):
+        with pytest.raises(fa.FaError) as e:
+            cache.read(0, batch, k, v)
+        assert e.value.code == fa.ERR_ARG
+    cache.write(0, batch, apart[0][:1].expand(spans.rows, -1, -1), apart[1][:1].expand(spans.rows, -1, -1))
+    fa.device_status()
