@@ -676,6 +676,17 @@ def _angles(t, head_dim):
     return t.data_ptr()
 
 
+def _head_norm(norm, head_dim):
+    """(query weights, key weights, eps) as a fa_head_norm, or None: the kernels read head_dim f32 of
+    each."""
+    if norm is not None:
+        import torch
+        for t in norm[:2]:
+            if t is not None and (t.dtype != torch.float32 or t.shape != (head_dim,) or not t.is_contiguous()):
+                raise ValueError(f"norm weights: {head_dim} contiguous float32")
+    return _norm(norm)
+
+
 class PagedCache:
     """A KV cache in pages of one pool (fa_paged_cache): keys and values are device tensors
     [layers, pages, kv_heads, page_size, head_dim] of bf16 or (Q8) int8, with 8-bit pages beside
@@ -744,7 +755,7 @@ class PagedCache:
             raise ValueError("q_out has qkv's dtype")
         _check(lib().fa_attention_input_paged(
             self._ref, layer, batch._ref, rope if angles is not None else ROPE_NONE,
-            _angles(angles, self.shape.head_dim), _norm(norm), src, stride, dt, dst, q_stride,
+            _angles(angles, self.shape.head_dim), _head_norm(norm, self.shape.head_dim), src, stride, dt, dst, q_stride,
             self._on(stream)))
 
     def _rows(self, batch, keys, values):
@@ -783,7 +794,7 @@ class PagedCache:
         batch.covers(qkv, out, angles)
         _check(lib().fa_attention_paged(
             self._ref, layer, batch._ref, rope if angles is not None else ROPE_NONE,
-            _angles(angles, self.shape.head_dim), _norm(norm),
+            _angles(angles, self.shape.head_dim), _head_norm(norm, self.shape.head_dim),
             *_row_array(qkv, "qkv", self._qkv_width), *_row_array(out, "out", self._width),
             self._on(stream, batch)))
 

@@ -65,3 +65,28 @@ def test_overlaps_as_counted():
             rows, heads, rs, hs, apart)
         seen.add(want)
     assert seen == {True, False}
+
+
+def test_norm_weights_are_checked():
+    """Weights shorter than a head, of another type or with gaps are refused before the library (whose
+    kernels read head_dim floats) is called."""
+    import torch
+
+    pages = torch.zeros((1, 3, 2, 16, 64), dtype=torch.bfloat16)
+    cache = fa.PagedCache(fa.Shape(1, 4, 2, 64), 3, 16, fa.BF16, keys=pages, values=pages.clone())
+
+    class Batch:
+        _ref = None
+
+        def covers(self, *tensors):
+            pass
+
+    qkv, out, angles = torch.zeros((2, 512)), torch.zeros((2, 256)), torch.zeros((2, 64))
+    good = torch.ones(64)
+    for bad in (torch.ones(63), torch.ones(128), torch.ones(64).bfloat16(), torch.ones(64).double(),
+                torch.ones(128)[::2], torch.ones((1, 64)), torch.tensor(1.0)):
+        for norm in ((bad, good, 1e-6), (good, bad, 1e-6), (bad, None, 1e-6), (None, bad, 1e-6)):
+            with pytest.raises(ValueError, match="norm weights"):
+                cache.attention_input(0, Batch(), qkv, angles, norm=norm)
+            with pytest.raises(ValueError, match="norm weights"):
+                cache.attention(0, Batch(), qkv, out, angles, norm=norm)
