@@ -242,8 +242,11 @@ def test_no_rows_allowed_to_a_sequence(dtype):
 
 def eight_bit_reference(cache, spans, q, weighty):
     """Outputs of one sequence's causal rows in f64 and their bounds: test_paged_gpu.py's, with the
-    scores' errors taken over the keys that a row sees, or (weighty) over those that have a weight
-    in f64, and one more. The weights go into the products in f16, where those below 2^-14 are off by
+    scores' errors D taken over the keys that a row sees, or (weighty) over those that have a weight
+    in f64, and two changes. D is not small where a huge key is seen: numerator and sum are within
+    e^D of what they are without it, so every p_j is within e^(2 D) of it, and with weights and
+    values off by w an output by at most ((1 + w) e^(2 D) - 1) x sum_j p_j |v_j| (a row whose D is
+    large may give a huge key all of its weight or none: its bound says nothing). The weights go into the products in f16, where those below 2^-14 are off by
     at most 2^-25. The token kernel's weights carry their value's scale s_j and the largest is at
     least 2^6: each is off by at most 2^-31 of the largest p_j s_j. The chunk kernel's go with values
     whose scales are put into [2^8, 2^9), the largest of a tile (which here lie within 2^2 of each
@@ -268,7 +271,8 @@ def eight_bit_reference(cache, spans, q, weighty):
             qh.abs().amax(1, keepdim=True) @ kh.abs().sum(1)[None])
         off = torch.where(p > 0 if weighty else see, off / math.sqrt(d), 0.0).amax(1, keepdim=True)
         want[:, cols] = p @ vh
-        tol[:, cols] = (3 * 2.0 ** -11 + 2 * off + 1e-4) * (p @ vh.abs())
+        tol[:, cols] = ((1 + 3 * 2.0 ** -11 + 1e-4) * torch.exp(2 * off.clamp(max=100)) - 1) * (p @ vh.abs())
+        tol[:, cols][off.squeeze(1) > 100] = math.inf  # (e^200 of what p has lost below 1e-308, too)
         tol[:, cols] += end * 127 * 2.0 ** -29 * (p * scales[:, kv]).amax(1, keepdim=True)
     return want, tol
 
