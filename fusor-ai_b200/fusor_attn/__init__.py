@@ -238,6 +238,17 @@ def _stream_object(device, raw, stream):
     return stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(raw, device)
 
 
+def _capturing(device, raw, stream):
+    import torch
+    if _raw_stream(device) == raw and torch.cuda.current_device() == device:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.stream(stream):
+        return torch.cuda.is_current_stream_capturing()
+
+
+_made = {}  # (device, stream handle) -> an event after what handles made there last
+
+
 class _Owned:
     """Tensors that a handle allocates (and fills) on torch's current stream of `device`, for calls on
     any stream: one that has not used them yet waits for what was queued when they were made, and
@@ -248,20 +259,23 @@ class _Owned:
         import torch
         self.tensors = tensors
         home = torch.cuda.current_stream(device)
-        self.streams = {home.cuda_stream}
+        raw = home.cuda_stream
+        self.streams = {raw}
         self.made = None
-        with torch.cuda.stream(home):
-            if not torch.cuda.is_current_stream_capturing():
-                self.made = home.record_event()
+        if not _capturing(device, raw, home):
+            # (one event for all that is made on a stream: waiting for a later one waits longer)
+            self.made = _made.get((device, raw))
+            if self.made is None:
+                self.made = _made[device, raw] = torch.cuda.Event()
+            self.made.record(home)
 
     def on(self, device, raw, stream):
         if raw in self.streams:
             return
         import torch
         stream = _stream_object(device, raw, stream)
-        with torch.cuda.stream(stream):
-            if torch.cuda.is_current_stream_capturing():
-                return
+        if _capturing(device, raw, stream):
+            return
         if self.made is not None:
             stream.wait_event(self.made)
         for t in self.tensors:
