@@ -306,7 +306,9 @@ int attend(const fa_paged_cache* c, int layer, const fa_paged_batch* b, const vo
   // A batch may hold both kinds of sequences: each kernel leaves the other's alone. Where the
   // rows are as many as sequences of max_rows each make (a uniform batch, a single sequence) the
   // chunk kernel takes every sequence, and where no sequence has many rows the token kernel does:
-  // one launch.
+  // one launch. (The host knows no more of the rows: among chunks of unequal lengths the token kernel
+  // finds nothing to do, and padding rows that make up the product send single tokens to the chunk
+  // kernel, which is slower and as right.)
   const bool chunks = int64_t(b->max_rows) * a.group > a.token_cols;
   const bool tokens = !chunks || (a.group <= a.token_cols &&
                                   b->rows < int64_t(b->sequences) * b->max_rows);

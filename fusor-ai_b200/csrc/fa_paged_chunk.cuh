@@ -41,9 +41,10 @@
 // of them (0 x inf): the loaders take it out and mark its key, and the rows that see the key get
 // a NaN sum. Every wait is bounded (mbar_wait).
 //
-// Measured: 2048 rows after 14336 positions, 32/8 heads of 128 (515 GFLOP): 0.563 ms over bf16 pages
-// (916 TFLOP/s, the softmax and the handshakes between the roles), 0.758 ms over 8-bit pages (680
-// TFLOP/s: the conversion next to it; 56 % of the shared memory's bandwidth, tensor pipe 31 %). Five
+// Measured: 2048 rows after 14336 positions, 32/8 heads of 128 (515 GFLOP): 0.569 ms over bf16 pages
+// (905 TFLOP/s, the softmax and the handshakes between the roles; one tile at a time on its way), 0.789
+// ms over 8-bit pages (653 TFLOP/s: the conversion next to it; 54 % of the load/store data path, tensor
+// pipe 31 %; 2.7 ms if every tile's scales lie far apart: such a tile's softmax is a rolled loop). Five
 // chunks of 100 to 999 rows under a window of 1024, 8/2 heads of 256: 98 us, shares of about 12
 // tiles a CTA whose fixed costs (plan 6-9 thousand cycles, queries 4-16, merge 20) weigh as much.
 #pragma once

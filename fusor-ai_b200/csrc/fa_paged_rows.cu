@@ -123,7 +123,10 @@ __device__ __forceinline__ uint32_t pack_bytes(int a, int b, int c, int d) {
 // Bound by issued instructions (80 % of the cycles of a long call) with memory close behind, so each
 // kind has a loop of its own, and calls whose arrays are all 16-byte aligned have a kernel without
 // the element-wise accesses (Vec): 8500 rows of 32/8 heads of 128 (bf16 rows, 8-bit pages, 196 MB)
-// take 44 us (4.4 TB/s), 51 us in one loop of all kinds that tests the alignment.
+// take 42 us (4.7 TB/s), 51 us in one loop of all kinds that tests the alignment; 2800 f32 rows of
+// 8/2 heads of 256 with head norms into bf16 pages 16 us; the keys and values alone, as they are, of
+// 8500 rows 20 us. The arithmetic is one f32 at a time, and 40 registers (12 CTAs an SM) spill 12 to 48
+// bytes of stores in every instantiation.
 template <typename T, int D, bool Vec>
 __global__ void __launch_bounds__(kRowWarps * 32, 12)
     paged_write_kernel(const __grid_constant__ PagedWriteArgs a) {
@@ -263,8 +266,11 @@ __global__ void __launch_bounds__(kRowWarps * 32, 12)
 }
 
 // A warp takes two rows: their places, then 16 bytes of them a lane at a time, eight such loads in
-// flight (two vectors of keys and of values of each row). Bound by memory: 125 thousand positions of
-// 8 KV heads of 128 out of 8-bit pages to bf16 rows (780 MB) take 162 us, 4.8 TB/s.
+// flight (two vectors of keys and of values of each row). 125 thousand positions of 8 KV heads of 128
+// to bf16 rows take 159 us out of bf16 pages (1029 MB, 6.5 TB/s: the rate of a copy) and 161 us out
+// of 8-bit pages (780 MB, 4.8 TB/s: a lane stores 32 bytes in two vectors, so that each store
+// instruction of a warp writes half of every sector that it touches; so do bf16 pages to f32 rows,
+// at 5.7 TB/s).
 constexpr int kReadWarps = 8, kReadRows = 2 * kReadWarps;
 
 template <bool Q8, int D>

@@ -535,7 +535,10 @@ int fa_paged_read(const fa_paged_cache* cache, int32_t layer, const fa_paged_bat
  * call. Queries and probabilities are rounded to 16 bits for the tensor cores, scores, sums and
  * outputs accumulated in f32. A row that sees no position (its pages out of range) is zero. A value
  * that is not finite reaches the rows that see its position, whose elements may all become NaN,
- * and no others. Value scales are to be below 2^70 (larger ones may lose smaller values' weights). */
+ * and no others. Value scales are to be below 2^70 (larger ones may lose smaller values' weights).
+ * Over 8-bit pages the weights are in f16 below the row's largest weighted value: each position may
+ * leave an element off by 2^-22 of the row's largest p_j x 127 scale_j besides. Keys and values of any
+ * sizes beside one another keep their precision otherwise. */
 int fa_attend_paged(const fa_paged_cache* cache, int32_t layer, const fa_paged_batch* batch,
                     const void* q, int64_t q_stride, int32_t dtype, void* out,
                     int64_t out_stride, int32_t out_dtype, void* stream);
@@ -547,8 +550,8 @@ int fa_attention_paged(const fa_paged_cache* cache, int32_t layer, const fa_page
                        const void* qkv, int64_t qkv_stride, int32_t dtype, void* out,
                        int64_t out_stride, int32_t out_dtype, void* stream);
 
-/* Waits for `stream` and reports whether any kernel of this library gave up a device-side wait
- * since the last call (FA_ERR_TIMEOUT, clearing the flag), whether a paged call met spans
+/* Waits for `stream` and reports whether any kernel of this library on the current device gave up a
+ * device-side wait since the last call (FA_ERR_TIMEOUT, clearing the flag), whether a paged call met spans
  * (FA_ERR_CAPACITY) or page ids (FA_ERR_ARG) out of range, or FA_OK. */
 int fa_device_status(void* stream);
 

@@ -246,8 +246,8 @@ def eight_bit_reference(cache, spans, q, weighty):
     in f64, and two changes. D is not small where a huge key is seen: numerator and sum are within
     e^D of what they are without it, so every p_j is within e^(2 D) of it, and with weights and
     values off by w an output by at most ((1 + w) e^(2 D) - 1) x sum_j p_j |v_j| (a row whose D is
-    large may give a huge key all of its weight or none: its bound says nothing). The weights go into the products in f16, where those below 2^-14 are off by
-    at most 2^-25. The token kernel's weights carry their value's scale s_j and the largest is at
+    large may give a huge key all of its weight or none: its bound says nothing). The weights go into
+    the products in f16, where those below 2^-14 are off by at most 2^-25. The token kernel's weights carry their value's scale s_j and the largest is at
     least 2^6: each is off by at most 2^-31 of the largest p_j s_j. The chunk kernel's go with values
     whose scales are put into [2^8, 2^9), the largest of a tile (which here lie within 2^2 of each
     other, or have units of their own) or each its own: the largest weight is at least 2^7 and its
